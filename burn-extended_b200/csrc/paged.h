@@ -1,0 +1,112 @@
+// paged.h -- what the paged key-value cache's entry points (paged_api.cu) and
+// kernels (paged_append.cu, paged_decode.cu, paged_evict.cu) share.
+//
+// Keys and values lie in pools [n_pages][kv_heads][page_size][head_dim]; the
+// cache index n of a sequence is slot n % page_size of the page that its table
+// row names at n / page_size.  Every kernel checks table entries, indexes and
+// positions against these bounds before it forms an address: what is out of
+// range is skipped (a read gives zero) and leaves its bit in the status word.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace mxmoe {
+
+// Bits of the cache's status word.
+constexpr int kPagedBadPage = 1;      // a table entry outside [0, n_pages)
+constexpr int kPagedBadIndex = 2;     // a cache index, length or row outside its table
+constexpr int kPagedBadPosition = 4;  // a position outside the rotary table
+
+struct PagedView {
+  void* k;
+  void* v;
+  const float* k_scale;  // [kv_heads] (8-bit cache) or null: 1
+  const float* v_scale;
+  float* weight;      // [n_pages][kv_heads][page_size] or null
+  int32_t* position;  // the same shape, or null
+  int* status;
+  int n_pages, page_size, n_heads, kv_heads, head_dim, dtype;
+  uint32_t page_mul, page_shift;  // n / page_size = umulhi(n, page_mul) >> page_shift for 0 <= n < 2^31
+};
+
+struct PagedTables {
+  const int32_t* tables;  // [n_rows][max_pages], rows `stride` apart
+  int64_t stride;
+  int n_rows, max_pages;
+};
+
+struct AppendParams {
+  PagedView c;
+  PagedTables t;
+  const void *q, *k, *v;  // [tokens][heads][head_dim], strides in elements
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  void *q_out, *k_out;
+  int64_t qo_token, qo_head, ko_token, ko_head;
+  int dtype, tokens;
+  const int32_t *rows, *index, *positions;
+  const float *cos, *sin;  // [n_positions][rot / 2]
+  int rot, n_positions, interleaved;
+  float sign;  // -1: the inverse rotation
+};
+
+struct DecodeParams {
+  PagedView c;
+  PagedTables t;
+  const void* q;
+  int64_t q_row, q_head;
+  int q_dtype;
+  void* out;
+  int64_t out_row, out_head;
+  int out_dtype;
+  float* lse;  // [rows][n_heads] or null
+  int rows;
+  const int32_t* lens;
+  float scale;
+  int window;
+  const float* sinks;
+  int quiet;
+  const float* bias;  // [rows][n_heads][bias_len] by strides, or null
+  int64_t bias_row, bias_head;
+  int bias_len;
+  int track;
+};
+
+struct EvictParams {
+  PagedView c;
+  PagedTables t;
+  int rows;
+  const int32_t *lens, *seen;
+  int32_t* new_lens;
+  int budget, sink, recent;
+};
+
+cudaError_t launch_paged_append(const AppendParams& p, cudaStream_t st);
+cudaError_t launch_paged_decode(const DecodeParams& p, cudaStream_t st);
+cudaError_t launch_paged_evict(const EvictParams& p, cudaStream_t st);
+cudaError_t launch_rotary_table(const double* inv_freq, int half, int64_t first, int n, double factor, float* cos,
+                                float* sin, cudaStream_t st);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int page_of(const PagedView& c, int n) {
+  return c.page_mul ? static_cast<int>(__umulhi(static_cast<uint32_t>(n), c.page_mul) >> c.page_shift) : n;
+}
+
+// The slot of cache index n of a table row: (page * kv_heads + 0) * page_size + n % page_size, head h's is
+// page_size * h further.  -1 where the table has none.
+__device__ __forceinline__ int64_t slot_of(const PagedView& c, const PagedTables& t, int row, int n) {
+  const int pi = page_of(c, n);
+  if (n < 0 || pi >= t.max_pages) {
+    atomicOr(c.status, kPagedBadIndex);
+    return -1;
+  }
+  const int page = __ldg(t.tables + row * t.stride + pi);
+  if (page < 0 || page >= c.n_pages) {
+    atomicOr(c.status, kPagedBadPage);
+    return -1;
+  }
+  return static_cast<int64_t>(page) * c.kv_heads * c.page_size + (n - pi * c.page_size);
+}
+#endif
+
+}  // namespace mxmoe

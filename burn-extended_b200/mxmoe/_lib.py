@@ -13,7 +13,7 @@ STATUS_NAMES = {
     0: "OK", 1: "INVALID_ARG", 2: "NOT_READY", 3: "CUDA", 4: "OOM",
     5: "UNSUPPORTED", 6: "TIMEOUT", 7: "TOO_LARGE",
 }
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2
 
 FLAG_INTERLEAVED_GLU = 0x1
 FLAG_BIAS_PER_FTILE = 0x2
@@ -76,6 +76,64 @@ _vp = ctypes.c_void_p
 _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
 _i32 = ctypes.c_int
+
+
+class PagedConfig(ctypes.Structure):
+    """mxmqa_paged_config"""
+    _fields_ = [("n_pages", _u32), ("page_size", _u32), ("n_heads", _u32), ("kv_heads", _u32), ("head_dim", _u32),
+                ("dtype", _u32), ("device", ctypes.c_int32)]
+
+
+class PagedBuffers(ctypes.Structure):
+    """mxmqa_paged_buffers"""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("weight", _vp), ("position", _vp)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """mxmqa_paged_append_args"""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_token", ctypes.c_int64), ("q_head", ctypes.c_int64),
+                ("k_token", ctypes.c_int64), ("k_head", ctypes.c_int64), ("v_token", ctypes.c_int64),
+                ("v_head", ctypes.c_int64), ("q_out", _vp), ("q_out_token", ctypes.c_int64),
+                ("q_out_head", ctypes.c_int64), ("k_out", _vp), ("k_out_token", ctypes.c_int64),
+                ("k_out_head", ctypes.c_int64), ("dtype", _u32), ("tokens", _u32), ("tables", _vp),
+                ("table_stride", ctypes.c_int64), ("n_rows", _u32), ("max_pages", _u32), ("rows", _vp),
+                ("index", _vp), ("positions", _vp), ("cos", _vp), ("sin", _vp), ("rot_dim", _u32),
+                ("n_positions", _u32), ("interleaved", _u32)]
+
+
+class PagedDecodeArgs(ctypes.Structure):
+    """mxmqa_paged_decode_args"""
+    _fields_ = [("q", _vp), ("q_row", ctypes.c_int64), ("q_head", ctypes.c_int64), ("out", _vp),
+                ("out_row", ctypes.c_int64), ("out_head", ctypes.c_int64), ("lse", _vp), ("q_dtype", _u32),
+                ("out_dtype", _u32), ("rows", _u32), ("max_pages", _u32), ("tables", _vp),
+                ("table_stride", ctypes.c_int64), ("lens", _vp), ("scale", ctypes.c_float), ("window", _u32),
+                ("sinks", _vp), ("bias", _vp), ("bias_row", ctypes.c_int64), ("bias_head", ctypes.c_int64),
+                ("bias_len", _u32), ("quiet", _u32), ("track", _u32)]
+
+
+class PagedEvictArgs(ctypes.Structure):
+    """mxmqa_paged_evict_args"""
+    _fields_ = [("tables", _vp), ("table_stride", ctypes.c_int64), ("rows", _u32), ("max_pages", _u32),
+                ("lens", _vp), ("seen", _vp), ("new_lens", _vp), ("budget", _u32), ("sink", _u32),
+                ("recent", _u32)]
+
+
+class RotaryTableConfig(ctypes.Structure):
+    """mxmqa_rotary_config"""
+    _fields_ = [("rot_dim", _u32), ("scaling", _u32), ("theta", ctypes.c_float),
+                ("scaling_factor", ctypes.c_float), ("initial_context", ctypes.c_float),
+                ("ntk_alpha", ctypes.c_float), ("ntk_beta", ctypes.c_float)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """mxmqa_rotary_args"""
+    _fields_ = [("x", _vp), ("x_token", ctypes.c_int64), ("x_head", ctypes.c_int64), ("out", _vp),
+                ("out_token", ctypes.c_int64), ("out_head", ctypes.c_int64), ("dtype", _u32), ("tokens", _u32),
+                ("heads", _u32), ("head_dim", _u32), ("positions", _vp), ("cos", _vp), ("sin", _vp),
+                ("rot_dim", _u32), ("n_positions", _u32), ("interleaved", _u32), ("inverse", _u32),
+                ("device", ctypes.c_int32)]
+
+
 _SIGS = {
     "mxmoe_abi_version": ([], _i32),
     "mxmoe_build_info": ([], ctypes.c_char_p),
@@ -110,6 +168,14 @@ _SIGS = {
     "mxmqa_cache_state": ([_vp, ctypes.POINTER(_u64), ctypes.POINTER(_u64)], _i32),
     "mxmqa_cache_destroy": ([_vp], _i32),
     "mxmqa_forward_streaming": ([_vp, _vp, _vp, _i32, _u32, _u32, _u64, _u32, _vp, _vp, _vp, _i32, _vp], _i32),
+    "mxmqa_paged_create": ([ctypes.POINTER(PagedConfig), ctypes.POINTER(PagedBuffers), ctypes.POINTER(_vp)], _i32),
+    "mxmqa_paged_destroy": ([_vp], _i32),
+    "mxmqa_paged_status": ([_vp, _vp], _i32),
+    "mxmqa_paged_append": ([_vp, ctypes.POINTER(PagedAppendArgs), _vp], _i32),
+    "mxmqa_paged_decode": ([_vp, ctypes.POINTER(PagedDecodeArgs), _vp], _i32),
+    "mxmqa_paged_evict": ([_vp, ctypes.POINTER(PagedEvictArgs), _vp], _i32),
+    "mxmqa_rotary_table": ([ctypes.POINTER(RotaryTableConfig), _u32, _u32, _vp, _vp, ctypes.c_int32, _vp], _i32),
+    "mxmqa_rotary": ([ctypes.POINTER(RotaryArgs), _vp], _i32),
     "mxmoe_last_profile": ([_vp, ctypes.POINTER(ctypes.c_float), _i32, ctypes.POINTER(_i32)], _i32),
     "mxmoe_route": ([_vp, _vp, _i32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _i32),
     "mxmoe_gather_pairs": ([_vp, _i32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _i32),

@@ -44,7 +44,8 @@ typedef enum mxmoe_status {
 /* Element types of activation / bias buffers. */
 typedef enum mxmoe_dtype {
   MXMOE_F32 = 0,
-  MXMOE_BF16 = 1
+  MXMOE_BF16 = 1,
+  MXMOE_E4M3 = 2 /* paged caches only */
 } mxmoe_dtype;
 
 /* Behaviour flags (mxmoe_config.flags). */
@@ -605,6 +606,186 @@ MXMOE_API int mxmqa_forward_streaming(mxmqa_layer* layer, mxmqa_cache* cache, co
                                       uint64_t start_pos, uint32_t window, const float* sinks,
                                       const float* attn_bias, void* y, mxmoe_dtype y_dtype,
                                       void* stream);
+
+/* ---- paged key-value cache ----
+ *
+ * One pool of pages that many sequences share: keys and values lie in
+ * [n_pages][kv_heads][page_size][head_dim]; a sequence is a row of page
+ * numbers, and its cache index n is slot n % page_size of page
+ * tables[row][n / page_size].  Three calls work on it:
+ *   append  rotary positions on new queries and keys, keys and values into
+ *           their pages;
+ *   decode  attention of one new token per row over its cached tokens,
+ *           optionally adding every token's share to its weight;
+ *   evict   the tokens of least weight leave, survivors take their places.
+ * All buffers are the caller's device memory.  Calls are stream-ordered,
+ * asynchronous and may be captured in a CUDA graph (they allocate nothing); a
+ * cache serves one stream at a time, as a layer does.  A table entry, index,
+ * length or position out of range is skipped on the device and reported by
+ * mxmqa_paged_status. */
+typedef struct mxmqa_paged_config {
+  uint32_t n_pages;
+  uint32_t page_size;  /* tokens per page, any size up to 65536 */
+  uint32_t n_heads;    /* query heads, at most 1024; n_heads % kv_heads == 0 */
+  uint32_t kv_heads;
+  uint32_t head_dim;   /* a multiple of 8 (16 in an 8-bit cache), at most 256 */
+  uint32_t dtype;      /* mxmoe_dtype of the cached keys and values */
+  int32_t device;
+} mxmqa_paged_config;
+
+typedef struct mxmqa_paged_buffers {
+  void* k;              /* [n_pages][kv_heads][page_size][head_dim], 16-byte aligned */
+  void* v;
+  const float* k_scale; /* [kv_heads]: an 8-bit key stands for code x scale; NULL: 1 */
+  const float* v_scale;
+  float* weight;        /* [n_pages][kv_heads][page_size], for track and evict; may be NULL */
+  int32_t* position;    /* the same shape, for evict; may be NULL */
+} mxmqa_paged_buffers;
+
+typedef struct mxmqa_paged_cache mxmqa_paged_cache;
+
+/* The buffers must outlive the handle; their contents are left as they are. */
+MXMOE_API int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers* buffers,
+                                 mxmqa_paged_cache** out);
+MXMOE_API int mxmqa_paged_destroy(mxmqa_paged_cache* cache);
+/* Waits for the stream; MXMOE_ERR_INVALID_ARG when a call since the last one
+ * met something out of range, and clears that. */
+MXMOE_API int mxmqa_paged_status(mxmqa_paged_cache* cache, void* stream);
+
+/* Strides are in elements.  q_out may be q (rotation in place), k_out k. */
+typedef struct mxmqa_paged_append_args {
+  const void* q;  /* [tokens][n_heads][head_dim], or NULL with q_out: keys and values only */
+  const void* k;  /* [tokens][kv_heads][head_dim] */
+  const void* v;
+  int64_t q_token;
+  int64_t q_head;
+  int64_t k_token;
+  int64_t k_head;
+  int64_t v_token;
+  int64_t v_head;
+  void* q_out;    /* rotated queries */
+  int64_t q_out_token;
+  int64_t q_out_head;
+  void* k_out;    /* rotated keys beside those in the cache, or NULL */
+  int64_t k_out_token;
+  int64_t k_out_head;
+  uint32_t dtype; /* of q, k, v, q_out and k_out: MXMOE_F32 or MXMOE_BF16 */
+  uint32_t tokens;
+  const int32_t* tables;    /* [n_rows][max_pages] */
+  int64_t table_stride;
+  uint32_t n_rows;
+  uint32_t max_pages;
+  const int32_t* rows;      /* [tokens] table row of a token; NULL: token t is row t */
+  const int32_t* index;     /* [tokens] cache index; negative: rotated, not written */
+  const int32_t* positions; /* [tokens]; NULL: the cache index */
+  const float* cos;         /* [n_positions][rot_dim / 2], mxmqa_rotary_table */
+  const float* sin;
+  uint32_t rot_dim;         /* leading columns that rotate; 0: none */
+  uint32_t n_positions;
+  uint32_t interleaved;     /* pairs (2i, 2i + 1) instead of (i, i + rot_dim / 2) */
+} mxmqa_paged_append_args;
+
+/* Two tokens of one call must not name the same slot.  Where the cache has
+ * them, the slot's weight becomes 0 and its position the token's. */
+MXMOE_API int mxmqa_paged_append(mxmqa_paged_cache* cache, const mxmqa_paged_append_args* args, void* stream);
+
+typedef struct mxmqa_paged_decode_args {
+  const void* q;         /* [rows][n_heads][head_dim], strides in elements */
+  int64_t q_row;
+  int64_t q_head;
+  void* out;             /* the same shape */
+  int64_t out_row;
+  int64_t out_head;
+  float* lse;            /* [rows][n_heads] log of the softmax's normalizer, or NULL */
+  uint32_t q_dtype;      /* MXMOE_F32 or MXMOE_BF16 */
+  uint32_t out_dtype;
+  uint32_t rows;
+  uint32_t max_pages;
+  const int32_t* tables; /* [rows][max_pages] */
+  int64_t table_stride;  /* 0: one table for all rows */
+  const int32_t* lens;   /* [rows] cached tokens, the new one among them; 0: the row gives zeros */
+  float scale;           /* on q . k, 1 / sqrt(head_dim) as a rule */
+  uint32_t window;       /* the last `window` tokens only; 0: all */
+  const float* sinks;    /* [n_heads] logits that join the normalizer, or NULL */
+  const float* bias;     /* [rows][n_heads][bias_len] added to the scores, or NULL */
+  int64_t bias_row;
+  int64_t bias_head;     /* 0: one bias for all heads */
+  uint32_t bias_len;     /* cache indexes from here on have no bias */
+  uint32_t quiet;        /* 1 joins the normalizer (quiet softmax) */
+  uint32_t track;        /* adds each token's share to its weight; window 0, no page in two rows */
+} mxmqa_paged_decode_args;
+
+/* The rows of a call may share pages (a common prefix, or several new tokens
+ * of one sequence as rows of their own with rising lens), except with track. */
+MXMOE_API int mxmqa_paged_decode(mxmqa_paged_cache* cache, const mxmqa_paged_decode_args* args, void* stream);
+
+typedef struct mxmqa_paged_evict_args {
+  const int32_t* tables; /* [rows][max_pages]; no page in two rows */
+  int64_t table_stride;
+  uint32_t rows;
+  uint32_t max_pages;
+  const int32_t* lens;   /* [rows] cached tokens */
+  const int32_t* seen;   /* [rows] tokens of the sequence so far: one above its newest position */
+  int32_t* new_lens;     /* [rows] min(lens, budget); may be lens */
+  uint32_t budget;       /* tokens that stay */
+  uint32_t sink;         /* positions below this stay */
+  uint32_t recent;       /* positions from seen - recent on stay; sink + recent <= budget */
+} mxmqa_paged_evict_args;
+
+/* Of a row with more than `budget` tokens the lowest by (protected, weight,
+ * cache index) leave, each key head its own; a NaN weight counts as +inf.  The
+ * i-th of them below the budget is overwritten by the i-th survivor at or above
+ * it; slots from the budget on keep their contents.  Cache indexes are not in
+ * the order of positions afterwards. */
+MXMOE_API int mxmqa_paged_evict(mxmqa_paged_cache* cache, const mxmqa_paged_evict_args* args, void* stream);
+
+/* How rotary frequencies theta^(-2i / rot_dim) are scaled for long contexts. */
+#define MXMQA_ROTARY_PLAIN 0u
+#define MXMQA_ROTARY_LINEAR 1u    /* divided by scaling_factor */
+#define MXMQA_ROTARY_NTK 2u       /* base x scaling_factor^(rot_dim / (rot_dim - 2)) */
+#define MXMQA_ROTARY_YARN 3u      /* low frequencies divided, a ramp between ntk_alpha and ntk_beta turns within
+                                     initial_context, cos and sin x (0.1 ln scaling_factor + 1) */
+#define MXMQA_ROTARY_STREAMING 4u /* the interpolation of mxmqa_set_rope, for caches beside that step */
+
+typedef struct mxmqa_rotary_config {
+  uint32_t rot_dim;      /* even, at most 256 */
+  uint32_t scaling;      /* MXMQA_ROTARY_* */
+  float theta;
+  float scaling_factor;
+  float initial_context;
+  float ntk_alpha;
+  float ntk_beta;
+} mxmqa_rotary_config;
+
+/* cos, sin: device [n][rot_dim / 2] for positions first .. first + n - 1. */
+MXMOE_API int mxmqa_rotary_table(const mxmqa_rotary_config* cfg, uint32_t first, uint32_t n, float* cos,
+                                 float* sin, int32_t device, void* stream);
+
+/* The rotation alone: x [tokens][heads][head_dim] to out (which may be x), at
+ * positions [tokens].  inverse turns back, which is also the gradient. */
+typedef struct mxmqa_rotary_args {
+  const void* x;
+  int64_t x_token;
+  int64_t x_head;
+  void* out;
+  int64_t out_token;
+  int64_t out_head;
+  uint32_t dtype;
+  uint32_t tokens;
+  uint32_t heads;
+  uint32_t head_dim;
+  const int32_t* positions;
+  const float* cos;
+  const float* sin;
+  uint32_t rot_dim;
+  uint32_t n_positions;
+  uint32_t interleaved;
+  uint32_t inverse;
+  int32_t device;
+} mxmqa_rotary_args;
+
+/* A position outside the table turns as position 0. */
+MXMOE_API int mxmqa_rotary(const mxmqa_rotary_args* args, void* stream);
 
 #ifdef __cplusplus
 }

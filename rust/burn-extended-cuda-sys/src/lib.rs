@@ -23,6 +23,14 @@ pub const MXMOE_ERR_TOO_LARGE: mxmoe_status = 7;
 pub type mxmoe_dtype = c_int;
 pub const MXMOE_F32: mxmoe_dtype = 0;
 pub const MXMOE_BF16: mxmoe_dtype = 1;
+/// Paged caches only.
+pub const MXMOE_E4M3: mxmoe_dtype = 2;
+
+pub const MXMQA_ROTARY_PLAIN: u32 = 0;
+pub const MXMQA_ROTARY_LINEAR: u32 = 1;
+pub const MXMQA_ROTARY_NTK: u32 = 2;
+pub const MXMQA_ROTARY_YARN: u32 = 3;
+pub const MXMQA_ROTARY_STREAMING: u32 = 4;
 
 pub const MXMOE_FLAG_INTERLEAVED_GLU: u32 = 0x1;
 pub const MXMOE_FLAG_BIAS_PER_FTILE: u32 = 0x2;
@@ -139,6 +147,154 @@ pub struct mxmqa_layer {
 #[repr(C)]
 pub struct mxmqa_cache {
     _private: [u8; 0],
+}
+
+/// Opaque paged key-value cache handle.
+#[repr(C)]
+pub struct mxmqa_paged_cache {
+    _private: [u8; 0],
+}
+
+/// Shape of a paged key-value cache.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mxmqa_paged_config {
+    pub n_pages: u32,
+    pub page_size: u32,
+    pub n_heads: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub dtype: u32,
+    pub device: i32,
+}
+
+/// The caller's device memory behind a paged cache.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mxmqa_paged_buffers {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scale: *const f32,
+    pub v_scale: *const f32,
+    pub weight: *mut f32,
+    pub position: *mut i32,
+}
+
+/// Arguments of `mxmqa_paged_append`; strides in elements.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mxmqa_paged_append_args {
+    pub q: *const c_void,
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub q_token: i64,
+    pub q_head: i64,
+    pub k_token: i64,
+    pub k_head: i64,
+    pub v_token: i64,
+    pub v_head: i64,
+    pub q_out: *mut c_void,
+    pub q_out_token: i64,
+    pub q_out_head: i64,
+    pub k_out: *mut c_void,
+    pub k_out_token: i64,
+    pub k_out_head: i64,
+    pub dtype: u32,
+    pub tokens: u32,
+    pub tables: *const i32,
+    pub table_stride: i64,
+    pub n_rows: u32,
+    pub max_pages: u32,
+    pub rows: *const i32,
+    pub index: *const i32,
+    pub positions: *const i32,
+    pub cos: *const f32,
+    pub sin: *const f32,
+    pub rot_dim: u32,
+    pub n_positions: u32,
+    pub interleaved: u32,
+}
+
+/// Arguments of `mxmqa_paged_decode`; strides in elements.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mxmqa_paged_decode_args {
+    pub q: *const c_void,
+    pub q_row: i64,
+    pub q_head: i64,
+    pub out: *mut c_void,
+    pub out_row: i64,
+    pub out_head: i64,
+    pub lse: *mut f32,
+    pub q_dtype: u32,
+    pub out_dtype: u32,
+    pub rows: u32,
+    pub max_pages: u32,
+    pub tables: *const i32,
+    pub table_stride: i64,
+    pub lens: *const i32,
+    pub scale: f32,
+    pub window: u32,
+    pub sinks: *const f32,
+    pub bias: *const f32,
+    pub bias_row: i64,
+    pub bias_head: i64,
+    pub bias_len: u32,
+    pub quiet: u32,
+    pub track: u32,
+}
+
+/// Arguments of `mxmqa_paged_evict`.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mxmqa_paged_evict_args {
+    pub tables: *const i32,
+    pub table_stride: i64,
+    pub rows: u32,
+    pub max_pages: u32,
+    pub lens: *const i32,
+    pub seen: *const i32,
+    pub new_lens: *mut i32,
+    pub budget: u32,
+    pub sink: u32,
+    pub recent: u32,
+}
+
+/// Frequencies of a rotary table (`MXMQA_ROTARY_*`).
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mxmqa_rotary_config {
+    pub rot_dim: u32,
+    pub scaling: u32,
+    pub theta: f32,
+    pub scaling_factor: f32,
+    pub initial_context: f32,
+    pub ntk_alpha: f32,
+    pub ntk_beta: f32,
+}
+
+/// Arguments of `mxmqa_rotary`.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mxmqa_rotary_args {
+    pub x: *const c_void,
+    pub x_token: i64,
+    pub x_head: i64,
+    pub out: *mut c_void,
+    pub out_token: i64,
+    pub out_head: i64,
+    pub dtype: u32,
+    pub tokens: u32,
+    pub heads: u32,
+    pub head_dim: u32,
+    pub positions: *const i32,
+    pub cos: *const f32,
+    pub sin: *const f32,
+    pub rot_dim: u32,
+    pub n_positions: u32,
+    pub interleaved: u32,
+    pub inverse: u32,
+    pub device: i32,
 }
 
 extern "C" {
@@ -450,6 +606,38 @@ extern "C" {
         y_dtype: mxmoe_dtype,
         stream: *mut c_void,
     ) -> c_int;
+    pub fn mxmqa_paged_create(
+        cfg: *const mxmqa_paged_config,
+        buffers: *const mxmqa_paged_buffers,
+        out: *mut *mut mxmqa_paged_cache,
+    ) -> c_int;
+    pub fn mxmqa_paged_destroy(cache: *mut mxmqa_paged_cache) -> c_int;
+    pub fn mxmqa_paged_status(cache: *mut mxmqa_paged_cache, stream: *mut c_void) -> c_int;
+    pub fn mxmqa_paged_append(
+        cache: *mut mxmqa_paged_cache,
+        args: *const mxmqa_paged_append_args,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn mxmqa_paged_decode(
+        cache: *mut mxmqa_paged_cache,
+        args: *const mxmqa_paged_decode_args,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn mxmqa_paged_evict(
+        cache: *mut mxmqa_paged_cache,
+        args: *const mxmqa_paged_evict_args,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn mxmqa_rotary_table(
+        cfg: *const mxmqa_rotary_config,
+        first: u32,
+        n: u32,
+        cos: *mut f32,
+        sin: *mut f32,
+        device: i32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn mxmqa_rotary(args: *const mxmqa_rotary_args, stream: *mut c_void) -> c_int;
 }
 
 /// The CUDA runtime calls the safe crate uses for its device buffers (the
