@@ -81,8 +81,24 @@ struct EvictParams {
   int budget, sink, recent;
 };
 
+constexpr int kDecodeTile = 16;       // keys per tile
+constexpr int kDecodeMaxRows = 1024;  // rows per launch: their prefix sums lie in shared memory
+constexpr int kDecodeHeads = 8;       // query heads of a segment
+constexpr int kDecodeWarps = 8;       // of a block, at most
+
+// Device memory that decode needs beside its arguments.
+struct DecodeScratch {
+  float* part;    // [2 * workers][8 * (head_dim + 2)] partial outputs, maxima and sums
+  int* tickets;   // [workers], zero between calls
+  float* scores;  // [score_tiles][32 lanes][4] (track)
+  int64_t score_tiles;
+  float* lse;  // [kDecodeMaxRows][n_heads] (track)
+};
+
 cudaError_t launch_paged_append(const AppendParams& p, cudaStream_t st);
-cudaError_t launch_paged_decode(const DecodeParams& p, cudaStream_t st);
+cudaError_t launch_paged_decode(const DecodeParams& p, const DecodeScratch& ws, int sms, cudaStream_t st);
+size_t decode_part_floats(const PagedView& c, int sms);  // of DecodeScratch::part
+int decode_workers(const PagedView& c, int sms);         // of DecodeScratch::tickets
 cudaError_t launch_paged_evict(const EvictParams& p, cudaStream_t st);
 cudaError_t launch_rotary_table(const double* inv_freq, int half, int64_t first, int n, double factor, float* cos,
                                 float* sin, cudaStream_t st);

@@ -21,6 +21,8 @@ int set_last_error(int code, const char* msg);  // api.cu
 struct mxmqa_paged_cache {
   mxmqa_paged_config cfg{};
   mxmoe::PagedView view{};
+  mxmoe::DecodeScratch scratch{};
+  int sms = 148;
 };
 
 namespace {
@@ -55,6 +57,17 @@ struct PDevice {
     if (prev >= 0) cudaSetDevice(prev);
   }
 };
+
+template <typename T>
+int palloc(T** p, size_t n, bool zero) {
+  const cudaError_t e = cudaMalloc(reinterpret_cast<void**>(p), n * sizeof(T));
+  if (e != cudaSuccess) {
+    *p = nullptr;
+    return pfail(MXMOE_ERR_OOM, "cudaMalloc(%zu bytes): %s", n * sizeof(T), cudaGetErrorString(e));
+  }
+  if (zero) P_CUDA(cudaMemset(*p, 0, n * sizeof(T)));
+  return MXMOE_OK;
+}
 
 constexpr uint64_t kMaxTokens = 0x7FFFFFFFu;
 
@@ -173,11 +186,25 @@ int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers*
     w.page_shift = l - 1;
   }
   PDevice g(cfg->device);
-  int rc = MXMOE_OK;
-  if (cudaMalloc(reinterpret_cast<void**>(&w.status), sizeof(int)) != cudaSuccess)
-    rc = pfail(MXMOE_ERR_OOM, "cudaMalloc of the status word failed");
-  else if (cudaMemset(w.status, 0, sizeof(int)) != cudaSuccess)
-    rc = pfail(MXMOE_ERR_CUDA, "cudaMemset of the status word failed");
+  if (cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, cfg->device) != cudaSuccess || c->sms < 1) {
+    cudaGetLastError();
+    delete c;
+    return pfail(MXMOE_ERR_CUDA, "device %d is not available", cfg->device);
+  }
+  // Everything that the calls need is allocated here, once: a tracked decode
+  // keeps the scores of every cached token (32 bytes per token, key head and 8
+  // query heads).
+  mxmoe::DecodeScratch& ws = c->scratch;
+  const size_t group = cfg->n_heads / cfg->kv_heads, segs = cfg->kv_heads * ((group + mxmoe::kDecodeHeads - 1) / mxmoe::kDecodeHeads);
+  int rc = palloc(&w.status, 1, true);
+  if (rc == MXMOE_OK) rc = palloc(&ws.part, mxmoe::decode_part_floats(w, c->sms), false);
+  if (rc == MXMOE_OK) rc = palloc(&ws.tickets, mxmoe::decode_workers(w, c->sms), true);
+  if (rc == MXMOE_OK && w.weight) {
+    ws.score_tiles = static_cast<int64_t>(
+        (static_cast<uint64_t>(cfg->n_pages) * cfg->page_size / mxmoe::kDecodeTile + mxmoe::kDecodeMaxRows) * segs);
+    rc = palloc(&ws.scores, static_cast<size_t>(ws.score_tiles) * 128, false);
+    if (rc == MXMOE_OK) rc = palloc(&ws.lse, static_cast<size_t>(mxmoe::kDecodeMaxRows) * cfg->n_heads, false);
+  }
   if (rc != MXMOE_OK) {
     cudaGetLastError();
     mxmqa_paged_destroy(c);
@@ -190,7 +217,11 @@ int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers*
 int mxmqa_paged_destroy(mxmqa_paged_cache* c) {
   if (!c) return MXMOE_OK;
   PDevice g(c->cfg.device);
-  if (c->view.status) cudaFree(c->view.status);
+  cudaFree(c->view.status);
+  cudaFree(c->scratch.part);
+  cudaFree(c->scratch.tickets);
+  cudaFree(c->scratch.scores);
+  cudaFree(c->scratch.lse);
   delete c;
   return MXMOE_OK;
 }
@@ -295,7 +326,7 @@ int mxmqa_paged_decode(mxmqa_paged_cache* c, const mxmqa_paged_decode_args* a, v
   p.bias_len = static_cast<int>(a->bias_len);
   p.track = a->track ? 1 : 0;
   PDevice g(c->cfg.device);
-  P_CUDA(mxmoe::launch_paged_decode(p, static_cast<cudaStream_t>(stream)));
+  P_CUDA(mxmoe::launch_paged_decode(p, c->scratch, c->sms, static_cast<cudaStream_t>(stream)));
   return MXMOE_OK;
 }
 

@@ -7,140 +7,107 @@
 //   o = sum_n e^(s_n - m) v_n / L
 // A row without keys, or whose scores are all -inf, gives zeros.  With track
 // the shares e^(s_n - m) / L of the heads that read key head g are added to the
-// weight of slot n.
-#include <cuda_bf16.h>
-#include <cuda_fp8.h>
+// weight of slot n: the attention kernel leaves the scores and each head's log
+// of the normalizer, and a second kernel turns them into shares once the
+// normalizers are known.
+#include "paged_decode.cuh"
 
-#include "../../include/mxmoe.h"
-#include "launch_util.h"
-#include "paged.h"
+#include <algorithm>
 
 namespace mxmoe {
 namespace {
 
-__device__ __forceinline__ float ld_any(const void* p, int dtype, int64_t i) {
-  if (dtype == MXMOE_F32) return static_cast<const float*>(p)[i];
-  if (dtype == MXMOE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  __nv_fp8_e4m3 x;
-  x.__x = static_cast<const uint8_t*>(p)[i];
-  return static_cast<float>(x);
+constexpr int kRingBytes = 214 * 1024;  // of an SM's 227 KB, beside the row list
+
+// The ring of each warp: at least three stages, so that two are in flight while
+// one is read, with as many warps as that allows.
+DecodePlan decode_plan(const PagedView& c, int sms) {
+  DecodePlan d{};
+  const int es = c.dtype == MXMOE_F32 ? 4 : c.dtype == MXMOE_BF16 ? 2 : 1;
+  d.row_bytes = (c.head_dim * es / 16 | 1) * 16;
+  d.stage_bytes = std::max(2 * kDecodeTile * d.row_bytes, kDecodeHeads * (c.head_dim + 8) * 4);
+  d.warps = kDecodeWarps;
+  while (d.warps > 1 && 3 * d.warps * d.stage_bytes > kRingBytes) d.warps >>= 1;
+  d.stages = std::min(kDecodeMaxStages, kRingBytes / (d.warps * d.stage_bytes));
+  d.smem = d.warps * d.stages * d.stage_bytes + 128;
+  d.grid = sms;
+  return d;
 }
 
-constexpr int kThreads = 128;
-constexpr int kMaxGroup = 1024;  // query heads, checked at creation
-
-// One block per (key head, row); it takes the head's query heads in turn: a
-// pass for the maximum and the sum, a thread per key, and a pass over tiles of
-// keys for the output, a thread per column.
-__global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams p) {
-  __shared__ float qs[256], ps[kThreads], red[kThreads];
-  __shared__ int64_t at[kThreads];
-  __shared__ float top[kMaxGroup], inv[kMaxGroup];
-  const int kvh = blockIdx.x, row = blockIdx.y, hd = p.c.head_dim, tid = threadIdx.x;
-  const int G = p.c.n_heads / p.c.kv_heads;
-  int len = p.lens[row];
-  const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size;
-  if (len < 0 || len > cap) {
-    if (tid == 0) atomicOr(p.c.status, kPagedBadIndex);
-    len = len < 0 ? 0 : static_cast<int>(cap);
-  }
-  const int lo = p.window && p.window < len ? len - p.window : 0;
-  const float ks = p.scale * (p.c.k_scale ? p.c.k_scale[kvh] : 1.0f), vs = p.c.v_scale ? p.c.v_scale[kvh] : 1.0f;
-  for (int g = 0; g < G; ++g) {
-    const int h = kvh * G + g;
-    __syncthreads();
-    for (int i = tid; i < hd; i += kThreads) qs[i] = ld_any(p.q, p.q_dtype, row * p.q_row + h * p.q_head + i);
-    __syncthreads();
-    const float* bias = p.bias ? p.bias + row * p.bias_row + h * p.bias_head : nullptr;
-    auto score = [&](int n, int64_t slot) {
-      const int64_t base = (slot + static_cast<int64_t>(kvh) * p.c.page_size) * hd;
-      float s = 0.0f;
-      for (int i = 0; i < hd; ++i) s = fmaf(qs[i], ld_any(p.c.k, p.c.dtype, base + i), s);
-      s *= ks;
-      return bias && n < p.bias_len ? s + bias[n] : s;
-    };
-    float m = -INFINITY, l = 0.0f;
-    bool nan = false;
-    for (int n = lo + tid; n < len; n += kThreads) {
-      const int64_t slot = slot_of(p.c, p.t, row, n);
-      const float s = slot < 0 ? -INFINITY : score(n, slot);
-      nan |= s != s;
-      const float mn = fmaxf(m, s);
-      if (s != -INFINITY) {
-        l = l * (m == -INFINITY ? 0.0f : expf(m - mn)) + expf(s - mn);
-        m = mn;
-      }
+// One warp per 16 cached keys of a (row, key head): the 8 lanes that hold one
+// key's scores of 8 heads sum their shares, lane j < 16 adds key j's to its
+// slot.  Moves 8 bytes of weight and 32 of scores per key and 8 heads.
+__global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const DecodeScratch ws) {
+  __shared__ int64_t before[kDecodeMaxRows + 1];
+  __shared__ int len_of[kDecodeMaxRows];
+  const decode::Rows rows{before, len_of};
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int H = p.c.kv_heads, G = p.c.n_heads / H, hgroups = (G + kDecodeHeads - 1) / kDecodeHeads;
+  decode::list_rows(p, rows);
+  const int64_t total = before[p.rows] * H, step = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32);
+  for (int64_t x = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5); x < total; x += step) {
+    decode::Place at;
+    at.find(p, rows, H, x);  // seg: the key head
+    const int64_t first = before[at.row] * H * hgroups + static_cast<int64_t>(at.seg) * hgroups * at.tiles + at.tile;
+    float w[4] = {};
+    for (int hg = 0; hg < hgroups; ++hg) {
+      const int h = hg * kDecodeHeads + g;
+      const int64_t tile = first + static_cast<int64_t>(hg) * at.tiles;
+      if (h >= G || tile >= ws.score_tiles) continue;
+      const float lse = ws.lse[at.row * p.c.n_heads + at.seg * G + h];
+      const float4 s = *reinterpret_cast<const float4*>(ws.scores + (tile * 32 + lane) * 4);
+      w[0] += decode::exp_diff(s.x, lse);
+      w[1] += decode::exp_diff(s.y, lse);
+      w[2] += decode::exp_diff(s.z, lse);
+      w[3] += decode::exp_diff(s.w, lse);
     }
-    red[tid] = nan ? NAN : m;
-    __syncthreads();
-    float M = p.sinks ? p.sinks[h] : -INFINITY;
-    if (p.quiet) M = M != M ? M : fmaxf(M, 0.0f);
-    for (int i = 0; i < kThreads; ++i) M = (M != M || red[i] != red[i]) ? NAN : fmaxf(M, red[i]);
-    __syncthreads();
-    red[tid] = m == -INFINITY ? 0.0f : l * expf(m - M);
-    __syncthreads();
-    float L = 0.0f;
-    for (int i = 0; i < kThreads; ++i) L += red[i];
-    if (p.sinks && M != -INFINITY) L += expf(p.sinks[h] - M);
-    if (p.quiet) L += expf(-M);
-    const bool none = M == -INFINITY;
-    if (tid == 0) {
-      top[g] = M;
-      inv[g] = none ? 0.0f : 1.0f / L;
-    }
-    float acc[2] = {0.0f, 0.0f};
-    for (int n0 = lo; n0 < len && !none; n0 += kThreads) {
-      const int n = n0 + tid;
-      __syncthreads();
-      if (n < len) {
-        const int64_t slot = slot_of(p.c, p.t, row, n);
-        const float s = slot < 0 ? -INFINITY : score(n, slot), w = s == -INFINITY ? 0.0f : expf(s - M) / L;
-        ps[tid] = w;
-        at[tid] = slot;
-      }
-      __syncthreads();
-      for (int j = 0; j < min(kThreads, len - n0); ++j) {
-        if (at[j] < 0) continue;
-        const int64_t base = (at[j] + static_cast<int64_t>(kvh) * p.c.page_size) * hd;
-        for (int e = 0; e < 2; ++e)
-          if (tid + e * kThreads < hd) acc[e] = fmaf(ps[j], ld_any(p.c.v, p.c.dtype, base + tid + e * kThreads), acc[e]);
-      }
-    }
-    for (int e = 0; e < 2; ++e) {
-      const int i = tid + e * kThreads;
-      if (i >= hd) continue;
-      const int64_t o = row * p.out_row + h * p.out_head + i;
-      if (p.out_dtype == MXMOE_F32)
-        static_cast<float*>(p.out)[o] = acc[e] * vs;
-      else
-        static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(acc[e] * vs);
-    }
-    if (p.lse && tid == 0) p.lse[static_cast<int64_t>(row) * p.c.n_heads + h] = none ? -INFINITY : M + logf(L);
-  }
-  if (!p.track) return;
-  __syncthreads();
-  for (int n = lo + tid; n < len; n += kThreads) {  // the heads' shares together, then one addition
-    const int64_t slot = slot_of(p.c, p.t, row, n);
-    if (slot < 0) continue;
-    const int64_t base = (slot + static_cast<int64_t>(kvh) * p.c.page_size) * hd;
-    float w = 0.0f;
-    for (int g = 0; g < G; ++g) {
-      const int h = kvh * G + g;
-      float s = 0.0f;
-      for (int i = 0; i < hd; ++i)
-        s = fmaf(ld_any(p.q, p.q_dtype, row * p.q_row + h * p.q_head + i), ld_any(p.c.k, p.c.dtype, base + i), s);
-      s *= ks;
-      if (p.bias && n < p.bias_len) s += p.bias[row * p.bias_row + h * p.bias_head + n];
-      if (s != -INFINITY) w += expf(s - top[g]) * inv[g];
-    }
-    p.c.weight[slot + static_cast<int64_t>(kvh) * p.c.page_size] += w;
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] += __shfl_xor_sync(0xFFFFFFFFu, w[i], o);
+    if (g >= 4) continue;
+    const int key = 8 * (g >> 1) + 2 * t + (g & 1), n = at.lo + at.tile * kDecodeTile + key;
+    if (n >= at.len) continue;
+    const int64_t slot = slot_of(p.c, p.t, at.row, n);
+    const float add = g == 0 ? w[0] : g == 1 ? w[1] : g == 2 ? w[2] : w[3];
+    if (slot >= 0) p.c.weight[slot + static_cast<int64_t>(at.seg) * p.c.page_size] += add;
   }
 }
 
 }  // namespace
 
-cudaError_t launch_paged_decode(const DecodeParams& p, cudaStream_t st) {
-  return launch_kernel(decode_kernel, dim3(p.c.kv_heads, p.rows), dim3(kThreads), 0, st, p);
+size_t decode_part_floats(const PagedView& c, int sms) {
+  const DecodePlan d = decode_plan(c, sms);
+  return static_cast<size_t>(2) * d.grid * d.warps * kDecodeHeads * (c.head_dim + 2);
+}
+
+int decode_workers(const PagedView& c, int sms) {
+  const DecodePlan d = decode_plan(c, sms);
+  return d.grid * d.warps;
+}
+
+cudaError_t launch_paged_decode(const DecodeParams& all, const DecodeScratch& ws, int sms, cudaStream_t st) {
+  const DecodePlan plan = decode_plan(all.c, sms);
+  for (int r0 = 0; r0 < all.rows; r0 += kDecodeMaxRows) {
+    DecodeParams p = all;
+    const int act = all.q_dtype == MXMOE_F32 ? 4 : 2, oact = all.out_dtype == MXMOE_F32 ? 4 : 2;
+    p.rows = std::min(kDecodeMaxRows, all.rows - r0);
+    p.q = static_cast<const char*>(all.q) + r0 * all.q_row * act;
+    p.out = static_cast<char*>(all.out) + r0 * all.out_row * oact;
+    p.lens += r0;
+    p.t.tables += r0 * all.t.stride;
+    p.t.n_rows = p.rows;
+    if (p.lse) p.lse += static_cast<int64_t>(r0) * all.c.n_heads;
+    if (p.bias) p.bias += r0 * all.bias_row;
+    const cudaError_t e = all.c.dtype == MXMOE_BF16   ? launch_attend_bf16(p, ws, plan, st)
+                          : all.c.dtype == MXMOE_E4M3 ? launch_attend_e4m3(p, ws, plan, st)
+                                                      : launch_attend_f32(p, ws, plan, st);
+    if (e != cudaSuccess) return e;
+    if (!p.track) continue;
+    const cudaError_t f = launch_kernel(weigh_kernel, dim3(4 * sms), dim3(256), 0, st, p, ws);
+    if (f != cudaSuccess) return f;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace mxmoe
