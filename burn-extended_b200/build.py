@@ -14,8 +14,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "mxmoe", "libmxmoe.so")
 SOURCES = ["api.cu", "kernels.cu", "dqgemv.cu", "attention.cu", "paged_api.cu", "paged_append.cu",
-           "paged_decode.cu", "paged_decode_bf16.cu", "paged_decode_e4m3.cu", "paged_decode_f32.cu", "paged_evict.cu",
-           "gemm_tc.cu", "modelbin.cpp", "safetensors.cpp"]
+           "paged_decode.cu", "paged_decode_bf16.cu", "paged_decode_bf16_x32.cu", "paged_decode_e4m3.cu",
+           "paged_decode_e4m3_x32.cu", "paged_decode_f32.cu", "paged_evict.cu", "gemm_tc.cu", "modelbin.cpp", "safetensors.cpp"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

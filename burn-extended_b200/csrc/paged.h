@@ -59,6 +59,7 @@ struct DecodeParams {
   void* out;
   int64_t out_row, out_head;
   int out_dtype;
+  int out_wide;  // four columns of out can be stored at once
   float* lse;  // [rows][n_heads] or null
   int rows;
   const int32_t* lens;

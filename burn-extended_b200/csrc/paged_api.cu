@@ -313,6 +313,7 @@ int mxmqa_paged_decode(mxmqa_paged_cache* c, const mxmqa_paged_decode_args* a, v
   p.out_row = a->out_row;
   p.out_head = a->out_head;
   p.out_dtype = static_cast<int>(a->out_dtype);
+  p.out_wide = aligned(a->out, 4 * elem_bytes(a->out_dtype)) && a->out_row % 4 == 0 && a->out_head % 4 == 0;
   p.lse = a->lse;
   p.rows = static_cast<int>(a->rows);
   p.lens = a->lens;

@@ -19,13 +19,20 @@ namespace {
 
 constexpr int kRingBytes = 214 * 1024;  // of an SM's 227 KB, beside the row list
 
+// The register arrays' head size that the kernels are built for.
+int padded_head(const PagedView& c) {
+  for (const int d : {64, 80, 96, 128})
+    if (c.head_dim <= d && (d != 80 || c.dtype == MXMOE_BF16)) return d;
+  return 256;
+}
+
 // The ring of each warp: at least three stages, so that two are in flight while
 // one is read, with as many warps as that allows.
 DecodePlan decode_plan(const PagedView& c, int sms) {
   DecodePlan d{};
   const int es = c.dtype == MXMOE_F32 ? 4 : c.dtype == MXMOE_BF16 ? 2 : 1;
-  d.row_bytes = (c.head_dim * es / 16 | 1) * 16;
-  d.stage_bytes = std::max(2 * kDecodeTile * d.row_bytes, kDecodeHeads * (c.head_dim + 8) * 4);
+  const int hd = padded_head(c);
+  d.stage_bytes = std::max(2 * kDecodeTile * decode::ring_row(hd * es), kDecodeHeads * (hd + 8) * 4);
   d.warps = kDecodeWarps;
   while (d.warps > 1 && 3 * d.warps * d.stage_bytes > kRingBytes) d.warps >>= 1;
   d.stages = std::min(kDecodeMaxStages, kRingBytes / (d.warps * d.stage_bytes));
@@ -99,9 +106,12 @@ cudaError_t launch_paged_decode(const DecodeParams& all, const DecodeScratch& ws
     p.t.n_rows = p.rows;
     if (p.lse) p.lse += static_cast<int64_t>(r0) * all.c.n_heads;
     if (p.bias) p.bias += r0 * all.bias_row;
-    const cudaError_t e = all.c.dtype == MXMOE_BF16   ? launch_attend_bf16(p, ws, plan, st)
-                          : all.c.dtype == MXMOE_E4M3 ? launch_attend_e4m3(p, ws, plan, st)
-                                                      : launch_attend_f32(p, ws, plan, st);
+    // 32-bit queries or outputs keep 22 bits and more of queries and shares
+    const bool x32 = p.q_dtype == MXMOE_F32 || p.out_dtype == MXMOE_F32;
+    const auto attend = p.c.dtype == MXMOE_F32    ? launch_attend_f32
+                        : p.c.dtype == MXMOE_BF16 ? (x32 ? launch_attend_bf16_x32 : launch_attend_bf16)
+                                                  : (x32 ? launch_attend_e4m3_x32 : launch_attend_e4m3);
+    const cudaError_t e = attend(p, ws, plan, st);
     if (e != cudaSuccess) return e;
     if (!p.track) continue;
     const cudaError_t f = launch_kernel(weigh_kernel, dim3(4 * sms), dim3(256), 0, st, p, ws);

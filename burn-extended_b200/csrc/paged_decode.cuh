@@ -32,13 +32,16 @@ constexpr int kDecodeMaxStages = 6;
 // How one launch is laid out; set by decode_plan in paged_decode.cu.
 struct DecodePlan {
   int warps, stages;
-  int row_bytes;    // of a key in the ring: an odd number of 16-byte pieces, so 8 rows at one column hit 8 banks
   int stage_bytes;  // K rows, then V rows; room for 8 x (head_dim + 8) floats
   int smem;         // of the block: the warps' rings, and 128 bytes that a read past the last row may touch
   int grid;
 };
 
 namespace decode {
+
+// Bytes from one key to the next in a ring: an odd number of 16-byte pieces, so
+// that 8 rows at one column lie in 8 different groups of banks.
+constexpr int ring_row(int bytes) { return (bytes / 16 | 1) * 16; }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -126,7 +129,7 @@ __device__ __forceinline__ float ld_act(const void* p, int dtype, int64_t i) {
 
 template <int HDT, bool X>
 struct Bf16 {
-  static constexpr int kElem = 2, kLanes = 8;  // lanes that copy one key's row
+  static constexpr int kElem = 2, rb = ring_row(HDT * 2);
   struct Q {
     uint32_t a[HDT / 16][X ? 6 : 2];
     float back;
@@ -155,15 +158,13 @@ struct Bf16 {
       }
     }
   }
-  static __device__ __forceinline__ void scores(float (&s)[4], const Q& q, uint32_t k, int rb, int hd, int lane) {
+  static __device__ __forceinline__ void scores(float (&s)[4], const Q& q, uint32_t k, int lane) {
     float c[2][4] = {};
     const uint32_t at = k + ((lane >> 4) * 8 + (lane & 7)) * rb + ((lane >> 3) & 1) * 16;
 #pragma unroll
     for (int i = 0; i < HDT / 16; ++i) {
-      if (16 * i >= hd) break;
       uint32_t b[4];
       ldm4(b, at + 32 * i);
-      if (16 * i + 8 >= hd) b[1] = b[3] = 0;  // past the row
       if (X) {
         mma_bf16(c[0], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], b[0], b[1]);
         mma_bf16(c[1], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], b[2], b[3]);
@@ -180,8 +181,8 @@ struct Bf16 {
       s[2 * j + 1] = X ? c[j][1] + c[j][3] : c[j][1];
     }
   }
-  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4], float corr, uint32_t v, int rb,
-                                             int hd, int lane) {
+  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4], float corr, uint32_t v,
+                                             int lane) {
     const uint32_t h0 = pack_bf16(p[0], p[1]), h1 = pack_bf16(p[2], p[3]);
     const float r[4] = {p[0] - lo_of(h0), p[1] - hi_of(h0), p[2] - lo_of(h1), p[3] - hi_of(h1)};
     const uint32_t l0 = pack_bf16(r[0], r[1]), l1 = pack_bf16(r[2], r[3]);
@@ -190,7 +191,6 @@ struct Bf16 {
     const uint32_t at = v + (((lane >> 3) & 1) * 8 + (lane & 7)) * rb + (lane >> 4) * 16;
 #pragma unroll
     for (int n = 0; n < HDT / 8; n += 2) {
-      if (8 * n >= hd) break;
       uint32_t b[4];
       ldm4t(b, at + 16 * n);
 #pragma unroll
@@ -214,7 +214,7 @@ struct Bf16 {
 // agree: lane t takes bytes 4t to 4t + 3 of a key's 16, as one ldmatrix gives.
 template <int HDT, bool X>
 struct E4m3 {
-  static constexpr int kElem = 1, kLanes = HDT / 16 < 8 ? HDT / 16 : 8;
+  static constexpr int kElem = 1, rb = ring_row(HDT);
   struct Q {
     uint32_t a[HDT / 16][4];
     float back;
@@ -251,18 +251,16 @@ struct E4m3 {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
     return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
   }
-  static __device__ __forceinline__ void scores(float (&s)[4], const Q& q, uint32_t k, int rb, int hd, int lane) {
+  static __device__ __forceinline__ void scores(float (&s)[4], const Q& q, uint32_t k, int lane) {
     float c[2][4] = {};
     // one ldmatrix: keys 0-7 and 8-15 of two 16-byte pieces
     const uint32_t at = k + ((lane >> 4) * 8 + (lane & 7)) * rb + ((lane >> 3) & 1) * 16;
 #pragma unroll
     for (int i = 0; i < HDT / 16; i += 2) {
-      if (16 * i >= hd) break;
       uint32_t b[4];
       ldm4(b, at + 16 * i);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        if (16 * (i + e) >= hd) break;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t w = b[2 * j + e];
@@ -276,8 +274,8 @@ struct E4m3 {
       s[2 * j + 1] = X ? c[j][1] + c[j][3] : c[j][1];
     }
   }
-  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4], float corr, uint32_t v, int rb,
-                                             int hd, int lane) {
+  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4], float corr, uint32_t v,
+                                             int lane) {
     const int g = lane >> 2, t = lane & 3;
     const uint32_t h0 = pack_f16(p[0], p[1]), h1 = pack_f16(p[2], p[3]);
     const __half2 a = *reinterpret_cast<const __half2*>(&h0), b = *reinterpret_cast<const __half2*>(&h1);
@@ -286,7 +284,6 @@ struct E4m3 {
     const uint32_t at = v + 2 * t * rb + 4 * g;
 #pragma unroll
     for (int n = 0; n < HDT / 8; n += 4) {  // 32 columns: lane g holds 4g to 4g + 3 of four keys
-      if (8 * n >= hd) break;
       const uint32_t w0 = lds32(at + 8 * n), w1 = lds32(at + rb + 8 * n);
       const uint32_t w2 = lds32(at + 8 * rb + 8 * n), w3 = lds32(at + 9 * rb + 8 * n);
       const uint32_t x[4] = {__byte_perm(w0, w1, 0x5140), __byte_perm(w0, w1, 0x7362), __byte_perm(w2, w3, 0x5140),
@@ -308,7 +305,7 @@ struct E4m3 {
 // exact: 21 bits of either operand.
 template <int HDT, bool X>
 struct F32 {
-  static constexpr int kElem = 4, kLanes = 8;
+  static constexpr int kElem = 4, rb = ring_row(HDT * 4);
   struct Q {
     uint32_t a[HDT / 8][4];
     float back;
@@ -326,12 +323,11 @@ struct F32 {
         q.a[s][2 + half] = rest(x);
       }
   }
-  static __device__ __forceinline__ void scores(float (&s)[4], const Q& q, uint32_t k, int rb, int hd, int lane) {
+  static __device__ __forceinline__ void scores(float (&s)[4], const Q& q, uint32_t k, int lane) {
     float c[2][4] = {};
     const uint32_t at = k + ((lane >> 4) * 8 + (lane & 7)) * rb + ((lane >> 3) & 1) * 16;
 #pragma unroll
     for (int i = 0; i < HDT / 8; ++i) {
-      if (8 * i >= hd) break;
       uint32_t b[4];
       ldm4(b, at + 32 * i);
 #pragma unroll
@@ -347,13 +343,12 @@ struct F32 {
       s[2 * j + 1] = c[j][1] + c[j][3];
     }
   }
-  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4], float corr, uint32_t v, int rb,
-                                             int hd, int lane) {
+  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4], float corr, uint32_t v,
+                                             int lane) {
     const int g = lane >> 2, t = lane & 3;
     const uint32_t at = v + 2 * t * rb + 16 * g;
 #pragma unroll
     for (int n = 0; n < HDT / 8; n += 4) {
-      if (8 * n >= hd) break;
       float w[4][4];
       lds128(w[0], at + 32 * n);
       lds128(w[1], at + rb + 32 * n);
@@ -456,13 +451,41 @@ struct Place {
   }
 };
 
-__device__ __forceinline__ void store_out(const DecodeParams& p, int row, int h, int col, float x) {
+__device__ __forceinline__ void store_out(const DecodeParams& p, int row, int h, int col, float4 x) {
   const int64_t o = row * p.out_row + h * p.out_head + col;
-  if (p.out_dtype == MXMOE_F32)
-    static_cast<float*>(p.out)[o] = x;
-  else
-    static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(x);
+  if (p.out_dtype == MXMOE_F32) {
+    float* y = static_cast<float*>(p.out) + o;
+    if (p.out_wide) {
+      *reinterpret_cast<float4*>(y) = x;
+    } else {
+      y[0] = x.x; y[1] = x.y; y[2] = x.z; y[3] = x.w;
+    }
+  } else {
+    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.out) + o;
+    if (p.out_wide) {
+      *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+    } else {
+      y[0] = __float2bfloat16_rn(x.x); y[1] = __float2bfloat16_rn(x.y);
+      y[2] = __float2bfloat16_rn(x.z); y[3] = __float2bfloat16_rn(x.w);
+    }
+  }
 }
+
+// A head's maximum and sum so far, and four columns of its output.
+struct Joined {
+  float top = -INFINITY, sum = 0.0f;
+  float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+
+  __device__ __forceinline__ void add(float m, float l, float4 o) {
+    const float t = fmaxf(top, m), a = exp_diff(top, t), b = exp_diff(m, t);
+    top = t;
+    sum = fmaf(l, b, sum * a);
+    acc.x = fmaf(o.x, b, acc.x * a);
+    acc.y = fmaf(o.y, b, acc.y * a);
+    acc.z = fmaf(o.z, b, acc.z * a);
+    acc.w = fmaf(o.w, b, acc.w * a);
+  }
+};
 
 // Joins the sink's and the quiet softmax's terms to a head's maximum and sum:
 // the factor on its output, and the log of the normalizer.
@@ -482,8 +505,19 @@ __device__ __forceinline__ float finish(const DecodeParams& p, int h, float m, f
   return f / sum;
 }
 
+// Four finished columns of a head, and with the first its normalizer.
+__device__ __forceinline__ void write_head(const DecodeParams& p, const DecodeScratch& ws, int row, int h, int c, float vs,
+                                           const Joined& j) {
+  float lse;
+  const float f = finish(p, h, j.top, j.sum, lse) * vs;
+  store_out(p, row, h, c, make_float4(j.acc.x * f, j.acc.y * f, j.acc.z * f, j.acc.w * f));
+  if (c != 0) return;
+  if (p.lse) p.lse[static_cast<int64_t>(row) * p.c.n_heads + h] = lse;
+  if (p.track) ws.lse[row * p.c.n_heads + h] = lse;
+}
+
 template <class C, int HDT>
-__global__ void __launch_bounds__(32 * kDecodeWarps)
+__global__ void __launch_bounds__(32 * kDecodeWarps, 1)
     attend_kernel(const DecodeParams p, const DecodeScratch ws, const DecodePlan plan) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ int64_t before[kDecodeMaxRows + 1];
@@ -495,7 +529,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int hd = p.c.head_dim, H = p.c.kv_heads, G = p.c.n_heads / H;
   const int hgroups = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * hgroups;
-  const int rb = plan.row_bytes, W = plan.warps, ldo = hd + 8;
+  constexpr int rb = C::rb, ldo = HDT + 8;
+  const int W = plan.warps;
   const uint32_t mine = smem_u32(ring) + warp * plan.stages * plan.stage_bytes;
   list_rows(p, rows);
   const int64_t total = before[p.rows] * segs;
@@ -503,13 +538,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
   // Rows without keys: zeros.
   for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
     if (before[r + 1] != before[r]) continue;
-    for (int i = threadIdx.x; i < p.c.n_heads * hd; i += blockDim.x) store_out(p, r, i / hd, i % hd, 0.0f);
-    for (int h = threadIdx.x; h < p.c.n_heads; h += blockDim.x) {
-      float lse;
-      finish(p, h, -INFINITY, 0.0f, lse);
-      if (p.lse) p.lse[static_cast<int64_t>(r) * p.c.n_heads + h] = lse;
-      if (p.track) ws.lse[r * p.c.n_heads + h] = lse;
-    }
+    for (int i = threadIdx.x; i < p.c.n_heads * (hd / 4); i += blockDim.x)
+      write_head(p, ws, r, i / (hd / 4), 4 * (i % (hd / 4)), 0.0f, Joined());
   }
   if (total == 0) return;
 
@@ -575,16 +605,22 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
       const int64_t row = page < 0 ? -1
                                    : ((static_cast<int64_t>(page) * H + kvh) * p.c.page_size + slot) * (hd * C::kElem);
       const uint32_t ks = mine + ld_stage * plan.stage_bytes, vs = ks + kDecodeTile * rb;
-      constexpr int kKeys = 32 / C::kLanes;  // keys copied at once
+      constexpr int kPieces = HDT * C::kElem / 16;  // 16 bytes each, zeros past head_dim
+      constexpr int kLanes = kPieces % 8 == 0 ? 8 : 4, kKeys = 32 / kLanes;
+      const int piece = lane % kLanes * 16;
 #pragma unroll
       for (int i = 0; i < kDecodeTile / kKeys; ++i) {
-        const int key = i * kKeys + lane / C::kLanes;
+        const int key = i * kKeys + lane / kLanes;
         const int64_t at = __shfl_sync(0xFFFFFFFFu, row, key);
-        const int bytes = at < 0 ? 0 : 16;
         const int64_t from = at < 0 ? 0 : at;
-        for (int c = (lane % C::kLanes) * 16; c < hd * C::kElem; c += C::kLanes * 16) {
-          cp16(ks + key * rb + c, static_cast<const uint8_t*>(p.c.k) + from + c, bytes);
-          cp16(vs + key * rb + c, static_cast<const uint8_t*>(p.c.v) + from + c, bytes);
+        const uint8_t *kf = static_cast<const uint8_t*>(p.c.k) + from, *vf = static_cast<const uint8_t*>(p.c.v) + from;
+#pragma unroll
+        for (int j = 0; j < (kPieces + kLanes - 1) / kLanes; ++j) {
+          const int c = j * kLanes * 16 + piece;
+          if (kPieces % kLanes && c >= kPieces * 16) break;
+          const bool in = at >= 0 && c < hd * C::kElem;
+          cp16(ks + key * rb + c, kf + (in ? c : 0), in ? 16 : 0);
+          cp16(vs + key * rb + c, vf + (in ? c : 0), in ? 16 : 0);
         }
       }
       look_ahead();
@@ -617,7 +653,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
       load_tile();  // into the stage that the tile before this one left
       const uint32_t k = mine + stage * plan.stage_bytes, v = k + kDecodeTile * rb;
       float s[4];
-      C::scores(s, q, k, rb, hd, lane);
+      C::scores(s, q, k, lane);
       const uint32_t keys = there[warp][stage] >> (2 * t);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -641,55 +677,42 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
       for (int i = 0; i < 4; ++i) w[i] = exp_diff(s[i], top);
       l = fmaf(l, corr, (w[0] + w[1]) + (w[2] + w[3]));
       m = top;
-      C::add(o, w, corr, v, rb, hd, lane);
+      C::add(o, w, corr, v, lane);
       __syncwarp();
       if (++stage == plan.stages) stage = 0;
     }
 
-    // The group's warps join in shared memory.
+    // The group's warps join in shared memory, each in the stage that it loads
+    // next: nothing uses that until then.
     l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
     l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-    // (each in the stage that it loads next, which nothing uses until then)
     const int at_stage = (warp * plan.stages + ld_stage) * plan.stage_bytes;
     float* jo = reinterpret_cast<float*>(ring + at_stage) + g * ldo;
 #pragma unroll
     for (int i = 0; i < HDT / 8; ++i)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (C::column(i, e, t) < hd) jo[C::column(i, e, t)] = o[i][e];
+      for (int e = 0; e < 2; ++e) jo[C::column(i, e, t)] = o[i][e];
     if (t == 0) {
       join_ml[warp][g][0] = m;
       join_ml[warp][g][1] = l;
     }
     if (lane == 0) join_at[warp] = at_stage;
     group_sync();
-    const int w0 = group * wg, tid = threadIdx.x - w0 * 32;
+    const int w0 = group * wg, tid = threadIdx.x - w0 * 32, nt = 32 * wg;
     const bool whole = n == at.tiles;
-    const int slot_floats = kDecodeHeads * (hd + 2);
+    const int slot_floats = kDecodeHeads * (hd + 2), quads = hd / 4;
     float* part = ws.part + (2 * worker + (at.tile == 0 ? 1 : 0)) * slot_floats;
     const float vs = p.c.v_scale ? p.c.v_scale[kvh] : 1.0f;
-    for (int i = tid; i < heads * hd; i += 32 * wg) {
-      const int h = i / hd, c = i - h * hd;
-      float top = -INFINITY;
-      for (int w = w0; w < w0 + wg; ++w) top = fmaxf(top, join_ml[w][h][0]);
-      float sum = 0.0f, acc = 0.0f;
-      for (int w = w0; w < w0 + wg; ++w) {
-        const float f = exp_diff(join_ml[w][h][0], top);
-        sum = fmaf(join_ml[w][h][1], f, sum);
-        acc = fmaf(reinterpret_cast<const float*>(ring + join_at[w])[h * ldo + c], f, acc);
-      }
+    for (int i = tid; i < heads * quads; i += nt) {
+      const int h = i / quads, c = 4 * (i - h * quads);
+      Joined j;
+      for (int w = w0; w < w0 + wg; ++w)
+        j.add(join_ml[w][h][0], join_ml[w][h][1], *reinterpret_cast<const float4*>(ring + join_at[w] + 4 * (h * ldo + c)));
       if (whole) {
-        float lse;
-        const float f = finish(p, h0 + h, top, sum, lse);
-        store_out(p, at.row, h0 + h, c, acc * f * vs);
-        if (c == 0 && p.lse) p.lse[static_cast<int64_t>(at.row) * p.c.n_heads + h0 + h] = lse;
-        if (c == 0 && p.track) ws.lse[at.row * p.c.n_heads + h0 + h] = lse;
+        write_head(p, ws, at.row, h0 + h, c, vs, j);
       } else {
-        part[i] = acc;
-        if (c == 0) {
-          part[kDecodeHeads * hd + 2 * h] = top;
-          part[kDecodeHeads * hd + 2 * h + 1] = sum;
-        }
+        *reinterpret_cast<float4*>(part + 4 * i) = j.acc;
+        if (c == 0) *reinterpret_cast<float2*>(part + kDecodeHeads * hd + 2 * h) = make_float2(j.top, j.sum);
       }
     }
     if (!whole) {
@@ -704,24 +727,25 @@ __global__ void __launch_bounds__(32 * kDecodeWarps)
       if (arrived[group] == static_cast<int>(last_w - first_w)) {
         __threadfence();
         if (tid == 0) ws.tickets[first_w] = 0;
-        for (int i = tid; i < heads * hd; i += 32 * wg) {
-          const int h = i / hd, c = i - h * hd;
-          const float* first = ws.part + (2 * first_w + 1) * slot_floats;
-          float top = __ldcg(first + kDecodeHeads * hd + 2 * h);
-          for (int64_t w = first_w + 1; w <= last_w; ++w)
-            top = fmaxf(top, __ldcg(ws.part + 2 * w * slot_floats + kDecodeHeads * hd + 2 * h));
-          float sum = 0.0f, acc = 0.0f;
+        constexpr int kAtOnce = 4;  // pieces of the output whose loads are in flight together
+        for (int i0 = tid; i0 < heads * quads; i0 += kAtOnce * nt) {
+          Joined j[kAtOnce];
+#pragma unroll 2
           for (int64_t w = first_w; w <= last_w; ++w) {
-            const float* q = ws.part + (2 * w + (w == first_w ? 1 : 0)) * slot_floats;
-            const float f = exp_diff(__ldcg(q + kDecodeHeads * hd + 2 * h), top);
-            sum = fmaf(__ldcg(q + kDecodeHeads * hd + 2 * h + 1), f, sum);
-            acc = fmaf(__ldcg(q + i), f, acc);
+            const float* from = ws.part + (2 * w + (w == first_w ? 1 : 0)) * slot_floats;
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+              const int i = i0 + e * nt;
+              if (i >= heads * quads) break;
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + kDecodeHeads * hd) + i / quads);
+              j[e].add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(from) + i));
+            }
           }
-          float lse;
-          const float f = finish(p, h0 + h, top, sum, lse);
-          store_out(p, at.row, h0 + h, c, acc * f * vs);
-          if (c == 0 && p.lse) p.lse[static_cast<int64_t>(at.row) * p.c.n_heads + h0 + h] = lse;
-          if (c == 0 && p.track) ws.lse[at.row * p.c.n_heads + h0 + h] = lse;
+#pragma unroll
+          for (int e = 0; e < kAtOnce; ++e) {
+            const int i = i0 + e * nt, h = i / quads;
+            if (i < heads * quads) write_head(p, ws, at.row, h0 + h, 4 * (i - h * quads), vs, j[e]);
+          }
         }
       }
     }
@@ -743,7 +767,9 @@ cudaError_t launch(const DecodeParams& p, const DecodeScratch& ws, const DecodeP
 }  // namespace decode
 
 cudaError_t launch_attend_bf16(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st);
+cudaError_t launch_attend_bf16_x32(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st);
 cudaError_t launch_attend_e4m3(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st);
+cudaError_t launch_attend_e4m3_x32(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st);
 cudaError_t launch_attend_f32(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st);
 
 }  // namespace mxmoe

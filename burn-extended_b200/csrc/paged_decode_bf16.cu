@@ -1,16 +1,13 @@
-// paged_decode_bf16.cu -- the attention kernel of paged_decode.cuh over a cache of bf16.
+// paged_decode_bf16.cu -- the attention kernel of paged_decode.cuh over a cache of
+// bf16, bf16 queries and outputs.
 #include "paged_decode.cuh"
 
 namespace mxmoe {
 
 cudaError_t launch_attend_bf16(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st) {
-  // 32-bit queries or outputs keep 22 bits and more of queries and shares
-  if (p.q_dtype == MXMOE_F32 || p.out_dtype == MXMOE_F32) {
-    if (p.c.head_dim <= 64) return decode::launch<decode::Bf16<64, true>, 64>(p, ws, plan, st);
-    if (p.c.head_dim <= 128) return decode::launch<decode::Bf16<128, true>, 128>(p, ws, plan, st);
-    return decode::launch<decode::Bf16<256, true>, 256>(p, ws, plan, st);
-  }
   if (p.c.head_dim <= 64) return decode::launch<decode::Bf16<64, false>, 64>(p, ws, plan, st);
+  if (p.c.head_dim <= 80) return decode::launch<decode::Bf16<80, false>, 80>(p, ws, plan, st);
+  if (p.c.head_dim <= 96) return decode::launch<decode::Bf16<96, false>, 96>(p, ws, plan, st);
   if (p.c.head_dim <= 128) return decode::launch<decode::Bf16<128, false>, 128>(p, ws, plan, st);
   return decode::launch<decode::Bf16<256, false>, 256>(p, ws, plan, st);
 }
