@@ -82,8 +82,7 @@ struct EvictParams {
   int budget, sink, recent;
 };
 
-constexpr int kDecodeTile = 16;       // keys per tile
-constexpr int kDecodeMaxRows = 1024;  // rows per launch: their prefix sums lie in shared memory
+constexpr int kDecodeMaxRows = 512;   // rows per launch: their prefix sums lie in shared memory
 constexpr int kDecodeHeads = 8;       // query heads of a segment
 constexpr int kDecodeWarps = 8;       // of a block, at most
 
@@ -91,13 +90,14 @@ constexpr int kDecodeWarps = 8;       // of a block, at most
 struct DecodeScratch {
   float* part;    // [2 * workers][8 * (head_dim + 2)] partial outputs, maxima and sums
   int* tickets;   // [workers], zero between calls
-  float* scores;  // [score_tiles][32 lanes][4] (track)
+  float* scores;  // [score_tiles][tile / 16][32 lanes][4] (track)
   int64_t score_tiles;
   float* lse;  // [kDecodeMaxRows][n_heads] (track)
 };
 
 cudaError_t launch_paged_append(const AppendParams& p, cudaStream_t st);
 cudaError_t launch_paged_decode(const DecodeParams& p, const DecodeScratch& ws, int sms, cudaStream_t st);
+int decode_tile(const PagedView& c);                     // keys of a tile
 size_t decode_part_floats(const PagedView& c, int sms);  // of DecodeScratch::part
 int decode_workers(const PagedView& c, int sms);         // of DecodeScratch::tickets
 cudaError_t launch_paged_evict(const EvictParams& p, cudaStream_t st);

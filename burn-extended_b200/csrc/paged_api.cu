@@ -201,8 +201,8 @@ int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers*
   if (rc == MXMOE_OK) rc = palloc(&ws.tickets, mxmoe::decode_workers(w, c->sms), true);
   if (rc == MXMOE_OK && w.weight) {
     ws.score_tiles = static_cast<int64_t>(
-        (static_cast<uint64_t>(cfg->n_pages) * cfg->page_size / mxmoe::kDecodeTile + mxmoe::kDecodeMaxRows) * segs);
-    rc = palloc(&ws.scores, static_cast<size_t>(ws.score_tiles) * 128, false);
+        (static_cast<uint64_t>(cfg->n_pages) * cfg->page_size / mxmoe::decode_tile(w) + mxmoe::kDecodeMaxRows) * segs);
+    rc = palloc(&ws.scores, static_cast<size_t>(ws.score_tiles) * mxmoe::decode_tile(w) * 8, false);
     if (rc == MXMOE_OK) rc = palloc(&ws.lse, static_cast<size_t>(mxmoe::kDecodeMaxRows) * cfg->n_heads, false);
   }
   if (rc != MXMOE_OK) {

@@ -17,7 +17,7 @@
 namespace mxmoe {
 namespace {
 
-constexpr int kRingBytes = 214 * 1024;  // of an SM's 227 KB, beside the row list
+constexpr int kRingBytes = 217 * 1024;  // of an SM's 227 KB, beside the row list
 
 // The register arrays' head size that the kernels are built for.
 int padded_head(const PagedView& c) {
@@ -32,7 +32,7 @@ DecodePlan decode_plan(const PagedView& c, int sms) {
   DecodePlan d{};
   const int es = c.dtype == MXMOE_F32 ? 4 : c.dtype == MXMOE_BF16 ? 2 : 1;
   const int hd = padded_head(c);
-  d.stage_bytes = std::max(2 * kDecodeTile * decode::ring_row(hd * es), kDecodeHeads * (hd + 8) * 4);
+  d.stage_bytes = std::max(32 * decode::tile_halves(hd * es) * decode::ring_row(hd * es), kDecodeHeads * (hd + 8) * 4);
   d.warps = kDecodeWarps;
   while (d.warps > 1 && 3 * d.warps * d.stage_bytes > kRingBytes) d.warps >>= 1;
   d.stages = std::min(kDecodeMaxStages, kRingBytes / (d.warps * d.stage_bytes));
@@ -41,47 +41,59 @@ DecodePlan decode_plan(const PagedView& c, int sms) {
   return d;
 }
 
-// One warp per 16 cached keys of a (row, key head): the 8 lanes that hold one
-// key's scores of 8 heads sum their shares, lane j < 16 adds key j's to its
+// One warp per tile of cached keys of a (row, key head): the 8 lanes that hold
+// one key's scores of 8 heads sum their shares, lane j adds key j's to its
 // slot.  Moves 8 bytes of weight and 32 of scores per key and 8 heads.
+template <int NT>
 __global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const DecodeScratch ws) {
   __shared__ int64_t before[kDecodeMaxRows + 1];
   __shared__ int len_of[kDecodeMaxRows];
   const decode::Rows rows{before, len_of};
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int H = p.c.kv_heads, G = p.c.n_heads / H, hgroups = (G + kDecodeHeads - 1) / kDecodeHeads;
-  decode::list_rows(p, rows);
+  decode::list_rows(p, rows, 16 * NT);
   const int64_t total = before[p.rows] * H, step = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32);
   for (int64_t x = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5); x < total; x += step) {
     decode::Place at;
     at.find(p, rows, H, x);  // seg: the key head
     const int64_t first = before[at.row] * H * hgroups + static_cast<int64_t>(at.seg) * hgroups * at.tiles + at.tile;
-    float w[4] = {};
+    float w[4 * NT] = {};
     for (int hg = 0; hg < hgroups; ++hg) {
       const int h = hg * kDecodeHeads + g;
       const int64_t tile = first + static_cast<int64_t>(hg) * at.tiles;
       if (h >= G || tile >= ws.score_tiles) continue;
       const float lse = ws.lse[at.row * p.c.n_heads + at.seg * G + h];
-      const float4 s = *reinterpret_cast<const float4*>(ws.scores + (tile * 32 + lane) * 4);
-      w[0] += decode::exp_diff(s.x, lse);
-      w[1] += decode::exp_diff(s.y, lse);
-      w[2] += decode::exp_diff(s.z, lse);
-      w[3] += decode::exp_diff(s.w, lse);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const float4 s = *reinterpret_cast<const float4*>(ws.scores + ((tile * NT + u) * 32 + lane) * 4);
+        w[4 * u] += decode::exp_diff(s.x, lse);
+        w[4 * u + 1] += decode::exp_diff(s.y, lse);
+        w[4 * u + 2] += decode::exp_diff(s.z, lse);
+        w[4 * u + 3] += decode::exp_diff(s.w, lse);
+      }
     }
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] += __shfl_xor_sync(0xFFFFFFFFu, w[i], o);
-    if (g >= 4) continue;
-    const int key = 8 * (g >> 1) + 2 * t + (g & 1), n = at.lo + at.tile * kDecodeTile + key;
+      for (int i = 0; i < 4 * NT; ++i) w[i] += __shfl_xor_sync(0xFFFFFFFFu, w[i], o);
+    // w[i] is key 8 (i / 2) + 2t + i % 2; lane (g, t) takes i = g
+    if (g >= 4 * NT) continue;
+    const int n = at.lo + at.tile * 16 * NT + 8 * (g >> 1) + 2 * t + (g & 1);
     if (n >= at.len) continue;
+    float add = w[0];
+#pragma unroll
+    for (int i = 1; i < 4 * NT; ++i) add = g == i ? w[i] : add;
     const int64_t slot = slot_of(p.c, p.t, at.row, n);
-    const float add = g == 0 ? w[0] : g == 1 ? w[1] : g == 2 ? w[2] : w[3];
     if (slot >= 0) p.c.weight[slot + static_cast<int64_t>(at.seg) * p.c.page_size] += add;
   }
 }
 
 }  // namespace
+
+int decode_tile(const PagedView& c) {
+  const int es = c.dtype == MXMOE_F32 ? 4 : c.dtype == MXMOE_BF16 ? 2 : 1;
+  return 16 * decode::tile_halves(padded_head(c) * es);
+}
 
 size_t decode_part_floats(const PagedView& c, int sms) {
   const DecodePlan d = decode_plan(c, sms);
@@ -114,7 +126,7 @@ cudaError_t launch_paged_decode(const DecodeParams& all, const DecodeScratch& ws
     const cudaError_t e = attend(p, ws, plan, st);
     if (e != cudaSuccess) return e;
     if (!p.track) continue;
-    const cudaError_t f = launch_kernel(weigh_kernel, dim3(4 * sms), dim3(256), 0, st, p, ws);
+    const cudaError_t f = launch_kernel(decode_tile(p.c) == 32 ? weigh_kernel<2> : weigh_kernel<1>, dim3(4 * sms), dim3(256), 0, st, p, ws);
     if (f != cudaSuccess) return f;
   }
   return cudaSuccess;

@@ -43,6 +43,10 @@ namespace decode {
 // that 8 rows at one column lie in 8 different groups of banks.
 constexpr int ring_row(int bytes) { return (bytes / 16 | 1) * 16; }
 
+// Keys of a tile in 16s: two independent halves hide each other's latency where
+// a row is short; longer rows have enough columns for that.
+constexpr int tile_halves(int bytes) { return bytes <= 128 ? 2 : 1; }
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -129,7 +133,7 @@ __device__ __forceinline__ float ld_act(const void* p, int dtype, int64_t i) {
 
 template <int HDT, bool X>
 struct Bf16 {
-  static constexpr int kElem = 2, rb = ring_row(HDT * 2);
+  static constexpr int kElem = 2, rb = ring_row(HDT * 2), NT = tile_halves(HDT * 2);
   struct Q {
     uint32_t a[HDT / 16][X ? 6 : 2];
     float back;
@@ -158,48 +162,60 @@ struct Bf16 {
       }
     }
   }
-  static __device__ __forceinline__ void scores(float (&s)[4], const Q& q, uint32_t k, int lane) {
-    float c[2][4] = {};
+  static __device__ __forceinline__ void scores(float (&s)[4 * NT], const Q& q, uint32_t k, int lane) {
+    float c[2 * NT][4] = {};
     const uint32_t at = k + ((lane >> 4) * 8 + (lane & 7)) * rb + ((lane >> 3) & 1) * 16;
 #pragma unroll
     for (int i = 0; i < HDT / 16; ++i) {
-      uint32_t b[4];
-      ldm4(b, at + 32 * i);
-      if (X) {
-        mma_bf16(c[0], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], b[0], b[1]);
-        mma_bf16(c[1], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], b[2], b[3]);
-        mma_bf16(c[0], q.a[i][4], 0, q.a[i][5], 0, b[0], b[1]);
-        mma_bf16(c[1], q.a[i][4], 0, q.a[i][5], 0, b[2], b[3]);
-      } else {
-        mma_bf16(c[0], q.a[i][0], 0, q.a[i][1], 0, b[0], b[1]);
-        mma_bf16(c[1], q.a[i][0], 0, q.a[i][1], 0, b[2], b[3]);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        uint32_t b[4];
+        ldm4(b, at + 16 * u * rb + 32 * i);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (X) {
+            mma_bf16(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], b[2 * j], b[2 * j + 1]);
+            mma_bf16(c[2 * u + j], q.a[i][4], 0, q.a[i][5], 0, b[2 * j], b[2 * j + 1]);
+          } else {
+            mma_bf16(c[2 * u + j], q.a[i][0], 0, q.a[i][1], 0, b[2 * j], b[2 * j + 1]);
+          }
+        }
       }
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 2 * NT; ++j) {
       s[2 * j] = X ? c[j][0] + c[j][2] : c[j][0];
       s[2 * j + 1] = X ? c[j][1] + c[j][3] : c[j][1];
     }
   }
-  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4], float corr, uint32_t v,
+  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4 * NT], float corr, uint32_t v,
                                              int lane) {
-    const uint32_t h0 = pack_bf16(p[0], p[1]), h1 = pack_bf16(p[2], p[3]);
-    const float r[4] = {p[0] - lo_of(h0), p[1] - hi_of(h0), p[2] - lo_of(h1), p[3] - hi_of(h1)};
-    const uint32_t l0 = pack_bf16(r[0], r[1]), l1 = pack_bf16(r[2], r[3]);
-    const uint32_t m0 = X ? pack_bf16(r[0] - lo_of(l0), r[1] - hi_of(l0)) : 0;
-    const uint32_t m1 = X ? pack_bf16(r[2] - lo_of(l1), r[3] - hi_of(l1)) : 0;
+    uint32_t h[2 * NT], l[2 * NT], m[2 * NT];
+#pragma unroll
+    for (int j = 0; j < 2 * NT; ++j) {
+      h[j] = pack_bf16(p[2 * j], p[2 * j + 1]);
+      const float x = p[2 * j] - lo_of(h[j]), y = p[2 * j + 1] - hi_of(h[j]);
+      l[j] = pack_bf16(x, y);
+      m[j] = X ? pack_bf16(x - lo_of(l[j]), y - hi_of(l[j])) : 0;
+    }
     const uint32_t at = v + (((lane >> 3) & 1) * 8 + (lane & 7)) * rb + (lane >> 4) * 16;
 #pragma unroll
     for (int n = 0; n < HDT / 8; n += 2) {
-      uint32_t b[4];
-      ldm4t(b, at + 16 * n);
+      float d[2][4] = {};
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        uint32_t b[4];
+        ldm4t(b, at + 16 * u * rb + 16 * n);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mma_bf16(d[e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b[2 * e], b[2 * e + 1]);
+          if (X) mma_bf16(d[e], m[2 * u], 0, m[2 * u + 1], 0, b[2 * e], b[2 * e + 1]);
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float d[4] = {};
-        mma_bf16(d, h0, l0, h1, l1, b[2 * e], b[2 * e + 1]);
-        if (X) mma_bf16(d, m0, 0, m1, 0, b[2 * e], b[2 * e + 1]);
-        o[n + e][0] = fmaf(o[n + e][0], corr, d[0] + d[2]);
-        o[n + e][1] = fmaf(o[n + e][1], corr, d[1] + d[3]);
+        o[n + e][0] = fmaf(o[n + e][0], corr, d[e][0] + d[e][2]);
+        o[n + e][1] = fmaf(o[n + e][1], corr, d[e][1] + d[e][3]);
       }
     }
   }
@@ -214,7 +230,7 @@ struct Bf16 {
 // agree: lane t takes bytes 4t to 4t + 3 of a key's 16, as one ldmatrix gives.
 template <int HDT, bool X>
 struct E4m3 {
-  static constexpr int kElem = 1, rb = ring_row(HDT);
+  static constexpr int kElem = 1, rb = ring_row(HDT), NT = tile_halves(HDT);
   struct Q {
     uint32_t a[HDT / 16][4];
     float back;
@@ -251,50 +267,61 @@ struct E4m3 {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
     return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
   }
-  static __device__ __forceinline__ void scores(float (&s)[4], const Q& q, uint32_t k, int lane) {
-    float c[2][4] = {};
+  static __device__ __forceinline__ void scores(float (&s)[4 * NT], const Q& q, uint32_t k, int lane) {
+    float c[2 * NT][4] = {};
     // one ldmatrix: keys 0-7 and 8-15 of two 16-byte pieces
     const uint32_t at = k + ((lane >> 4) * 8 + (lane & 7)) * rb + ((lane >> 3) & 1) * 16;
 #pragma unroll
     for (int i = 0; i < HDT / 16; i += 2) {
-      uint32_t b[4];
-      ldm4(b, at + 16 * i);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int u = 0; u < NT; ++u) {
+        uint32_t b[4];
+        ldm4(b, at + 16 * u * rb + 16 * i);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t w = b[2 * j + e];
-          mma_f16(c[j], q.a[i + e][0], q.a[i + e][2], q.a[i + e][1], q.a[i + e][3], widen(w & 0xFFFF), widen(w >> 16));
+        for (int j = 0; j < 4; ++j) {
+          const int e = j & 1;
+          const uint32_t w = b[j];
+          mma_f16(c[2 * u + (j >> 1)], q.a[i + e][0], q.a[i + e][2], q.a[i + e][1], q.a[i + e][3], widen(w & 0xFFFF), widen(w >> 16));
         }
       }
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 2 * NT; ++j) {
       s[2 * j] = X ? c[j][0] + c[j][2] : c[j][0];
       s[2 * j + 1] = X ? c[j][1] + c[j][3] : c[j][1];
     }
   }
-  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4], float corr, uint32_t v,
+  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4 * NT], float corr, uint32_t v,
                                              int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t h0 = pack_f16(p[0], p[1]), h1 = pack_f16(p[2], p[3]);
-    const __half2 a = *reinterpret_cast<const __half2*>(&h0), b = *reinterpret_cast<const __half2*>(&h1);
-    const uint32_t l0 = pack_f16(p[0] - __low2float(a), p[1] - __high2float(a));
-    const uint32_t l1 = pack_f16(p[2] - __low2float(b), p[3] - __high2float(b));
+    uint32_t h[2 * NT], l[2 * NT];
+#pragma unroll
+    for (int j = 0; j < 2 * NT; ++j) {
+      h[j] = pack_f16(p[2 * j], p[2 * j + 1]);
+      const __half2 x = *reinterpret_cast<const __half2*>(&h[j]);
+      l[j] = pack_f16(p[2 * j] - __low2float(x), p[2 * j + 1] - __high2float(x));
+    }
     const uint32_t at = v + 2 * t * rb + 4 * g;
 #pragma unroll
     for (int n = 0; n < HDT / 8; n += 4) {  // 32 columns: lane g holds 4g to 4g + 3 of four keys
-      const uint32_t w0 = lds32(at + 8 * n), w1 = lds32(at + rb + 8 * n);
-      const uint32_t w2 = lds32(at + 8 * rb + 8 * n), w3 = lds32(at + 9 * rb + 8 * n);
-      const uint32_t x[4] = {__byte_perm(w0, w1, 0x5140), __byte_perm(w0, w1, 0x7362), __byte_perm(w2, w3, 0x5140),
-                             __byte_perm(w2, w3, 0x7362)};
+      float d[4][4] = {};
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const uint32_t from = at + 16 * u * rb + 8 * n;
+        const uint32_t w0 = lds32(from), w1 = lds32(from + rb), w2 = lds32(from + 8 * rb), w3 = lds32(from + 9 * rb);
+        const uint32_t x[4] = {__byte_perm(w0, w1, 0x5140), __byte_perm(w0, w1, 0x7362), __byte_perm(w2, w3, 0x5140),
+                               __byte_perm(w2, w3, 0x7362)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t y = x[e >> 1], z = x[2 + (e >> 1)];
+          mma_f16(d[e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], widen(e & 1 ? y >> 16 : y & 0xFFFF),
+                  widen(e & 1 ? z >> 16 : z & 0xFFFF));
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t y = x[e >> 1], z = x[2 + (e >> 1)];
-        float d[4] = {};
-        mma_f16(d, h0, l0, h1, l1, widen(e & 1 ? y >> 16 : y & 0xFFFF), widen(e & 1 ? z >> 16 : z & 0xFFFF));
-        o[n + e][0] = fmaf(o[n + e][0], corr, d[0] + d[2]);
-        o[n + e][1] = fmaf(o[n + e][1], corr, d[1] + d[3]);
+        o[n + e][0] = fmaf(o[n + e][0], corr, d[e][0] + d[e][2]);
+        o[n + e][1] = fmaf(o[n + e][1], corr, d[e][1] + d[e][3]);
       }
     }
   }
@@ -305,7 +332,7 @@ struct E4m3 {
 // exact: 21 bits of either operand.
 template <int HDT, bool X>
 struct F32 {
-  static constexpr int kElem = 4, rb = ring_row(HDT * 4);
+  static constexpr int kElem = 4, rb = ring_row(HDT * 4), NT = tile_halves(HDT * 4);
   struct Q {
     uint32_t a[HDT / 8][4];
     float back;
@@ -323,48 +350,52 @@ struct F32 {
         q.a[s][2 + half] = rest(x);
       }
   }
-  static __device__ __forceinline__ void scores(float (&s)[4], const Q& q, uint32_t k, int lane) {
-    float c[2][4] = {};
+  static __device__ __forceinline__ void scores(float (&s)[4 * NT], const Q& q, uint32_t k, int lane) {
+    float c[2 * NT][4] = {};
     const uint32_t at = k + ((lane >> 4) * 8 + (lane & 7)) * rb + ((lane >> 3) & 1) * 16;
 #pragma unroll
     for (int i = 0; i < HDT / 8; ++i) {
-      uint32_t b[4];
-      ldm4(b, at + 32 * i);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float x = __uint_as_float(b[2 * j]), y = __uint_as_float(b[2 * j + 1]);
-        mma_tf32(c[j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], top(x), top(y));
-        mma_tf32(c[j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], rest(x), rest(y));
+      for (int u = 0; u < NT; ++u) {
+        uint32_t b[4];
+        ldm4(b, at + 16 * u * rb + 32 * i);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float x = __uint_as_float(b[2 * j]), y = __uint_as_float(b[2 * j + 1]);
+          mma_tf32(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], top(x), top(y));
+          mma_tf32(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], rest(x), rest(y));
+        }
       }
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 2 * NT; ++j) {
       s[2 * j] = c[j][0] + c[j][2];
       s[2 * j + 1] = c[j][1] + c[j][3];
     }
   }
-  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4], float corr, uint32_t v,
+  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4 * NT], float corr, uint32_t v,
                                              int lane) {
     const int g = lane >> 2, t = lane & 3;
     const uint32_t at = v + 2 * t * rb + 16 * g;
 #pragma unroll
     for (int n = 0; n < HDT / 8; n += 4) {
-      float w[4][4];
-      lds128(w[0], at + 32 * n);
-      lds128(w[1], at + rb + 32 * n);
-      lds128(w[2], at + 8 * rb + 32 * n);
-      lds128(w[3], at + 9 * rb + 32 * n);
+      float d[4][4] = {};
+#pragma unroll
+      for (int u = 0; u < 2 * NT; ++u) {  // keys 8u to 8u + 7
+        float w[2][4];
+        lds128(w[0], at + 8 * u * rb + 32 * n);
+        lds128(w[1], at + (8 * u + 1) * rb + 32 * n);
+        const float p0 = p[2 * u], p1 = p[2 * u + 1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          mma_tf32(d[e], top(p0), rest(p0), top(p1), rest(p1), top(w[0][e]), top(w[1][e]));
+          mma_tf32(d[e], top(p0), rest(p0), top(p1), rest(p1), rest(w[0][e]), rest(w[1][e]));
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float d[4] = {};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float x = w[2 * j][e], y = w[2 * j + 1][e];
-          mma_tf32(d, top(p[2 * j]), rest(p[2 * j]), top(p[2 * j + 1]), rest(p[2 * j + 1]), top(x), top(y));
-          mma_tf32(d, top(p[2 * j]), rest(p[2 * j]), top(p[2 * j + 1]), rest(p[2 * j + 1]), rest(x), rest(y));
-        }
-        o[n + e][0] = fmaf(o[n + e][0], corr, d[0] + d[2]);
-        o[n + e][1] = fmaf(o[n + e][1], corr, d[1] + d[3]);
+        o[n + e][0] = fmaf(o[n + e][0], corr, d[e][0] + d[e][2]);
+        o[n + e][1] = fmaf(o[n + e][1], corr, d[e][1] + d[e][3]);
       }
     }
   }
@@ -382,7 +413,7 @@ struct Rows {
 __device__ __forceinline__ int first_key(int len, int window) { return window && window < len ? len - window : 0; }
 
 // All threads; ends with a barrier.
-__device__ __forceinline__ void list_rows(const DecodeParams& p, Rows r) {
+__device__ __forceinline__ void list_rows(const DecodeParams& p, Rows r, int tile) {
   __shared__ int64_t sums[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = blockDim.x >> 5;
   const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size;
@@ -398,7 +429,7 @@ __device__ __forceinline__ void list_rows(const DecodeParams& p, Rows r) {
       }
       r.len[i] = len;
     }
-    int64_t x = (len - first_key(len, p.window) + kDecodeTile - 1) / kDecodeTile;
+    int64_t x = (len - first_key(len, p.window) + tile - 1) / tile;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
@@ -529,10 +560,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int hd = p.c.head_dim, H = p.c.kv_heads, G = p.c.n_heads / H;
   const int hgroups = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * hgroups;
-  constexpr int rb = C::rb, ldo = HDT + 8;
+  constexpr int rb = C::rb, ldo = HDT + 8, NT = C::NT, kTile = 16 * NT;
   const int W = plan.warps;
   const uint32_t mine = smem_u32(ring) + warp * plan.stages * plan.stage_bytes;
-  list_rows(p, rows);
+  list_rows(p, rows, kTile);
   const int64_t total = before[p.rows] * segs;
 
   // Rows without keys: zeros.
@@ -566,7 +597,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
   };
 
   // What this warp loads next: its tile, and each lane's page of the tile's key
-  // lane % 16, read one tile ahead.
+  // of that number, read one tile ahead.
   Place ld;
   ld.find(p, rows, segs, begin);
   int64_t ld_left = end - begin;
@@ -586,7 +617,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
     }
     ld_tile = ld.tile + ld_off;
     ld_off += wg;
-    const int n = ld.lo + ld_tile * kDecodeTile + (lane & 15);
+    const int n = ld.lo + ld_tile * kTile + lane % kTile;
     page = -1;
     if (n < ld.len) {
       const int pi = page_of(p.c, n);
@@ -604,12 +635,12 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
       const int kvh = ld.seg / hgroups;
       const int64_t row = page < 0 ? -1
                                    : ((static_cast<int64_t>(page) * H + kvh) * p.c.page_size + slot) * (hd * C::kElem);
-      const uint32_t ks = mine + ld_stage * plan.stage_bytes, vs = ks + kDecodeTile * rb;
+      const uint32_t ks = mine + ld_stage * plan.stage_bytes, vs = ks + kTile * rb;
       constexpr int kPieces = HDT * C::kElem / 16;  // 16 bytes each, zeros past head_dim
       constexpr int kLanes = kPieces % 8 == 0 ? 8 : 4, kKeys = 32 / kLanes;
       const int piece = lane % kLanes * 16;
 #pragma unroll
-      for (int i = 0; i < kDecodeTile / kKeys; ++i) {
+      for (int i = 0; i < kTile / kKeys; ++i) {
         const int key = i * kKeys + lane / kLanes;
         const int64_t at = __shfl_sync(0xFFFFFFFFu, row, key);
         const int64_t from = at < 0 ? 0 : at;
@@ -651,31 +682,38 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
       cp_wait_for(plan.stages - 2);
       __syncwarp();
       load_tile();  // into the stage that the tile before this one left
-      const uint32_t k = mine + stage * plan.stage_bytes, v = k + kDecodeTile * rb;
-      float s[4];
+      const uint32_t k = mine + stage * plan.stage_bytes, v = k + kTile * rb;
+      float s[4 * NT], w[4 * NT];
       C::scores(s, q, k, lane);
       const uint32_t keys = there[warp][stage] >> (2 * t);
+      float top = m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 4 * NT; ++i) {
         const int e = 8 * (i >> 1) + (i & 1);
         s[i] *= ks;
         if (bias) {
-          const int n = at.lo + (at.tile + j) * kDecodeTile + e + 2 * t;
+          const int n = at.lo + (at.tile + j) * kTile + e + 2 * t;
           if (n < p.bias_len && n < at.len) s[i] += bias[n];
         }
         if (!(keys >> e & 1)) s[i] = -INFINITY;
+        top = fmaxf(top, s[i]);
       }
-      if (p.track && x + j < ws.score_tiles)
-        *reinterpret_cast<float4*>(ws.scores + ((x + j) * 32 + lane) * 4) = make_float4(s[0], s[1], s[2], s[3]);
-      float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+      if (p.track && x + j < ws.score_tiles) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+          *reinterpret_cast<float4*>(ws.scores + (((x + j) * NT + u) * 32 + lane) * 4) =
+              make_float4(s[4 * u], s[4 * u + 1], s[4 * u + 2], s[4 * u + 3]);
+      }
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      top = fmaxf(top, m);
       const float corr = exp_diff(m, top);
-      float w[4];
+      float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = exp_diff(s[i], top);
-      l = fmaf(l, corr, (w[0] + w[1]) + (w[2] + w[3]));
+      for (int i = 0; i < 4 * NT; ++i) {
+        w[i] = exp_diff(s[i], top);
+        sum += w[i];
+      }
+      l = fmaf(l, corr, sum);
       m = top;
       C::add(o, w, corr, v, lane);
       __syncwarp();
