@@ -56,10 +56,11 @@ struct DecodeParams {
   const void* q;
   int64_t q_row, q_head;
   int q_dtype;
+  int q_wide;  // four columns of q can be loaded at once
   void* out;
   int64_t out_row, out_head;
   int out_dtype;
-  int out_wide;  // four columns of out can be stored at once
+  int out_wide;  // two bf16 columns of out can be stored at once
   float* lse;  // [rows][n_heads] or null
   int rows;
   const int32_t* lens;
@@ -88,7 +89,7 @@ constexpr int kDecodeWarps = 8;       // of a block, at most
 
 // Device memory that decode needs beside its arguments.
 struct DecodeScratch {
-  float* part;    // [2 * workers][8 * (head_dim + 2)] partial outputs, maxima and sums
+  float* part;    // [2 * workers][8 * (padded head_dim + 2)] partial outputs, maxima and sums
   int* tickets;   // [workers], zero between calls
   float* scores;  // [score_tiles][tile / 16][32 lanes][4] (track)
   int64_t score_tiles;

@@ -160,6 +160,8 @@ int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers*
                  "head_dim must be a multiple of 8 (16 in an 8-bit cache) and at most 256, page_size at most 65536, "
                  "n_heads at most 1024");
   P_CHECK(cfg->dtype == MXMOE_E4M3 || (!buf->k_scale && !buf->v_scale), "scales are for the 8-bit cache");
+  if (static_cast<uint64_t>(cfg->n_pages) * cfg->page_size > kMaxTokens / cfg->kv_heads)
+    return pfail(MXMOE_ERR_UNSUPPORTED, "n_pages x page_size x kv_heads must be below 2^31");
   mxmqa_paged_cache* c = new (std::nothrow) mxmqa_paged_cache();
   if (!c) return pfail(MXMOE_ERR_OOM, "host allocation failed");
   c->cfg = *cfg;
@@ -304,16 +306,19 @@ int mxmqa_paged_decode(mxmqa_paged_cache* c, const mxmqa_paged_decode_args* a, v
   P_CHECK(!a->track || a->window == 0, "a tracked cache attends in full: window must be 0");
   mxmoe::DecodeParams p{};
   if (const int rc = check_tables(c, a->tables, a->table_stride, a->rows, a->max_pages, p.t)) return rc;
+  if (static_cast<uint64_t>(a->max_pages) * c->cfg.page_size * c->cfg.n_heads > 16ull * kMaxTokens)
+    return pfail(MXMOE_ERR_UNSUPPORTED, "max_pages x page_size x n_heads must be below 2^35");
   p.c = c->view;
   p.q = a->q;
   p.q_row = a->q_row;
   p.q_head = a->q_head;
   p.q_dtype = static_cast<int>(a->q_dtype);
+  p.q_wide = aligned(a->q, 4 * elem_bytes(a->q_dtype)) && a->q_row % 4 == 0 && a->q_head % 4 == 0;
   p.out = a->out;
   p.out_row = a->out_row;
   p.out_head = a->out_head;
   p.out_dtype = static_cast<int>(a->out_dtype);
-  p.out_wide = aligned(a->out, 4 * elem_bytes(a->out_dtype)) && a->out_row % 4 == 0 && a->out_head % 4 == 0;
+  p.out_wide = aligned(a->out, 4) && a->out_row % 2 == 0 && a->out_head % 2 == 0;
   p.lse = a->lse;
   p.rows = static_cast<int>(a->rows);
   p.lens = a->lens;

@@ -13,6 +13,7 @@
 #include "paged_decode.cuh"
 
 #include <algorithm>
+#include <cstdint>
 
 namespace mxmoe {
 namespace {
@@ -32,7 +33,7 @@ DecodePlan decode_plan(const PagedView& c, int sms) {
   DecodePlan d{};
   const int es = c.dtype == MXMOE_F32 ? 4 : c.dtype == MXMOE_BF16 ? 2 : 1;
   const int hd = padded_head(c);
-  d.stage_bytes = std::max(32 * decode::tile_halves(hd * es) * decode::ring_row(hd * es), kDecodeHeads * (hd + 8) * 4);
+  d.stage_bytes = std::max(32 * decode::tile_halves(hd * es) * decode::ring_row(hd * es), kDecodeHeads * hd * 4);
   d.warps = kDecodeWarps;
   while (d.warps > 1 && 3 * d.warps * d.stage_bytes > kRingBytes) d.warps >>= 1;
   d.stages = std::min(kDecodeMaxStages, kRingBytes / (d.warps * d.stage_bytes));
@@ -46,23 +47,23 @@ DecodePlan decode_plan(const PagedView& c, int sms) {
 // slot.  Moves 8 bytes of weight and 32 of scores per key and 8 heads.
 template <int NT>
 __global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const DecodeScratch ws) {
-  __shared__ int64_t before[kDecodeMaxRows + 1];
+  __shared__ int before[kDecodeMaxRows + 1];
   __shared__ int len_of[kDecodeMaxRows];
   const decode::Rows rows{before, len_of};
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int H = p.c.kv_heads, G = p.c.n_heads / H, hgroups = (G + kDecodeHeads - 1) / kDecodeHeads;
   decode::list_rows(p, rows, 16 * NT);
-  const int64_t total = before[p.rows] * H, step = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32);
-  for (int64_t x = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5); x < total; x += step) {
+  const int total = before[p.rows] * H, step = gridDim.x * (blockDim.x / 32);
+  for (int x = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); x < total; x += step) {
     decode::Place at;
-    at.find(p, rows, H, x);  // seg: the key head
-    const int64_t first = before[at.row] * H * hgroups + static_cast<int64_t>(at.seg) * hgroups * at.tiles + at.tile;
+    at.find(p, rows, 1, x);
+    const int first = (before[at.row] * H + at.kvh * at.tiles) * hgroups + at.tile;
     float w[4 * NT] = {};
     for (int hg = 0; hg < hgroups; ++hg) {
       const int h = hg * kDecodeHeads + g;
-      const int64_t tile = first + static_cast<int64_t>(hg) * at.tiles;
+      const int64_t tile = first + hg * at.tiles;
       if (h >= G || tile >= ws.score_tiles) continue;
-      const float lse = ws.lse[at.row * p.c.n_heads + at.seg * G + h];
+      const float lse = ws.lse[at.row * p.c.n_heads + at.kvh * G + h];
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         const float4 s = *reinterpret_cast<const float4*>(ws.scores + ((tile * NT + u) * 32 + lane) * 4);
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const 
 #pragma unroll
     for (int i = 1; i < 4 * NT; ++i) add = g == i ? w[i] : add;
     const int64_t slot = slot_of(p.c, p.t, at.row, n);
-    if (slot >= 0) p.c.weight[slot + static_cast<int64_t>(at.seg) * p.c.page_size] += add;
+    if (slot >= 0) p.c.weight[slot + static_cast<int64_t>(at.kvh) * p.c.page_size] += add;
   }
 }
 
@@ -97,7 +98,7 @@ int decode_tile(const PagedView& c) {
 
 size_t decode_part_floats(const PagedView& c, int sms) {
   const DecodePlan d = decode_plan(c, sms);
-  return static_cast<size_t>(2) * d.grid * d.warps * kDecodeHeads * (c.head_dim + 2);
+  return static_cast<size_t>(2) * d.grid * d.warps * kDecodeHeads * (padded_head(c) + 2);
 }
 
 int decode_workers(const PagedView& c, int sms) {
@@ -107,10 +108,14 @@ int decode_workers(const PagedView& c, int sms) {
 
 cudaError_t launch_paged_decode(const DecodeParams& all, const DecodeScratch& ws, int sms, cudaStream_t st) {
   const DecodePlan plan = decode_plan(all.c, sms);
-  for (int r0 = 0; r0 < all.rows; r0 += kDecodeMaxRows) {
+  // Rows of one launch: their tiles are numbered in 32 bits.
+  const int G = all.c.n_heads / all.c.kv_heads, segs = all.c.kv_heads * ((G + kDecodeHeads - 1) / kDecodeHeads);
+  const int64_t most = (static_cast<int64_t>(all.t.max_pages) * all.c.page_size / decode_tile(all.c) + 1) * segs;
+  const int chunk = static_cast<int>(std::min<int64_t>(kDecodeMaxRows, INT32_MAX / most));
+  for (int r0 = 0; r0 < all.rows; r0 += chunk) {
     DecodeParams p = all;
     const int act = all.q_dtype == MXMOE_F32 ? 4 : 2, oact = all.out_dtype == MXMOE_F32 ? 4 : 2;
-    p.rows = std::min(kDecodeMaxRows, all.rows - r0);
+    p.rows = std::min(chunk, all.rows - r0);
     p.q = static_cast<const char*>(all.q) + r0 * all.q_row * act;
     p.out = static_cast<char*>(all.out) + r0 * all.out_row * oact;
     p.lens += r0;

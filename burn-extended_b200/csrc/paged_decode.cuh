@@ -21,6 +21,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "../../include/mxmoe.h"
 #include "launch_util.h"
 #include "paged.h"
@@ -32,7 +34,7 @@ constexpr int kDecodeMaxStages = 6;
 // How one launch is laid out; set by decode_plan in paged_decode.cu.
 struct DecodePlan {
   int warps, stages;
-  int stage_bytes;  // K rows, then V rows; room for 8 x (head_dim + 8) floats
+  int stage_bytes;  // K rows, then V rows; room for a warp's 8 x head_dim floats
   int smem;         // of the block: the warps' rings, and 128 bytes that a read past the last row may touch
   int grid;
 };
@@ -118,49 +120,81 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 __device__ __forceinline__ float lo_of(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_of(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
 
-__device__ __forceinline__ float ld_act(const void* p, int dtype, int64_t i) {
-  return dtype == MXMOE_F32 ? static_cast<const float*>(p)[i]
-                            : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
+// The queries of up to 8 heads on their way to shared memory: lane l holds
+// columns 4 (l + 32 i) of [8][HDT], zeros past `heads` and head_dim.  Loaded one
+// segment ahead, since under a full memory pipe the answer takes microseconds.
+template <int HDT, bool X>
+struct Queries {
+  using Quad = typename std::conditional<X, float4, uint2>::type;  // bf16 queries stay packed
+  static constexpr int kQuads = kDecodeHeads * HDT / 128;
+  Quad x[kQuads];
+
+  __device__ __forceinline__ void load(const DecodeParams& p, int64_t base, int heads, int lane) {
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int e = lane + 32 * i, h = e / (HDT / 4), c = 4 * (e % (HDT / 4));
+      const int64_t at = base + h * p.q_head + c;
+      x[i] = Quad{};
+      if (h >= heads || c >= p.c.head_dim) continue;
+      if (X && p.q_dtype == MXMOE_F32) {
+        const float* q = static_cast<const float*>(p.q) + at;
+        set(i, p.q_wide ? *reinterpret_cast<const float4*>(q) : make_float4(q[0], q[1], q[2], q[3]));
+      } else {
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
+        const uint2 u = p.q_wide ? *reinterpret_cast<const uint2*>(q)
+                                 : make_uint2(q[0] | static_cast<uint32_t>(q[1]) << 16, q[2] | static_cast<uint32_t>(q[3]) << 16);
+        set(i, u);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float* to, int lane) const {
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) *reinterpret_cast<float4*>(to + 4 * (lane + 32 * i)) = wide(x[i]);
+  }
+
+ private:
+  static __device__ __forceinline__ float4 wide(uint2 u) { return make_float4(lo_of(u.x), hi_of(u.x), lo_of(u.y), hi_of(u.y)); }
+  static __device__ __forceinline__ float4 wide(float4 v) { return v; }
+  __device__ __forceinline__ void set(int i, uint2 u) { put(x[i], u); }
+  __device__ __forceinline__ void set(int i, float4 v) { put(x[i], v); }
+  static __device__ __forceinline__ void put(uint2& d, uint2 u) { d = u; }
+  static __device__ __forceinline__ void put(float4& d, uint2 u) { d = wide(u); }
+  static __device__ __forceinline__ void put(float4& d, float4 v) { d = v; }
+  static __device__ __forceinline__ void put(uint2&, float4) {}
+};
 
 // ---- the cache's element types ----
 //
 // Each has: Q, the query operand; load(), which fills it for lane (g, t) =
-// (lane / 4, lane % 4) from head g's row; scores(), s[4] of keys 2t, 2t + 1,
+// (lane / 4, lane % 4) from head g's row in shared memory; scores(), s[4] of keys 2t, 2t + 1,
 // 8 + 2t, 9 + 2t; and add(), o = o corr + p V over the tile's 16 keys.  HDT:
 // head_dim rounded up to the register arrays' size; X: 32-bit activations, a
 // third term each for queries and shares where two hold 16 bits only.
 
 template <int HDT, bool X>
 struct Bf16 {
+  static constexpr bool kWide = X;
   static constexpr int kElem = 2, rb = ring_row(HDT * 2), NT = tile_halves(HDT * 2);
   struct Q {
     uint32_t a[HDT / 16][X ? 6 : 2];
     float back;
   };
-  static __device__ __forceinline__ void load(Q& q, const void* src, int dtype, int64_t base, bool on, int hd, int t) {
+  static __device__ __forceinline__ void load(Q& q, const float* row, int t) {
     q.back = 1.0f;
 #pragma unroll
-    for (int s = 0; s < HDT / 16; ++s) {
+    for (int s = 0; s < HDT / 16; ++s)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int c = 16 * s + 8 * half + 2 * t;
-        float x = 0.0f, y = 0.0f;
-        if (on && c < hd) {
-          x = ld_act(src, dtype, base + c);
-          y = ld_act(src, dtype, base + c + 1);
-        }
-        const uint32_t h = pack_bf16(x, y);
+        const float2 x = *reinterpret_cast<const float2*>(row + 16 * s + 8 * half + 2 * t);
+        const uint32_t h = pack_bf16(x.x, x.y);
         q.a[s][half] = h;
         if (X) {
-          x -= lo_of(h);
-          y -= hi_of(h);
-          const uint32_t l = pack_bf16(x, y);
+          const float u = x.x - lo_of(h), v = x.y - hi_of(h);
+          const uint32_t l = pack_bf16(u, v);
           q.a[s][2 + half] = l;
-          q.a[s][4 + half] = pack_bf16(x - lo_of(l), y - hi_of(l));
+          q.a[s][4 + half] = pack_bf16(u - lo_of(l), v - hi_of(l));
         }
       }
-    }
   }
   static __device__ __forceinline__ void scores(float (&s)[4 * NT], const Q& q, uint32_t k, int lane) {
     float c[2 * NT][4] = {};
@@ -219,8 +253,9 @@ struct Bf16 {
       }
     }
   }
-  // The column of o[n][e].
-  static __device__ __forceinline__ int column(int n, int e, int t) { return 8 * n + 2 * t + e; }
+  // The columns of o[n]: the first, and how far the second is.
+  static constexpr int kApart = 1;
+  static __device__ __forceinline__ int column(int n, int t) { return 8 * n + 2 * t; }
 };
 
 // 8-bit keys and values widen to f16 without loss.  A query row is scaled by a
@@ -230,18 +265,19 @@ struct Bf16 {
 // agree: lane t takes bytes 4t to 4t + 3 of a key's 16, as one ldmatrix gives.
 template <int HDT, bool X>
 struct E4m3 {
+  static constexpr bool kWide = X;
   static constexpr int kElem = 1, rb = ring_row(HDT), NT = tile_halves(HDT);
   struct Q {
     uint32_t a[HDT / 16][4];
     float back;
   };
-  static __device__ __forceinline__ void load(Q& q, const void* src, int dtype, int64_t base, bool on, int hd, int t) {
+  static __device__ __forceinline__ void load(Q& q, const float* row, int t) {
     float top = 0.0f;
 #pragma unroll
-    for (int s = 0; s < HDT / 16; ++s)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (on && 16 * s < hd) top = fmaxf(top, fabsf(ld_act(src, dtype, base + 16 * s + 4 * t + e)));
+    for (int s = 0; s < HDT / 16; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(row + 16 * s + 4 * t);
+      top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+    }
     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
     const int ex = (__float_as_uint(top) >> 23) & 255;
@@ -252,15 +288,11 @@ struct E4m3 {
     for (int s = 0; s < HDT / 16; ++s)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float x = 0.0f, y = 0.0f;
-        if (on && 16 * s < hd) {
-          x = ld_act(src, dtype, base + 16 * s + 4 * t + 2 * half) * f;
-          y = ld_act(src, dtype, base + 16 * s + 4 * t + 2 * half + 1) * f;
-        }
-        const uint32_t h = pack_f16(x, y);
+        const float2 x = *reinterpret_cast<const float2*>(row + 16 * s + 4 * t + 2 * half);
+        const uint32_t h = pack_f16(x.x * f, x.y * f);
         const __half2 hh = *reinterpret_cast<const __half2*>(&h);
         q.a[s][half] = h;
-        q.a[s][2 + half] = X ? pack_f16(x - __low2float(hh), y - __high2float(hh)) : 0;
+        q.a[s][2 + half] = X ? pack_f16(x.x * f - __low2float(hh), x.y * f - __high2float(hh)) : 0;
       }
   }
   static __device__ __forceinline__ uint32_t widen(uint32_t two) {
@@ -325,13 +357,15 @@ struct E4m3 {
       }
     }
   }
-  static __device__ __forceinline__ int column(int n, int e, int t) { return 32 * (n / 4) + 8 * t + 4 * e + n % 4; }
+  static constexpr int kApart = 4;
+  static __device__ __forceinline__ int column(int n, int t) { return 32 * (n / 4) + 8 * t + n % 4; }
 };
 
 // 32-bit keys and values as two tf32 terms each, cut off so that the second is
 // exact: 21 bits of either operand.
 template <int HDT, bool X>
 struct F32 {
+  static constexpr bool kWide = true;
   static constexpr int kElem = 4, rb = ring_row(HDT * 4), NT = tile_halves(HDT * 4);
   struct Q {
     uint32_t a[HDT / 8][4];
@@ -339,13 +373,13 @@ struct F32 {
   };
   static __device__ __forceinline__ uint32_t top(float x) { return __float_as_uint(x) & 0xFFFFE000u; }
   static __device__ __forceinline__ uint32_t rest(float x) { return __float_as_uint(x - __uint_as_float(top(x))); }
-  static __device__ __forceinline__ void load(Q& q, const void* src, int dtype, int64_t base, bool on, int hd, int t) {
+  static __device__ __forceinline__ void load(Q& q, const float* row, int t) {
     q.back = 1.0f;
 #pragma unroll
     for (int s = 0; s < HDT / 8; ++s)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float x = on && 8 * s < hd ? ld_act(src, dtype, base + 8 * s + 4 * half + t) : 0.0f;
+        const float x = row[8 * s + 4 * half + t];
         q.a[s][half] = top(x);
         q.a[s][2 + half] = rest(x);
       }
@@ -399,14 +433,15 @@ struct F32 {
       }
     }
   }
-  static __device__ __forceinline__ int column(int n, int e, int t) { return 32 * (n / 4) + 8 * t + 4 * e + n % 4; }
+  static constexpr int kApart = 4;
+  static __device__ __forceinline__ int column(int n, int t) { return 32 * (n / 4) + 8 * t + n % 4; }
 };
 
 // ---- the list of tiles ----
 
 // Rows of a launch: cached length, and the tiles of the rows before.
 struct Rows {
-  int64_t* before;  // [rows + 1]
+  int* before;  // [rows + 1]
   int* len;         // [rows]
 };
 
@@ -414,10 +449,11 @@ __device__ __forceinline__ int first_key(int len, int window) { return window &&
 
 // All threads; ends with a barrier.
 __device__ __forceinline__ void list_rows(const DecodeParams& p, Rows r, int tile) {
-  __shared__ int64_t sums[32];
+  __shared__ int sums[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = blockDim.x >> 5;
   const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size;
-  int64_t base = 0;
+  int base = 0;
+#pragma unroll 1
   for (int r0 = 0; r0 < p.rows; r0 += blockDim.x) {
     const int i = r0 + threadIdx.x;
     int len = 0;
@@ -429,15 +465,16 @@ __device__ __forceinline__ void list_rows(const DecodeParams& p, Rows r, int til
       }
       r.len[i] = len;
     }
-    int64_t x = (len - first_key(len, p.window) + tile - 1) / tile;
+    int x = (len - first_key(len, p.window) + tile - 1) / tile;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+      const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
       if (lane >= o) x += y;
     }
     if (lane == 31) sums[warp] = x;
     __syncthreads();
-    int64_t all = base;
+    int all = base;
+#pragma unroll 1
     for (int w = 0; w < n_warps; ++w) {
       if (w == warp) x += all;
       all += sums[w];
@@ -450,145 +487,132 @@ __device__ __forceinline__ void list_rows(const DecodeParams& p, Rows r, int til
   __syncthreads();
 }
 
-// A place in the list: segment `seg` (key head x group of 8 query heads) of row
-// `row`, its tile `tile` of `tiles`.
+// A place in the list: tile `tile` of the `tiles` of a segment, which is a row,
+// a key head and up to 8 of the query heads that read it.
 struct Place {
-  int row, seg, tile, tiles, len, lo;
+  int row, kvh, part, tile, tiles, len, lo;
 
   __device__ __forceinline__ void at_row(const DecodeParams& p, Rows r, int i) {
     row = i;
-    tiles = static_cast<int>(r.before[i + 1] - r.before[i]);
+    tiles = r.before[i + 1] - r.before[i];
     len = r.len[i];
     lo = first_key(len, p.window);
   }
-  __device__ __forceinline__ void find(const DecodeParams& p, Rows r, int segs, int64_t x) {
+  // Tile x of the list, in which a row has `parts` segments per key head.
+  __device__ __forceinline__ void find(const DecodeParams& p, Rows r, int parts, int x) {
+    const int segs = p.c.kv_heads * parts;
     int a = 0, b = p.rows;  // before[a] segs <= x < before[b] segs
+#pragma unroll 1
     while (b - a > 1) {
       const int m = (a + b) >> 1;
       if (r.before[m] * segs <= x) a = m; else b = m;
     }
     at_row(p, r, a);
-    const int64_t y = x - r.before[a] * segs;
-    seg = static_cast<int>(y / tiles);
-    tile = static_cast<int>(y - static_cast<int64_t>(seg) * tiles);
+    const int y = x - r.before[a] * segs, seg = y / tiles;
+    tile = y - seg * tiles;
+    kvh = seg / parts;
+    part = seg - kvh * parts;
   }
-  __device__ __forceinline__ void next_segment(const DecodeParams& p, Rows r, int segs) {
+  __device__ __forceinline__ void next_segment(const DecodeParams& p, Rows r, int parts) {
     tile = 0;
-    if (++seg < segs) return;
-    seg = 0;
+    if (++part < parts) return;
+    part = 0;
+    if (++kvh < p.c.kv_heads) return;
+    kvh = 0;
     int i = row + 1;
+#pragma unroll 1
     while (r.before[i + 1] == r.before[i]) ++i;
     at_row(p, r, i);
   }
 };
 
-__device__ __forceinline__ void store_out(const DecodeParams& p, int row, int h, int col, float4 x) {
-  const int64_t o = row * p.out_row + h * p.out_head + col;
-  if (p.out_dtype == MXMOE_F32) {
-    float* y = static_cast<float*>(p.out) + o;
-    if (p.out_wide) {
-      *reinterpret_cast<float4*>(y) = x;
-    } else {
-      y[0] = x.x; y[1] = x.y; y[2] = x.z; y[3] = x.w;
-    }
-  } else {
-    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.out) + o;
-    if (p.out_wide) {
-      *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
-    } else {
-      y[0] = __float2bfloat16_rn(x.x); y[1] = __float2bfloat16_rn(x.y);
-      y[2] = __float2bfloat16_rn(x.z); y[3] = __float2bfloat16_rn(x.w);
-    }
-  }
+// Joins the sink's term (-inf: none) and the quiet softmax's to a head's maximum
+// and sum: the factor on its output, and the log of the normalizer.
+static __device__ __noinline__ float2 finish(float sink, int quiet, float m, float l) {
+  const float top = fmaxf(fmaxf(m, sink), quiet ? 0.0f : -INFINITY);
+  if (top == -INFINITY && l == 0.0f) return make_float2(0.0f, -INFINITY);  // no key, or every score -inf
+  const float f = exp_diff(m, top), sum = l * f + exp_diff(sink, top) + (quiet ? exp_diff(0.0f, top) : 0.0f);
+  return make_float2(f / sum, top + logf(sum));
 }
 
-// A head's maximum and sum so far, and four columns of its output.
-struct Joined {
-  float top = -INFINITY, sum = 0.0f;
-  float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-
-  __device__ __forceinline__ void add(float m, float l, float4 o) {
-    const float t = fmaxf(top, m), a = exp_diff(top, t), b = exp_diff(m, t);
-    top = t;
-    sum = fmaf(l, b, sum * a);
-    acc.x = fmaf(o.x, b, acc.x * a);
-    acc.y = fmaf(o.y, b, acc.y * a);
-    acc.z = fmaf(o.z, b, acc.z * a);
-    acc.w = fmaf(o.w, b, acc.w * a);
-  }
-};
-
-// Joins the sink's and the quiet softmax's terms to a head's maximum and sum:
-// the factor on its output, and the log of the normalizer.
-__device__ __forceinline__ float finish(const DecodeParams& p, int h, float m, float l, float& lse) {
-  float top = m;
-  if (p.sinks) top = fmaxf(top, p.sinks[h]);
-  if (p.quiet) top = fmaxf(top, 0.0f);
-  if (top == -INFINITY && l == 0.0f) {  // no key, or every score -inf
-    lse = -INFINITY;
-    return 0.0f;
-  }
-  const float f = exp_diff(m, top);
-  float sum = l * f;
-  if (p.sinks) sum += exp_diff(p.sinks[h], top);
-  if (p.quiet) sum += exp_diff(0.0f, top);
-  lse = top + logf(sum);
-  return f / sum;
-}
-
-// Four finished columns of a head, and with the first its normalizer.
-__device__ __forceinline__ void write_head(const DecodeParams& p, const DecodeScratch& ws, int row, int h, int c, float vs,
-                                           const Joined& j) {
-  float lse;
-  const float f = finish(p, h, j.top, j.sum, lse) * vs;
-  store_out(p, row, h, c, make_float4(j.acc.x * f, j.acc.y * f, j.acc.z * f, j.acc.w * f));
-  if (c != 0) return;
+__device__ __forceinline__ void store_lse(const DecodeParams& p, const DecodeScratch& ws, int row, int h, float lse) {
   if (p.lse) p.lse[static_cast<int64_t>(row) * p.c.n_heads + h] = lse;
   if (p.track) ws.lse[row * p.c.n_heads + h] = lse;
+}
+
+// Two finished columns of a head; `apart` is 1 or 4.
+template <int kApart>
+__device__ __forceinline__ void store_out(const DecodeParams& p, int row, int h, int col, float x, float y) {
+  const int64_t o = row * p.out_row + h * p.out_head + col;
+  const int hd = p.c.head_dim;
+  if (p.out_dtype == MXMOE_F32) {
+    float* d = static_cast<float*>(p.out) + o;
+    if (col < hd) d[0] = x;
+    if (col + kApart < hd) d[kApart] = y;
+  } else {
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.out) + o;
+    if (kApart == 1 && p.out_wide) {
+      if (col < hd) *reinterpret_cast<uint32_t*>(d) = pack_bf16(x, y);
+    } else {
+      if (col < hd) d[0] = __float2bfloat16_rn(x);
+      if (col + kApart < hd) d[kApart] = __float2bfloat16_rn(y);
+    }
+  }
 }
 
 template <class C, int HDT>
 __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
     attend_kernel(const DecodeParams p, const DecodeScratch ws, const DecodePlan plan) {
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ int64_t before[kDecodeMaxRows + 1];
+  __shared__ int before[kDecodeMaxRows + 1];
   __shared__ int len_of[kDecodeMaxRows];
-  __shared__ int arrived[kDecodeWarps], join_at[kDecodeWarps];
+  __shared__ int arrived[kDecodeWarps][2], join_at[kDecodeWarps];
   __shared__ float join_ml[kDecodeWarps][kDecodeHeads][2];
   __shared__ uint32_t there[kDecodeWarps][kDecodeMaxStages];  // which keys of a stage are in the cache
   const Rows rows{before, len_of};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int hd = p.c.head_dim, H = p.c.kv_heads, G = p.c.n_heads / H;
-  const int hgroups = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * hgroups;
-  constexpr int rb = C::rb, ldo = HDT + 8, NT = C::NT, kTile = 16 * NT;
-  const int W = plan.warps;
-  const uint32_t mine = smem_u32(ring) + warp * plan.stages * plan.stage_bytes;
+  const int parts = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * parts, W = plan.warps;
+  constexpr int rb = C::rb, NT = C::NT, kTile = 16 * NT, kPairs = HDT / 8;  // column pairs of a lane
+  uint8_t* const mine = ring + warp * plan.stages * plan.stage_bytes;
   list_rows(p, rows, kTile);
-  const int64_t total = before[p.rows] * segs;
+  const int total = before[p.rows] * segs;
 
   // Rows without keys: zeros.
+#pragma unroll 1
   for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
     if (before[r + 1] != before[r]) continue;
-    for (int i = threadIdx.x; i < p.c.n_heads * (hd / 4); i += blockDim.x)
-      write_head(p, ws, r, i / (hd / 4), 4 * (i % (hd / 4)), 0.0f, Joined());
+#pragma unroll 1
+    for (int i = threadIdx.x; i < p.c.n_heads * hd; i += blockDim.x) {
+      const int h = i / hd;
+      const int64_t o = r * p.out_row + h * p.out_head + (i - h * hd);
+      if (p.out_dtype == MXMOE_F32)
+        static_cast<float*>(p.out)[o] = 0.0f;
+      else
+        static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(0.0f);
+      if (i == h * hd) store_lse(p, ws, r, h, finish(p.sinks ? p.sinks[h] : -INFINITY, p.quiet, -INFINITY, 0.0f).y);
+    }
   }
   if (total == 0) return;
 
-  // Warps of a worker: one where every warp has many tiles (no join in shared
-  // memory), else up to half the tiles of a mean segment, so that short work
-  // spreads.
+  // Warps of a worker.  Alone, a warp waits for no other; but a segment should
+  // not fall to more than about four workers, whose parts one of them has to
+  // read, and no more warps than a mean segment has tiles.
   int wg = 1;
-  if (total < 16LL * W * gridDim.x) {
-    const int64_t mean = total / (static_cast<int64_t>(p.rows) * segs);
-    while (wg < W && 2 * wg < mean) wg <<= 1;
-  }
-  const int group = warp / wg, in_group = warp - group * wg;
-  // No more workers than give each of their warps a tile.
-  int64_t n_workers = static_cast<int64_t>(gridDim.x) * (W / wg);
-  if (n_workers > (total + wg - 1) / wg) n_workers = (total + wg - 1) / wg;
-  const int64_t worker = static_cast<int64_t>(group) * gridDim.x + blockIdx.x;
+  const int n_segs = p.rows * segs, warps = W * static_cast<int>(gridDim.x);
+#pragma unroll 1
+  while (wg < W && 4 * wg * n_segs < warps && wg * n_segs < total) wg <<= 1;
+  const int group = warp / wg, in_group = warp - group * wg, w0 = group * wg, tid = threadIdx.x - w0 * 32, nt = 32 * wg;
+  // No more workers than give each of their warps a tile.  The first `more`
+  // workers have one tile above the others.
+  const int n_workers = min(warps / wg, (total + wg - 1) / wg), each = total / n_workers, more = total - each * n_workers;
+  const int worker = group * gridDim.x + blockIdx.x;
   if (worker >= n_workers) return;
-  const int64_t begin = total * worker / n_workers, end = total * (worker + 1) / n_workers;
+  const int begin = worker * each + min(worker, more), end = begin + each + (worker < more ? 1 : 0);
+  auto worker_of = [&](int x) {
+    const int edge = more * (each + 1);
+    return x < edge ? x / (each + 1) : more + (x - edge) / each;
+  };
   auto group_sync = [&]() {
     if (wg == 1)
       __syncwarp();
@@ -596,202 +620,267 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * wg) : "memory");
   };
 
-  // What this warp loads next: its tile, and each lane's page of the tile's key
-  // of that number, read one tile ahead.
+  // The tiles that this warp loads next: each lane's row of the pools for the
+  // tile's key of that number, two tiles ahead of its use, as the page table's
+  // answer takes that long.
   Place ld;
-  ld.find(p, rows, segs, begin);
-  int64_t ld_left = end - begin;
-  int ld_off = in_group, ld_tile = 0, page = -1, slot = 0;
-  bool ld_on = true;
-  auto look_ahead = [&]() {
-    while (true) {
-      if (ld_left <= 0) {
-        ld_on = false;
-        return;
-      }
-      const int n = static_cast<int>(min(static_cast<int64_t>(ld.tiles - ld.tile), ld_left));
-      if (ld_off < n) break;
-      ld_left -= n;
-      ld_off = in_group;
-      if (ld_left > 0) ld.next_segment(p, rows, segs);
-    }
-    ld_tile = ld.tile + ld_off;
-    ld_off += wg;
-    const int n = ld.lo + ld_tile * kTile + lane % kTile;
-    page = -1;
-    if (n < ld.len) {
-      const int pi = page_of(p.c, n);
-      slot = n - pi * p.c.page_size;
-      page = __ldg(p.t.tables + ld.row * p.t.stride + pi);
-      if (page < 0 || page >= p.c.n_pages) page = -2;
-    }
+  ld.find(p, rows, parts, begin);
+  Place at = ld;
+  // The next segment's queries and its heads' sinks.
+  Queries<HDT, C::kWide> queries;
+  float sink_next = -INFINITY;
+  auto fetch = [&](const Place& of) {
+    const int h0 = of.kvh * G + of.part * kDecodeHeads, heads = min(kDecodeHeads, G - of.part * kDecodeHeads);
+    queries.load(p, of.row * p.q_row + h0 * p.q_head, heads, lane);
+    if (p.sinks && g < heads) sink_next = p.sinks[h0 + g];
   };
-  int ld_stage = 0;
+  fetch(at);
+  struct Ahead {
+    int page, slot, kvh;  // kvh -1: no tile; page -1: no key, -2: out of range
+  };
+  Ahead next{-1, 0, -1}, after{-1, 0, -1};
+  int ld_left = end - begin, ld_off = in_group, ld_stage = 0;
+  int prime = plan.stages + 1;  // loads before the first tile: two that only look ahead, then all stages but one
+  // Loads the next tile into the stage that is free, and looks two further.
   auto load_tile = [&]() {
-    if (ld_on) {
-      if (page == -2) atomicOr(p.c.status, kPagedBadPage);
-      const uint32_t keys = __ballot_sync(0xFFFFFFFFu, page >= 0);
+    if (next.kvh >= 0) {
+      if (next.page == -2) atomicOr(p.c.status, kPagedBadPage);
+      const uint32_t keys = __ballot_sync(0xFFFFFFFFu, next.page >= 0);
       if (lane == 0) there[warp][ld_stage] = keys;
-      const int kvh = ld.seg / hgroups;
-      const int64_t row = page < 0 ? -1
-                                   : ((static_cast<int64_t>(page) * H + kvh) * p.c.page_size + slot) * (hd * C::kElem);
-      const uint32_t ks = mine + ld_stage * plan.stage_bytes, vs = ks + kTile * rb;
+      const int row = next.page < 0 ? -1 : (next.page * H + next.kvh) * p.c.page_size + next.slot;
+      const uint32_t ks = smem_u32(mine) + ld_stage * plan.stage_bytes, vs = ks + kTile * rb;
       constexpr int kPieces = HDT * C::kElem / 16;  // 16 bytes each, zeros past head_dim
       constexpr int kLanes = kPieces % 8 == 0 ? 8 : 4, kKeys = 32 / kLanes;
       const int piece = lane % kLanes * 16;
 #pragma unroll
       for (int i = 0; i < kTile / kKeys; ++i) {
         const int key = i * kKeys + lane / kLanes;
-        const int64_t at = __shfl_sync(0xFFFFFFFFu, row, key);
-        const int64_t from = at < 0 ? 0 : at;
-        const uint8_t *kf = static_cast<const uint8_t*>(p.c.k) + from, *vf = static_cast<const uint8_t*>(p.c.v) + from;
+        const int from = __shfl_sync(0xFFFFFFFFu, row, key);
+        const int64_t byte = static_cast<int64_t>(max(from, 0)) * (hd * C::kElem);
+        const uint8_t *kf = static_cast<const uint8_t*>(p.c.k) + byte, *vf = static_cast<const uint8_t*>(p.c.v) + byte;
 #pragma unroll
         for (int j = 0; j < (kPieces + kLanes - 1) / kLanes; ++j) {
           const int c = j * kLanes * 16 + piece;
           if (kPieces % kLanes && c >= kPieces * 16) break;
-          const bool in = at >= 0 && c < hd * C::kElem;
+          const bool in = from >= 0 && c < hd * C::kElem;
           cp16(ks + key * rb + c, kf + (in ? c : 0), in ? 16 : 0);
           cp16(vs + key * rb + c, vf + (in ? c : 0), in ? 16 : 0);
         }
       }
-      look_ahead();
     }
-    cp_commit();
-    if (++ld_stage == plan.stages) ld_stage = 0;
+    if (prime < plan.stages) {
+      cp_commit();
+      if (++ld_stage == plan.stages) ld_stage = 0;
+    }
+    next = after;
+    after.kvh = -1;
+    int n = min(ld.tiles - ld.tile, ld_left);
+#pragma unroll 1
+    while (ld_off >= n && ld_left > 0) {
+      ld_left -= n;
+      ld_off = in_group;
+      if (ld_left > 0) ld.next_segment(p, rows, parts);
+      n = min(ld.tiles, ld_left);
+    }
+    if (ld_left <= 0) return;
+    const int key = ld.lo + (ld.tile + ld_off) * kTile + lane % kTile;
+    ld_off += wg;
+    after = Ahead{-1, 0, ld.kvh};
+    if (key < ld.len) {
+      const int pi = page_of(p.c, key);
+      after.slot = key - pi * p.c.page_size;
+      after.page = __ldg(p.t.tables + ld.row * p.t.stride + pi);
+      if (after.page < 0 || after.page >= p.c.n_pages) after.page = -2;
+    }
   };
-  look_ahead();
-  for (int i = 0; i + 1 < plan.stages; ++i) load_tile();
 
-  Place at;
-  at.find(p, rows, segs, begin);
-  int stage = 0;
-  for (int64_t x = begin; x < end;) {
-    const int n = static_cast<int>(min(static_cast<int64_t>(at.tiles - at.tile), end - x));
-    const int kvh = at.seg / hgroups, h0 = kvh * G + (at.seg - kvh * hgroups) * kDecodeHeads;
-    const int heads = min(kDecodeHeads, (kvh + 1) * G - h0);
-    typename C::Q q;
-    C::load(q, p.q, p.q_dtype, at.row * p.q_row + static_cast<int64_t>(h0 + g) * p.q_head, g < heads, hd, t);
-    const float ks = p.scale * q.back * (p.c.k_scale ? p.c.k_scale[kvh] : 1.0f);
-    const float* bias = p.bias && g < heads ? p.bias + at.row * p.bias_row + (h0 + g) * p.bias_head : nullptr;
+  constexpr int kPartPairs = 32 * kPairs + kDecodeHeads;  // [pairs][lane] of o, then (m, l) by head
+  float2* const part_of = reinterpret_cast<float2*>(ws.part);
+  // Segments of this worker that others hold too: the one that it begins in
+  // (side 0) and the one that it ends in (side 1); row -1: none.
+  int split_row[2] = {-1, -1}, split_kvh[2], split_part[2], split_first[2], split_last[2];
+  int stage = 0, side = -1;
+  for (int x = begin;;) {
+    int row = at.row, kvh = at.kvh, part = at.part;
+    float2* to = nullptr;  // where this worker's part goes; null: the output
     float m = -INFINITY, l = 0.0f;
-    float o[HDT / 8][2];
+    float o[kPairs][2];
 #pragma unroll
-    for (int i = 0; i < HDT / 8; ++i) o[i][0] = o[i][1] = 0.0f;
-
-    for (int j = in_group; j < n; j += wg) {
-      cp_wait_for(plan.stages - 2);
-      __syncwarp();
-      load_tile();  // into the stage that the tile before this one left
-      const uint32_t k = mine + stage * plan.stage_bytes, v = k + kTile * rb;
-      float s[4 * NT], w[4 * NT];
-      C::scores(s, q, k, lane);
-      const uint32_t keys = there[warp][stage] >> (2 * t);
-      float top = m;
-#pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) {
-        const int e = 8 * (i >> 1) + (i & 1);
-        s[i] *= ks;
-        if (bias) {
-          const int n = at.lo + (at.tile + j) * kTile + e + 2 * t;
-          if (n < p.bias_len && n < at.len) s[i] += bias[n];
+    for (int i = 0; i < kPairs; ++i) o[i][0] = o[i][1] = 0.0f;
+    float sink = sink_next;
+    if (x < end) {
+      const int n = min(at.tiles - at.tile, end - x), h0 = kvh * G + part * kDecodeHeads;
+      if (n < at.tiles) {
+        const int e = at.tile == 0 ? 1 : 0;
+        const int s0 = before[row] * segs + (kvh * parts + part) * at.tiles;
+        split_row[e] = row;
+        split_kvh[e] = kvh;
+        split_part[e] = part;
+        split_first[e] = worker_of(s0);
+        split_last[e] = worker_of(s0 + at.tiles - 1);
+        to = part_of + (2 * worker + e) * kPartPairs;
+      }
+      // the queries go through the stage that is free until the next load
+      typename C::Q q;
+      {
+        float* qs = reinterpret_cast<float*>(mine + ld_stage * plan.stage_bytes);
+        queries.store(qs, lane);
+        __syncwarp();
+        C::load(q, qs + g * HDT, t);
+        __syncwarp();
+      }
+      const float ks = p.scale * q.back * (p.c.k_scale ? p.c.k_scale[kvh] : 1.0f);
+      const float* bias = p.bias && part * kDecodeHeads + g < G ? p.bias + row * p.bias_row + (h0 + g) * p.bias_head : nullptr;
+      if (x + n < end) {
+        Place then = at;
+        then.next_segment(p, rows, parts);
+        fetch(then);
+      }
+#pragma unroll 1
+      for (int j = in_group; j < n;) {
+        if (prime == 0) {
+          cp_wait_for(plan.stages - 2);
+          __syncwarp();
         }
-        if (!(keys >> e & 1)) s[i] = -INFINITY;
-        top = fmaxf(top, s[i]);
-      }
-      if (p.track && x + j < ws.score_tiles) {
+        load_tile();
+        if (prime > 0) {
+          --prime;
+          continue;
+        }
+        const uint32_t k = smem_u32(mine) + stage * plan.stage_bytes, v = k + kTile * rb;
+        float s[4 * NT], w[4 * NT];
+        C::scores(s, q, k, lane);
+        const uint32_t keys = there[warp][stage] >> (2 * t);
+        float top = m;
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-          *reinterpret_cast<float4*>(ws.scores + (((x + j) * NT + u) * 32 + lane) * 4) =
-              make_float4(s[4 * u], s[4 * u + 1], s[4 * u + 2], s[4 * u + 3]);
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      const float corr = exp_diff(m, top);
-      float sum = 0.0f;
+        for (int i = 0; i < 4 * NT; ++i) s[i] *= ks;
+        if (bias) {
 #pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) {
-        w[i] = exp_diff(s[i], top);
-        sum += w[i];
+          for (int i = 0; i < 4 * NT; ++i) {
+            const int key = at.lo + (at.tile + j) * kTile + 8 * (i >> 1) + (i & 1) + 2 * t;
+            if (key < p.bias_len && key < at.len) s[i] += bias[key];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * NT; ++i) {
+          if (!(keys >> (8 * (i >> 1) + (i & 1)) & 1)) s[i] = -INFINITY;
+          top = fmaxf(top, s[i]);
+        }
+        if (p.track && x + j < ws.score_tiles) {
+#pragma unroll
+          for (int u = 0; u < NT; ++u)
+            *reinterpret_cast<float4*>(ws.scores + ((static_cast<int64_t>(x + j) * NT + u) * 32 + lane) * 4) =
+                make_float4(s[4 * u], s[4 * u + 1], s[4 * u + 2], s[4 * u + 3]);
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        const float corr = exp_diff(m, top);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4 * NT; ++i) {
+          w[i] = exp_diff(s[i], top);
+          sum += w[i];
+        }
+        l = fmaf(l, corr, sum);
+        m = top;
+        C::add(o, w, corr, v, lane);
+        __syncwarp();
+        if (++stage == plan.stages) stage = 0;
+        j += wg;
       }
-      l = fmaf(l, corr, sum);
-      m = top;
-      C::add(o, w, corr, v, lane);
-      __syncwarp();
-      if (++stage == plan.stages) stage = 0;
+      l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+      l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+      x += n;
+      if (x < end) at.next_segment(p, rows, parts);
+    } else {
+      // All tiles are done.  Of the workers that hold a split segment, the last
+      // to come here joins the parts, each warp every wg-th of them.
+      if (side < 0) {
+        cp_wait<0>();
+        if (split_row[0] < 0 && split_row[1] < 0) return;
+        __threadfence();
+        group_sync();
+        if (tid < 2 && split_row[tid] >= 0) arrived[group][tid] = atomicAdd(ws.tickets + split_first[tid], 1);
+        group_sync();
+      }
+      while (++side < 2)
+        if (split_row[side] >= 0 && arrived[group][side] == split_last[side] - split_first[side]) break;
+      if (side >= 2) return;
+      __threadfence();
+      row = split_row[side];
+      kvh = split_kvh[side];
+      part = split_part[side];
+      if (p.sinks && part * kDecodeHeads + g < G) sink = p.sinks[kvh * G + part * kDecodeHeads + g];
+      const int first = split_first[side], last = split_last[side];
+      if (tid == 0) ws.tickets[first] = 0;
+#pragma unroll 2
+      for (int w = first + in_group; w <= last; w += wg) {
+        const float2* from = part_of + (2 * w + (w == first ? 1 : 0)) * kPartPairs;
+        const float2 ml = __ldcg(from + 32 * kPairs + g);
+        float2 y[kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) y[i] = __ldcg(from + 32 * i + lane);
+        const float top = fmaxf(m, ml.x), a = exp_diff(m, top), b = exp_diff(ml.x, top);
+        m = top;
+        l = l * a + ml.y * b;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          o[i][0] = fmaf(y[i].x, b, o[i][0] * a);
+          o[i][1] = fmaf(y[i].y, b, o[i][1] * a);
+        }
+      }
     }
 
     // The group's warps join in shared memory, each in the stage that it loads
     // next: nothing uses that until then.
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-    const int at_stage = (warp * plan.stages + ld_stage) * plan.stage_bytes;
-    float* jo = reinterpret_cast<float*>(ring + at_stage) + g * ldo;
+    const int heads = min(kDecodeHeads, G - part * kDecodeHeads), h = kvh * G + part * kDecodeHeads + g;
+    float2* mo = reinterpret_cast<float2*>(mine + ld_stage * plan.stage_bytes);
 #pragma unroll
-    for (int i = 0; i < HDT / 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) jo[C::column(i, e, t)] = o[i][e];
+    for (int i = 0; i < kPairs; ++i) mo[32 * i + lane] = make_float2(o[i][0], o[i][1]);
     if (t == 0) {
       join_ml[warp][g][0] = m;
       join_ml[warp][g][1] = l;
     }
-    if (lane == 0) join_at[warp] = at_stage;
+    if (lane == 0) join_at[warp] = (warp * plan.stages + ld_stage) * plan.stage_bytes;
     group_sync();
-    const int w0 = group * wg, tid = threadIdx.x - w0 * 32, nt = 32 * wg;
-    const bool whole = n == at.tiles;
-    const int slot_floats = kDecodeHeads * (hd + 2), quads = hd / 4;
-    float* part = ws.part + (2 * worker + (at.tile == 0 ? 1 : 0)) * slot_floats;
-    const float vs = p.c.v_scale ? p.c.v_scale[kvh] : 1.0f;
-    for (int i = tid; i < heads * quads; i += nt) {
-      const int h = i / quads, c = 4 * (i - h * quads);
-      Joined j;
-      for (int w = w0; w < w0 + wg; ++w)
-        j.add(join_ml[w][h][0], join_ml[w][h][1], *reinterpret_cast<const float4*>(ring + join_at[w] + 4 * (h * ldo + c)));
-      if (whole) {
-        write_head(p, ws, at.row, h0 + h, c, vs, j);
-      } else {
-        *reinterpret_cast<float4*>(part + 4 * i) = j.acc;
-        if (c == 0) *reinterpret_cast<float2*>(part + kDecodeHeads * hd + 2 * h) = make_float2(j.top, j.sum);
-      }
-    }
-    if (!whole) {
-      // Workers first_w to last_w hold this segment; the last of them to come
-      // here joins their parts in order.
-      const int64_t s0 = before[at.row] * segs + static_cast<int64_t>(at.seg) * at.tiles, s1 = s0 + at.tiles;
-      const int64_t first_w = ((s0 + 1) * n_workers - 1) / total, last_w = (s1 * n_workers - 1) / total;
-      __threadfence();
-      group_sync();
-      if (tid == 0) arrived[group] = atomicAdd(ws.tickets + first_w, 1);
-      group_sync();
-      if (arrived[group] == static_cast<int>(last_w - first_w)) {
-        __threadfence();
-        if (tid == 0) ws.tickets[first_w] = 0;
-        constexpr int kAtOnce = 4;  // pieces of the output whose loads are in flight together
-        for (int i0 = tid; i0 < heads * quads; i0 += kAtOnce * nt) {
-          Joined j[kAtOnce];
-#pragma unroll 2
-          for (int64_t w = first_w; w <= last_w; ++w) {
-            const float* from = ws.part + (2 * w + (w == first_w ? 1 : 0)) * slot_floats;
+    // nt is a multiple of 32: a thread's head is its lane's for every pair
+    float top = -INFINITY, sum = 0.0f, e[kDecodeWarps];
+    const float2* from[kDecodeWarps];
 #pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) {
-              const int i = i0 + e * nt;
-              if (i >= heads * quads) break;
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + kDecodeHeads * hd) + i / quads);
-              j[e].add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(from) + i));
-            }
-          }
+    for (int w = 0; w < kDecodeWarps; ++w)
+      if (w < wg) top = fmaxf(top, join_ml[w0 + w][g][0]);
 #pragma unroll
-          for (int e = 0; e < kAtOnce; ++e) {
-            const int i = i0 + e * nt, h = i / quads;
-            if (i < heads * quads) write_head(p, ws, at.row, h0 + h, 4 * (i - h * quads), vs, j[e]);
-          }
-        }
-      }
+    for (int w = 0; w < kDecodeWarps; ++w) {
+      if (w >= wg) break;
+      e[w] = exp_diff(join_ml[w0 + w][g][0], top);
+      sum = fmaf(join_ml[w0 + w][g][1], e[w], sum);
+      from[w] = reinterpret_cast<const float2*>(ring + join_at[w0 + w]);
     }
-    group_sync();  // the joining buffers are free again
-    x += n;
-    if (x < end) at.next_segment(p, rows, segs);
+    float f = 1.0f;
+    if (to) {
+      if (t == 0 && tid < 32) to[32 * kPairs + g] = make_float2(top, sum);
+    } else if (g < heads) {
+      const float2 y = finish(sink, p.quiet, top, sum);
+      f = y.x * (p.c.v_scale ? p.c.v_scale[kvh] : 1.0f);
+      if (t == 0 && tid < 32) store_lse(p, ws, row, h, y.y);
+    }
+#pragma unroll 1
+    for (int i = tid; i < 32 * kPairs; i += nt) {
+      float a = 0.0f, b = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kDecodeWarps; ++w) {
+        if (w >= wg) break;
+        const float2 y = from[w][i];
+        a = fmaf(y.x, e[w], a);
+        b = fmaf(y.y, e[w], b);
+      }
+      if (to)
+        to[i] = make_float2(a, b);
+      else if (g < heads)
+        store_out<C::kApart>(p, row, h, C::column(i / 32, t), a * f, b * f);
+    }
+    group_sync();  // the stages are free again
   }
-  cp_wait<0>();
 }
 
 template <class C, int HDT>
