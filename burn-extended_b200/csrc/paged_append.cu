@@ -10,6 +10,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "../../include/mxmoe.h"
 #include "launch_util.h"
 #include "paged.h"
@@ -33,28 +35,225 @@ __device__ __forceinline__ void st_cache(void* pool, int dtype, int64_t i, float
     static_cast<uint8_t*>(pool)[i] = __nv_cvt_float_to_fp8(x * inv_scale, __NV_SATFINITE, __NV_E4M3);
 }
 
-// One block per token: the pairs of every query and key head, the columns
-// that pass, then the value rows.
-template <typename T>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
-  const int t = blockIdx.x, hd = p.c.head_dim, half = p.rot / 2;
-  const int nH = p.q ? p.c.n_heads : 0, H = p.k ? p.c.kv_heads : 0;
-  const int index = p.index ? p.index[t] : -1;
-  int pos = p.positions ? p.positions[t] : (index > 0 ? index : 0);
-  if (p.rot && (pos < 0 || pos >= p.n_positions)) {
-    if (threadIdx.x == 0 && p.c.status) atomicOr(p.c.status, kPagedBadPosition);
-    pos = 0;
+// Where a token goes, and how far it turns.
+struct Token {
+  int64_t slot;  // its cache slot of head 0, -1: not written
+  int pos;
+  const float *cs, *sn;  // its row of the table
+};
+
+__device__ __forceinline__ Token token_of(const AppendParams& p, int t) {
+  const int index = p.index ? __ldg(p.index + t) : -1, half = p.rot / 2;
+  Token k{-1, p.positions ? __ldg(p.positions + t) : (index > 0 ? index : 0), nullptr, nullptr};
+  if (p.rot && (k.pos < 0 || k.pos >= p.n_positions)) {
+    if (p.c.status) atomicOr(p.c.status, kPagedBadPosition);
+    k.cs = p.cos;
+    k.sn = p.sin;
+  } else {
+    k.cs = p.cos + static_cast<int64_t>(k.pos) * half;  // unread without a rotation
+    k.sn = p.sin + static_cast<int64_t>(k.pos) * half;
   }
-  int64_t slot = -1;
-  if (H && index >= 0) {
-    const int row = p.rows ? p.rows[t] : t;
+  if (p.k && index >= 0) {
+    const int row = p.rows ? __ldg(p.rows + t) : t;
     if (row < 0 || row >= p.t.n_rows)
       atomicOr(p.c.status, kPagedBadIndex);
     else
-      slot = slot_of(p.c, p.t, row, index);
+      k.slot = slot_of(p.c, p.t, row, index);
   }
-  const float* cs = p.cos + static_cast<int64_t>(pos) * half;  // unread without a rotation
-  const float* sn = p.sin + static_cast<int64_t>(pos) * half;
+  return k;
+}
+
+__device__ __forceinline__ void mark_slot(const AppendParams& p, const Token& k) {
+  if (k.slot < 0 || !(p.c.weight || p.c.position)) return;
+  for (int h = threadIdx.x; h < p.c.kv_heads; h += blockDim.x) {
+    const int64_t at = k.slot + static_cast<int64_t>(h) * p.c.page_size;
+    if (p.c.weight) p.c.weight[at] = 0.0f;
+    if (p.c.position) p.c.position[at] = k.pos;
+  }
+}
+
+// 16 bytes of activations as floats.
+template <typename T>
+struct Piece;
+template <>
+struct Piece<__nv_bfloat16> {
+  static constexpr int kN = 8;
+  uint4 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void open(float (&x)[8]) const {
+    const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(v[i] << 16);
+      x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
+    }
+  }
+};
+template <>
+struct Piece<float> {
+  static constexpr int kN = 4;
+  float4 u;
+  __device__ __forceinline__ void load(const float* p) { u = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void open(float (&x)[4]) const { x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; }
+};
+
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <int N>
+__device__ __forceinline__ void store(float* p, const float (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+}
+template <int N>
+__device__ __forceinline__ void store(__nv_bfloat16* p, const float (&x)[N]) {
+  if (N == 8)
+    *reinterpret_cast<uint4*>(p) = make_uint4(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4 % N], x[5 % N]),
+                                              bf16_pair(x[6 % N], x[7 % N]));
+  else
+    *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]));
+}
+template <int N>
+__device__ __forceinline__ void store_cache(void* pool, int dtype, int64_t at, const float (&x)[N], float inv) {
+  if (dtype == MXMOE_F32) {
+    store(static_cast<float*>(pool) + at, x);
+  } else if (dtype == MXMOE_BF16) {
+    store(static_cast<__nv_bfloat16*>(pool) + at, x);
+  } else {
+    uint32_t w[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i] * inv, x[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2] * inv, x[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+      w[i] = a | b << 16;
+    }
+    uint8_t* d = static_cast<uint8_t*>(pool) + at;
+    if (N == 8)
+      *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[N / 4 - 1]);
+    else
+      *reinterpret_cast<uint32_t*>(d) = w[0];
+  }
+}
+
+// One block per token; everything moves in 16-byte pieces.  A thread keeps one
+// unit of columns (a pair of pieces that turn together, or one piece) for
+// several heads, so the token's cosines are read once per thread; up to
+// kBatch heads' loads are in flight while the token's index, page and cosines
+// come.  Memory-bound: each value is read and written once.
+constexpr int kBatch = 3;
+template <typename T, bool kInterleaved, bool kMany>
+__global__ void __launch_bounds__(kMany ? 128 : 512, kMany ? 7 : 1) append_wide_kernel(const AppendParams p, int units, int per_pass) {
+  constexpr int N = Piece<T>::kN;
+  griddep_wait();
+  const int t = blockIdx.x, hd = p.c.head_dim, half = p.rot / 2;
+  const int nH = p.q ? p.c.n_heads : 0, H = p.k ? p.c.kv_heads : 0;
+  const int unit = threadIdx.x % units, first = threadIdx.x / units;
+  const bool on = first < per_pass;
+  const bool turns = unit * N < (kInterleaved ? p.rot : half);
+  const int ca = kInterleaved || turns ? unit * N : half + unit * N, cb = ca + half;
+  const bool two = !kInterleaved && turns;
+  Piece<T> a[kBatch], b[kBatch];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = h0 + i * per_pass;
+      if (!on || h >= nH + H) continue;
+      const T* x = h < nH ? static_cast<const T*>(p.q) + t * p.q_token + h * p.q_head
+                          : static_cast<const T*>(p.k) + t * p.k_token + (h - nH) * p.k_head;
+      a[i].load(x + ca);
+      if (two) b[i].load(x + cb);
+    }
+  };
+  load(first);
+  const int pieces = hd / N, v_all = H * pieces;
+  auto value_at = [&](int i) {
+    const int h = i / pieces;
+    return static_cast<const T*>(p.v) + t * p.v_token + h * p.v_head + (i - h * pieces) * N;
+  };
+  Piece<T> v;
+  if (threadIdx.x < v_all) v.load(value_at(threadIdx.x));
+  const Token k = token_of(p, t);
+  __align__(16) float c[N];  // interleaved: the first half of them
+  __align__(16) float s[N];
+  if (turns && on) {
+    const int from = kInterleaved ? unit * N / 2 : unit * N;
+constexpr int kCos = kInterleaved ? N / 2 : N, kAtOnce = kCos % 4 ? 2 : 4;
+#pragma unroll
+    for (int i = 0; i < kCos; i += kAtOnce) {
+      if (kAtOnce == 4) {
+        *reinterpret_cast<float4*>(c + i) = __ldg(reinterpret_cast<const float4*>(k.cs + from + i));
+        *reinterpret_cast<float4*>(s + i) = __ldg(reinterpret_cast<const float4*>(k.sn + from + i));
+      } else {
+        *reinterpret_cast<float2*>(c + i) = __ldg(reinterpret_cast<const float2*>(k.cs + from + i));
+        *reinterpret_cast<float2*>(s + i) = __ldg(reinterpret_cast<const float2*>(k.sn + from + i));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kCos; ++i) s[i] *= p.sign;
+  }
+#pragma unroll 1
+  for (int h0 = first; on && h0 < nH + H; h0 += kBatch * per_pass) {
+    if (h0 != first) load(h0);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = h0 + i * per_pass;
+      if (h >= nH + H) break;
+      float x[N], y[N];
+      a[i].open(x);
+      if (two) {
+        b[i].open(y);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float u = x[j], w = y[j];
+          x[j] = u * c[j] - w * s[j];
+          y[j] = w * c[j] + u * s[j];
+        }
+      } else if (turns) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+          const float u = x[j], w = x[j + 1];
+          x[j] = u * c[j / 2] - w * s[j / 2];
+          x[j + 1] = w * c[j / 2] + u * s[j / 2];
+        }
+      }
+      const int kh = h - nH;
+      T* out = kh < 0 ? static_cast<T*>(p.q_out) + t * p.qo_token + h * p.qo_head
+                      : (p.k_out ? static_cast<T*>(p.k_out) + t * p.ko_token + kh * p.ko_head : nullptr);
+      if (out) {
+        store(out + ca, x);
+        if (two) store(out + cb, y);
+      }
+      if (kh >= 0 && k.slot >= 0) {
+        const int64_t at = (k.slot + static_cast<int64_t>(kh) * p.c.page_size) * hd;
+        const float inv = p.c.k_scale ? 1.0f / __ldg(p.c.k_scale + kh) : 1.0f;
+        store_cache(p.c.k, p.c.dtype, at + ca, x, inv);
+        if (two) store_cache(p.c.k, p.c.dtype, at + cb, y, inv);
+      }
+    }
+  }
+  if (k.slot >= 0) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < v_all; i += blockDim.x) {
+      if (i >= static_cast<int>(blockDim.x)) v.load(value_at(i));
+      const int h = i / pieces;
+      float x[N];
+      v.open(x);
+      store_cache(p.c.v, p.c.dtype, (k.slot + static_cast<int64_t>(h) * p.c.page_size) * hd + (i - h * pieces) * N, x,
+                  p.c.v_scale ? 1.0f / __ldg(p.c.v_scale + h) : 1.0f);
+    }
+  }
+  mark_slot(p, k);
+}
+
+// Any layout, stride and alignment, one pair or column per thread.  One block
+// per token.
+template <typename T>
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  griddep_wait();
+  const int t = blockIdx.x, hd = p.c.head_dim, half = p.rot / 2;
+  const int nH = p.q ? p.c.n_heads : 0, H = p.k ? p.c.kv_heads : 0;
+  const Token k = token_of(p, t);
   const int per = hd - half;  // pairs, then the columns that pass
   for (int i = threadIdx.x; i < (nH + H) * per; i += blockDim.x) {
     const int h = i / per, j = i - h * per;
@@ -64,13 +263,13 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
                      : static_cast<const T*>(p.k) + t * p.k_token + kh * p.k_head;
     T* y = isq ? static_cast<T*>(p.q_out) + t * p.qo_token + h * p.qo_head
                : (p.k_out ? static_cast<T*>(p.k_out) + t * p.ko_token + kh * p.ko_head : nullptr);
-    const int64_t kbase = isq || slot < 0 ? -1 : (slot + static_cast<int64_t>(kh) * p.c.page_size) * hd;
+    const int64_t kbase = isq || k.slot < 0 ? -1 : (k.slot + static_cast<int64_t>(kh) * p.c.page_size) * hd;
     const float inv = !isq && p.c.k_scale ? 1.0f / p.c.k_scale[kh] : 1.0f;
     const int ca = j < half ? (p.interleaved ? 2 * j : j) : half + j;
     const int cb = p.interleaved ? ca + 1 : ca + half;
     const float a = ld1(x + ca);
     if (j < half) {
-      const float b = ld1(x + cb), c = cs[j], s = p.sign * sn[j];
+      const float b = ld1(x + cb), c = k.cs[j], s = p.sign * k.sn[j];
       const float u = a * c - b * s, w = b * c + a * s;
       if (y) {
         st1(y + ca, u);
@@ -85,18 +284,15 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
       if (kbase >= 0) st_cache(p.c.k, p.c.dtype, kbase + ca, a, inv);
     }
   }
-  if (slot < 0) return;
-  for (int i = threadIdx.x; i < H * hd; i += blockDim.x) {
-    const int h = i / hd, j = i - h * hd;
-    const float inv = p.c.v_scale ? 1.0f / p.c.v_scale[h] : 1.0f;
-    st_cache(p.c.v, p.c.dtype, (slot + static_cast<int64_t>(h) * p.c.page_size) * hd + j,
-             ld1(static_cast<const T*>(p.v) + t * p.v_token + h * p.v_head + j), inv);
+  if (k.slot >= 0) {
+    for (int i = threadIdx.x; i < H * hd; i += blockDim.x) {
+      const int h = i / hd, j = i - h * hd;
+      const float inv = p.c.v_scale ? 1.0f / p.c.v_scale[h] : 1.0f;
+      st_cache(p.c.v, p.c.dtype, (k.slot + static_cast<int64_t>(h) * p.c.page_size) * hd + j,
+               ld1(static_cast<const T*>(p.v) + t * p.v_token + h * p.v_head + j), inv);
+    }
   }
-  for (int h = threadIdx.x; h < H; h += blockDim.x) {
-    const int64_t at = slot + static_cast<int64_t>(h) * p.c.page_size;
-    if (p.c.weight) p.c.weight[at] = 0.0f;
-    if (p.c.position) p.c.position[at] = pos;
-  }
+  mark_slot(p, k);
 }
 
 // cos and sin of position x frequency, the product and its cosine in 64 bits:
@@ -112,11 +308,33 @@ __global__ void rotary_table_kernel(const double* __restrict__ inv_freq, int hal
   sn[i] = static_cast<float>(s * factor);
 }
 
+bool wide(const void* p, int64_t a, int64_t b, int n, size_t elem) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (a * elem) % 16 == 0 && (b * elem) % 16 == 0 && n * elem % 16 == 0;
+}
+
+template <typename T>
+cudaError_t launch_append(const AppendParams& p, cudaStream_t st) {
+  constexpr int N = Piece<T>::kN;
+  const int hd = p.c.head_dim, half = p.rot / 2;
+  const bool aligned = wide(p.q, p.q_token, p.q_head, hd, sizeof(T)) && wide(p.k, p.k_token, p.k_head, hd, sizeof(T)) &&
+                       wide(p.v, p.v_token, p.v_head, hd, sizeof(T)) && wide(p.q_out, p.qo_token, p.qo_head, hd, sizeof(T)) &&
+                       wide(p.k_out, p.ko_token, p.ko_head, hd, sizeof(T)) && (p.interleaved ? p.rot : half) % N == 0;
+  const int units = (hd - (p.interleaved ? 0 : half)) / N;
+  if (!aligned || units > 512) return launch_kernel(append_kernel<T>, dim3(p.tokens), dim3(256), 0, st, p);
+  // Threads of a token: enough of them to fill the SMs (2048 a SM), up to a
+  // thread per unit for the shortest chain; at 128 seven blocks share a SM.
+  const int heads = (p.q ? p.c.n_heads : 0) + (p.k ? p.c.kv_heads : 0);
+  const int want = std::min(512, std::max(128, 148 * 2048 / p.tokens / 32 * 32)), passes = (heads * units + want - 1) / want;
+  const int per_pass = (heads + passes - 1) / passes, threads = (per_pass * units + 31) / 32 * 32;
+  const auto fn = threads <= 128 ? (p.interleaved ? append_wide_kernel<T, true, true> : append_wide_kernel<T, false, true>)
+                                 : (p.interleaved ? append_wide_kernel<T, true, false> : append_wide_kernel<T, false, false>);
+  return launch_kernel(fn, dim3(p.tokens), dim3(threads), 0, st, p, units, per_pass);
+}
+
 }  // namespace
 
 cudaError_t launch_paged_append(const AppendParams& p, cudaStream_t st) {
-  if (p.dtype == MXMOE_BF16) return launch_kernel(append_kernel<__nv_bfloat16>, dim3(p.tokens), dim3(256), 0, st, p);
-  return launch_kernel(append_kernel<float>, dim3(p.tokens), dim3(256), 0, st, p);
+  return p.dtype == MXMOE_BF16 ? launch_append<__nv_bfloat16>(p, st) : launch_append<float>(p, st);
 }
 
 cudaError_t launch_rotary_table(const double* inv_freq, int half, int64_t first, int n, double factor, float* cos,

@@ -41,10 +41,10 @@ def _act(name: str, t) -> int:
     return code
 
 
-def _heads(name: str, t, heads: int, head_dim: int, device):
+def _heads(name: str, t, n: int, heads: int, head_dim: int, device):
     """[n, heads, head_dim] with contiguous columns -> strides of the first two dimensions."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
-        _bad(f"{name}: expected [n, {heads}, {head_dim}], got {tuple(t.shape)}")
+    if t.shape != (n, heads, head_dim):
+        _bad(f"{name}: expected [{n}, {heads}, {head_dim}], got {tuple(t.shape)}")
     if t.device != device:
         _bad(f"{name}: expected a tensor on {device}, got {t.device}")
     a, b, c = t.stride()
@@ -54,13 +54,13 @@ def _heads(name: str, t, heads: int, head_dim: int, device):
 
 
 def _ints(name: str, t, n: int, device) -> int:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.shape != (n,) or t.device != device or (n > 1 and t.stride(0) != 1):
         _bad(f"{name}: expected {n} contiguous int32 on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 @dataclass
@@ -119,7 +119,7 @@ class RotaryTable:
         if out.dtype != x.dtype or out.shape != x.shape:
             _bad("out: expected x's shape and dtype")
         n, heads, hd = x.shape
-        xs, os = _heads("x", x, heads, hd, self.device), _heads("out", out, heads, hd, self.device)
+        xs, os = _heads("x", x, n, heads, hd, self.device), _heads("out", out, n, heads, hd, self.device)
         a = RotaryArgs(x.data_ptr(), *xs, out.data_ptr(), *os, _act("x", x), n, heads, hd,
                        _ints("positions", positions, n, self.device), *self._ptrs, int(inverse), self.device.index)
         check(lib().mxmqa_rotary(ctypes.byref(a), _stream(self.device)))
@@ -153,7 +153,7 @@ class PagedKvCache:
         return self
 
     def _open(self, k, v, n_heads, weight, position, k_scale, v_scale):
-        self._h = None
+        self._h, self._lib = None, lib()
         if k.dtype not in _CACHE:
             _bad(f"unsupported cache dtype {k.dtype} (float32, bfloat16 or float8_e4m3fn)")
         if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype:
@@ -182,10 +182,13 @@ class PagedKvCache:
         self._h = h
 
     def _tables(self, tables):
-        if tables.dtype != torch.int32 or tables.dim() != 2 or tables.device != self.device or \
-                (tables.stride(1) != 1 and tables.shape[1] > 1):
+        shape = tables.shape
+        if tables.dtype != torch.int32 or len(shape) != 2 or tables.device != self.device:
             _bad(f"tables: expected int32 [rows, max_pages] on {self.device}")
-        return tables.data_ptr(), tables.stride(0), *tables.shape
+        stride, one = tables.stride()
+        if one != 1 and shape[1] > 1:
+            _bad("tables: a row must be contiguous")
+        return tables.data_ptr(), stride, shape[0], shape[1]
 
     def append(self, q, k, v, tables, index, rotary: Optional[RotaryTable] = None, positions=None, rows=None,
                q_out=None, k_out=None):
@@ -194,29 +197,29 @@ class PagedKvCache:
         negative index is turned but not written.  positions: None for the cache indexes.  Returns the turned
         queries (q_out, which may be q; None where q is None); k_out gets the turned keys too.  A written slot's
         weight becomes 0, its position the token's."""
-        n, dev, hd = k.shape[0], self.device, self.head_dim
-        ks, vs = _heads("k", k, self.kv_heads, hd, dev), _heads("v", v, self.kv_heads, hd, dev)
+        n, dev, hd, dtype = k.shape[0], self.device, self.head_dim, k.dtype
+        ks, vs = _heads("k", k, n, self.kv_heads, hd, dev), _heads("v", v, n, self.kv_heads, hd, dev)
         code = _act("k", k)
         qs = os = kos = (0, 0)
-        if v.shape[0] != n or v.dtype != k.dtype:
-            _bad("v: expected k's tokens and dtype")
+        if v.dtype != dtype:
+            _bad("v: expected k's dtype")
         if q is not None:
-            qs = _heads("q", q, self.n_heads, hd, dev)
-            if q.shape[0] != n or q.dtype != k.dtype:
-                _bad("q: expected k's tokens and dtype")
+            qs = _heads("q", q, n, self.n_heads, hd, dev)
+            if q.dtype != dtype:
+                _bad("q: expected k's dtype")
             if q_out is None:
-                q_out = torch.empty((n, self.n_heads, hd), dtype=q.dtype, device=dev)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
                 os = (self.n_heads * hd, hd)
             else:
-                os = _heads("q_out", q_out, self.n_heads, hd, dev)
-                if q_out.shape[0] != n or q_out.dtype != q.dtype:
-                    _bad("q_out: expected q's shape and dtype")
+                os = _heads("q_out", q_out, n, self.n_heads, hd, dev)
+                if q_out.dtype != dtype:
+                    _bad("q_out: expected q's dtype")
         elif q_out is not None:
             _bad("q_out without q")
         if k_out is not None:
-            kos = _heads("k_out", k_out, self.kv_heads, hd, dev)
-            if k_out.shape[0] != n or k_out.dtype != k.dtype:
-                _bad("k_out: expected k's shape and dtype")
+            kos = _heads("k_out", k_out, n, self.kv_heads, hd, dev)
+            if k_out.dtype != dtype:
+                _bad("k_out: expected k's dtype")
         t, stride, n_rows, max_pages = self._tables(tables)
         if rotary is not None and rotary.device != dev:
             _bad(f"rotary: expected a table on {dev}, got {rotary.device}")
@@ -226,7 +229,7 @@ class PagedKvCache:
             t, stride, n_rows, max_pages, None if rows is None else _ints("rows", rows, n, dev),
             _ints("index", index, n, dev), None if positions is None else _ints("positions", positions, n, dev),
             *((None, None, 0, 0, 0) if rotary is None else rotary._ptrs))
-        check(lib().mxmqa_paged_append(self._h, ctypes.byref(a), _stream(dev)))
+        check(self._lib.mxmqa_paged_append(self._h, ctypes.byref(a), _stream(dev)))
         return q_out
 
     def decode(self, q, tables, lens, scale: Optional[float] = None, window: int = 0, sinks=None, quiet: bool = False,
@@ -238,18 +241,18 @@ class PagedKvCache:
         summed over the heads that read its key head, is added to its weight.  lse: float32 [rows, n_heads] gets
         the log of the normalizer.  Rows may share pages, except with track."""
         dev, hd, nH = self.device, self.head_dim, self.n_heads
-        qs = _heads("q", q, nH, hd, dev)
         n = q.shape[0]
+        qs = _heads("q", q, n, nH, hd, dev)
         t, stride, n_rows, max_pages = self._tables(tables)
         if n_rows != n:
             _bad(f"tables: expected {n} rows, got {n_rows}")
         if out is None:
-            out = torch.empty((n, nH, hd), dtype=out_dtype or q.dtype, device=dev)
+            out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
             os = (nH * hd, hd)
         else:
-            os = _heads("out", out, nH, hd, dev)
-            if out.shape[0] != n or (out_dtype is not None and out.dtype != out_dtype):
-                _bad("out: expected q's shape and out_dtype")
+            os = _heads("out", out, n, nH, hd, dev)
+            if out_dtype is not None and out.dtype != out_dtype:
+                _bad("out: expected out_dtype")
         if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (nH,) or sinks.device != dev
                                   or not sinks.is_contiguous()):
             _bad(f"sinks: expected contiguous float32 [{nH}] on {dev}")
@@ -269,7 +272,7 @@ class PagedKvCache:
                             _act("q", q), _act("out", out), n, max_pages, t, stride, _ints("lens", lens, n, dev),
                             1.0 / math.sqrt(hd) if scale is None else scale, window,
                             None if sinks is None else sinks.data_ptr(), *b, int(quiet), int(track))
-        check(lib().mxmqa_paged_decode(self._h, ctypes.byref(a), _stream(dev)))
+        check(self._lib.mxmqa_paged_decode(self._h, ctypes.byref(a), _stream(dev)))
         return out
 
     def evict(self, tables, lens, seen, budget: int, sink: int = 4, recent: int = 0, new_lens=None):
@@ -281,12 +284,12 @@ class PagedKvCache:
         dev = self.device
         t, stride, n, max_pages = self._tables(tables)
         if new_lens is None:
-            new_lens = torch.empty((n,), dtype=torch.int32, device=dev)
+            new_lens = torch.empty_like(lens)
         if budget < 0 or sink < 0 or recent < 0:
             _bad("budget, sink and recent must not be negative")
         a = PagedEvictArgs(t, stride, n, max_pages, _ints("lens", lens, n, dev), _ints("seen", seen, n, dev),
                            _ints("new_lens", new_lens, n, dev), budget, sink, recent)
-        check(lib().mxmqa_paged_evict(self._h, ctypes.byref(a), _stream(dev)))
+        check(self._lib.mxmqa_paged_evict(self._h, ctypes.byref(a), _stream(dev)))
         return new_lens
 
     def sync_status(self):
