@@ -101,7 +101,7 @@ cudaError_t launch_paged_decode(const DecodeParams& p, const DecodeScratch& ws, 
 int decode_tile(const PagedView& c);                     // keys of a tile
 size_t decode_part_floats(const PagedView& c, int sms);  // of DecodeScratch::part
 int decode_workers(const PagedView& c, int sms);         // of DecodeScratch::tickets
-cudaError_t launch_paged_evict(const EvictParams& p, cudaStream_t st);
+cudaError_t launch_paged_evict(const EvictParams& p, int sms, cudaStream_t st);
 cudaError_t launch_rotary_table(const double* inv_freq, int half, int64_t first, int n, double factor, float* cos,
                                 float* sin, cudaStream_t st);
 

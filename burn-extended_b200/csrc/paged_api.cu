@@ -356,7 +356,7 @@ int mxmqa_paged_evict(mxmqa_paged_cache* c, const mxmqa_paged_evict_args* a, voi
   p.sink = static_cast<int>(a->sink);
   p.recent = static_cast<int>(a->recent);
   PDevice g(c->cfg.device);
-  P_CUDA(mxmoe::launch_paged_evict(p, static_cast<cudaStream_t>(stream)));
+  P_CUDA(mxmoe::launch_paged_evict(p, c->sms, static_cast<cudaStream_t>(stream)));
   return MXMOE_OK;
 }
 

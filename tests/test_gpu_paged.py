@@ -506,6 +506,21 @@ def test_evict_in_place_lens(torch):
     check_evict(torch, [500, 20, 130], 100, 4, 50, H=8, in_place=True)
 
 
+@pytest.mark.parametrize("max_pages", [300, 2000, 13000])
+def test_evict_under_wide_tables(torch, max_pages):
+    """Tables far wider than the rows: the work is laid out by what a row could hold."""
+    P = Pool(torch, [900, 30, 513], 4, 2, 64, 16, track=True)
+    wide = torch.full((3, max_pages), -1, dtype=torch.int32, device="cuda")
+    wide[:, : P.tables.shape[1]] = P.tables
+    got = P.cache.evict(wide, P.lens, P.lens, 300, 4, 50)
+    P.cache.sync_status()
+    want = po.evict(P.hk, P.hv, P.hw, P.hp, P.htab, P.hlens, P.hlens, 300, 4, 50)
+    assert np.array_equal(got.cpu().numpy(), want) and np.array_equal(P.position.cpu().numpy(), P.hp)
+    assert np.array_equal(P.weight.cpu().numpy(), P.hw)
+    for x, y in ((P.k, P.hk), (P.v, P.hv)):
+        assert np.array_equal(x.to(torch.float64).cpu().numpy(), y, equal_nan=True)
+
+
 def test_steps_of_a_thinned_conversation(torch):
     """append, decode and evict together over 40 steps against the oracle: the cache never grows past its budget."""
     nH, H, hd, page, budget, rows = 8, 2, 64, 8, 24, 3
