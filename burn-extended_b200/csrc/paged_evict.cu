@@ -28,77 +28,73 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int sink, int fi
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kThreads = 512;
-constexpr int kBins = 2048;  // 11 bits a pass: the key's 32 in three
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kBins = 2 * kThreads;  // 11 bits a pass: the key's 32 in three
+constexpr int kFew = kThreads;       // candidates that are ranked one against another
 constexpr int kMaxCluster = 8;
 
-// Inclusive prefix sums over the block of two counts at once.
-__device__ __forceinline__ int2 block_scan(int2 x, int2* sums) {
+// The sums of the warps before this one and of all, of two counts.
+__device__ __forceinline__ void over_warps(int2 x, int2* sums, int2& before, int2& all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) sums[warp] = x;
+  __syncthreads();
+  int2 y = sums[lane];  // one for each of the 32 warps
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xFFFFFFFFu, x.x, o), b = __shfl_up_sync(0xFFFFFFFFu, x.y, o);
+    const int a = __shfl_up_sync(0xFFFFFFFFu, y.x, o), b = __shfl_up_sync(0xFFFFFFFFu, y.y, o);
     if (lane >= o) {
-      x.x += a;
-      x.y += b;
+      y.x += a;
+      y.y += b;
     }
   }
-  if (lane == 31) sums[warp] = x;
+  all = make_int2(__shfl_sync(0xFFFFFFFFu, y.x, 31), __shfl_sync(0xFFFFFFFFu, y.y, 31));
+  const int from = warp == 0 ? 0 : warp - 1;
+  before = make_int2(__shfl_sync(0xFFFFFFFFu, y.x, from), __shfl_sync(0xFFFFFFFFu, y.y, from));
+  if (warp == 0) before = make_int2(0, 0);
   __syncthreads();
-  if (warp == 0) {
-    int2 y = lane < kThreads / 32 ? sums[lane] : make_int2(0, 0);
-#pragma unroll
-    for (int o = 1; o < kThreads / 32; o <<= 1) {
-      const int a = __shfl_up_sync(0xFFFFFFFFu, y.x, o), b = __shfl_up_sync(0xFFFFFFFFu, y.y, o);
-      if (lane >= o) {
-        y.x += a;
-        y.y += b;
-      }
-    }
-    if (lane < kThreads / 32) sums[lane] = y;
-  }
-  __syncthreads();
-  if (warp > 0) {
-    x.x += sums[warp - 1].x;
-    x.y += sums[warp - 1].y;
-  }
-  return x;
 }
 
 // One cluster per (key head, row).  Each block keeps the keys of its share of
-// the slots in shared memory, so weights and positions are read once.  Three
-// passes over 11 bits, their histograms summed over the cluster, find the last
-// victim's key; prefix sums in the order of the slots number ties, holes and
-// movers; every hole and mover is written to the list of the block that will
-// move it, and the blocks move their pairs in 16-byte pieces.
-// Bound by latency where few tokens move (six cluster barriers), else by the
-// rows moved.
-__global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictParams p, int slots) {
+// the slots in shared memory, so weights and positions are read once.  The
+// last victim is found as a (key, index): passes over 11 bits of the key, their
+// histograms summed over the cluster, until at most kFew candidates share its
+// prefix, which are then ranked one against another.  Each warp numbers the
+// holes and movers of a stretch of slots by ballots; every hole and mover is
+// written to the list of the block that will move it, and the blocks move their
+// pairs in 16-byte pieces.  Bound by the latency of these steps where few
+// tokens move, else by the rows moved.
+__global__ void __launch_bounds__(kThreads, 1) evict_kernel(const EvictParams p, int slots) {
   extern __shared__ __align__(16) uint32_t keys[];  // [slots]; then to[slots / 2 + 1], by[slots / 2 + 1]
   __shared__ __align__(16) int hist[3][kBins];
-  __shared__ int2 sums[kThreads / 32];
-  __shared__ int pick[2];
-  __shared__ int2 count[2];  // this block's (ties, -), (holes, movers)
+  __shared__ uint2 few[kFew];  // of block 0: the candidates' keys and indexes
+  __shared__ int2 sums[kWarps], count[2];
+  __shared__ int pick[3], n_few;
+  __shared__ uint2 last;  // of block 0: the last victim
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const int h = blockIdx.x / C, row = blockIdx.y, tid = threadIdx.x;
+  const int h = blockIdx.x / C, row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto sync = [&]() {
+    if (C == 1)
+      __syncthreads();
+    else
+      cluster.sync();
+  };
   griddep_wait();
   const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size;
   int len = p.lens[row];
+  for (int i = tid; i < 3 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
+  if (tid == 0) n_few = 0;
   if (len < 0 || len > cap) {
     if (tid == 0) atomicOr(p.c.status, kPagedBadIndex);
     len = len < 0 ? 0 : static_cast<int>(cap);
   }
   if (h == 0 && rank == 0 && tid == 0 && p.new_lens) p.new_lens[row] = min(len, p.budget);
   if (len <= p.budget) return;
-  for (int i = tid; i < 3 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
+  const int first_recent = p.seen[row] - p.recent;
   __syncthreads();
 
-  // This block's slots [n0, n0 + mine); thread t owns `run` of them from t * run
-  // on (an odd number: its walk meets no bank conflict).
   const int share = (len + C - 1) / C, n0 = min(len, rank * share), mine = min(share, len - n0);
-  const int run = (mine + kThreads - 1) / kThreads | 1, first_recent = p.seen[row] - p.recent;
   auto slot_at = [&](int n) {
     const int64_t s = slot_of(p.c, p.t, row, n);
     return s < 0 ? -1 : static_cast<int>(s) + h * p.c.page_size;
@@ -110,88 +106,131 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictParams p,
     keys[i] = k;
     atomicAdd(&hist[0][k >> 21], 1);
   }
-  int need = len - p.budget;  // victims among the keys that share the prefix
+  int need = len - p.budget, candidates = len;  // victims among the keys that share the prefix
   uint32_t prefix = 0;
+  int above = 32;  // the prefix's lowest bit
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
+  for (int pass = 0; pass < 3 && (pass == 0 || candidates > kFew); ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     if (pass > 0) {
-      const int above = pass == 1 ? 21 : 10;
       for (int i = tid; i < mine; i += kThreads) {
         const uint32_t k = keys[i];
         if (k >> above == prefix >> above) atomicAdd(&hist[pass][(k >> shift) & (kBins - 1)], 1);
       }
     }
-    cluster.sync();
-    int bin[kBins / kThreads], all = 0;
-#pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) bin[i] = 0;
+    sync();
+    int2 bin = make_int2(0, 0);
     for (int c = 0; c < C; ++c) {
-      const int4 x = *reinterpret_cast<const int4*>(cluster.map_shared_rank(&hist[pass][0], c) + 4 * tid);
-      bin[0] += x.x;
-      bin[1] += x.y;
-      bin[2] += x.z;
-      bin[3] += x.w;
+      const int2 x = *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[pass][0], c) + 2 * tid);
+      bin.x += x.x;
+      bin.y += x.y;
     }
+    int upto = bin.x + bin.y;
 #pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) all += bin[i];
-    int below = block_scan(make_int2(all, 0), sums).x - all;
-    if (below < need && need <= below + all) {
-#pragma unroll
-      for (int i = 0; i < kBins / kThreads; ++i) {
-        if (need > below && need <= below + bin[i]) {
-          pick[0] = 4 * tid + i;
-          pick[1] = need - below;
-        }
-        below += bin[i];
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= o) upto += a;
+    }
+    int2 before, all;
+    over_warps(make_int2(__shfl_sync(0xFFFFFFFFu, upto, 31), 0), sums, before, all);
+    const int low = before.x + upto - bin.x - bin.y;  // keys below this thread's bins
+    if (need > low && need <= low + bin.x + bin.y) {
+      const bool second = need > low + bin.x;
+      pick[0] = 2 * tid + second;
+      pick[1] = need - low - (second ? bin.x : 0);
+      pick[2] = second ? bin.y : bin.x;
     }
     __syncthreads();
     prefix |= static_cast<uint32_t>(pick[0]) << shift;
     need = pick[1];
+    candidates = pick[2];
+    above = shift;
   }
 
-  // Victims are the keys below `prefix` and the first `need` equal to it.
-  const int i0 = min(mine, tid * run), i1 = min(mine, i0 + run);
-  int ties = 0;
-  for (int i = i0; i < i1; ++i) ties += keys[i] == prefix;
-  int2 upto = block_scan(make_int2(ties, 0), sums);
-  if (tid == kThreads - 1) count[0] = upto;
-  cluster.sync();
-  int tie = upto.x - ties;
-  for (int c = 0; c < rank; ++c) tie += cluster.map_shared_rank(&count[0], c)->x;
-  auto victim = [&](uint32_t k, int& t) { return k < prefix || (k == prefix && t++ < need); };
-  int2 own = make_int2(0, 0);  // holes, movers of this thread's run
-  for (int i = i0, t = tie; i < i1; ++i) {
-    const bool out = victim(keys[i], t), low = n0 + i < p.budget;
-    own.x += out && low;
-    own.y += !out && !low;
+  // The last victim: candidate number `need` by (key, index).
+  uint2 bound;
+  const int seg = (mine + kThreads - 1) / kThreads * 32, s0 = min(mine, warp * seg), s1 = min(mine, s0 + seg);  // this warp's slots
+  if (candidates <= kFew) {
+    int* counter = cluster.map_shared_rank(&n_few, 0);
+    uint2* list = cluster.map_shared_rank(few, 0);
+    for (int i = tid; i < mine; i += kThreads)
+      if (keys[i] >> above == prefix >> above) list[atomicAdd(counter, 1)] = make_uint2(keys[i], n0 + i);
+    sync();
+    if (rank == 0 && tid < candidates) {
+      const uint2 me = few[tid];
+      int less = 0;
+      for (int i = 0; i < candidates; ++i) {
+        const uint2 x = few[i];
+        less += x.x < me.x || (x.x == me.x && x.y < me.y);
+      }
+      if (less == need - 1) last = me;
+    }
+    sync();
+    bound = *cluster.map_shared_rank(&last, 0);
+  } else {
+    // whole keys, too many alike: the need-th of them in the order of the slots
+    int ties = 0;
+    for (int i = s0 + lane; i - lane < s1; i += 32) ties += __popc(__ballot_sync(0xFFFFFFFFu, i < s1 && keys[i] == prefix));
+    int2 before, all;
+    over_warps(make_int2(ties, 0), sums, before, all);
+    if (tid == 0) count[0] = all;
+    sync();
+    int upto = before.x;
+    for (int c = 0; c < rank; ++c) upto += cluster.map_shared_rank(&count[0], c)->x;
+    if (upto < need && need <= upto + ties) {
+      for (int i = s0 + lane; i - lane < s1; i += 32) {
+        const uint32_t b = __ballot_sync(0xFFFFFFFFu, i < s1 && keys[i] == prefix);
+        if ((b >> lane & 1) && upto + __popc(b & ((2u << lane) - 1)) == need)
+          *cluster.map_shared_rank(&last, 0) = make_uint2(prefix, n0 + i);
+        upto += __popc(b);
+      }
+    }
+    sync();
+    bound = *cluster.map_shared_rank(&last, 0);
   }
-  upto = block_scan(own, sums);
-  if (tid == kThreads - 1) count[1] = upto;
-  cluster.sync();
-  int2 at = make_int2(upto.x - own.x, upto.y - own.y);
-  int pairs = 0;
-  for (int c = 0; c < C; ++c) {
-    const int2 x = *cluster.map_shared_rank(&count[1], c);
-    pairs += x.x;
-    if (c < rank) {
-      at.x += x.x;
-      at.y += x.y;
+
+  auto victim = [&](int i) {
+    const uint32_t k = keys[i];
+    return k < bound.x || (k == bound.x && n0 + i <= static_cast<int>(bound.y));
+  };
+  int2 own = make_int2(0, 0), before, all;  // holes, movers of this warp's slots
+  for (int i = s0 + lane; i - lane < s1; i += 32) {
+    const bool in = i < s1, out = in && victim(i), low = n0 + i < p.budget;
+    own.x += __popc(__ballot_sync(0xFFFFFFFFu, out && low));
+    own.y += __popc(__ballot_sync(0xFFFFFFFFu, in && !out && !low));
+  }
+  over_warps(own, sums, before, all);
+  int pairs = all.x;
+  if (C > 1) {
+    if (tid == 0) count[1] = all;
+    cluster.sync();
+    pairs = 0;
+    for (int c = 0; c < C; ++c) {
+      const int2 x = *cluster.map_shared_rank(&count[1], c);
+      pairs += x.x;
+      if (c < rank) {
+        before.x += x.x;
+        before.y += x.y;
+      }
     }
   }
-  const int per = (pairs + C - 1) / C, room = slots / 2 + 1;  // pairs of a block's list; per <= room as holes <= len / 2
+  const int per = max(1, (pairs + C - 1) / C), room = slots / 2 + 1;  // pairs of a block; holes <= len / 2, so per <= room
   int* to = reinterpret_cast<int*>(keys + slots);
   int* by = to + room;
   if (own.x + own.y > 0) {
-    for (int i = i0, t = tie; i < i1; ++i) {
-      const bool out = victim(keys[i], t), low = n0 + i < p.budget;
-      if (out != low) continue;
-      const int e = out ? at.x++ : at.y++, c = e / per;
-      *cluster.map_shared_rank((out ? to : by) + (e - c * per), c) = slot_at(n0 + i);
+    for (int i = s0 + lane; i - lane < s1; i += 32) {
+      const bool in = i < s1, out = in && victim(i), low = n0 + i < p.budget;
+      const uint32_t holes = __ballot_sync(0xFFFFFFFFu, out && low), movers = __ballot_sync(0xFFFFFFFFu, in && !out && !low);
+      if (in && out == low) {
+        const int e = out ? before.x + __popc(holes & ((1u << lane) - 1)) : before.y + __popc(movers & ((1u << lane) - 1));
+        const int c = C == 1 ? 0 : e / per;
+        *cluster.map_shared_rank((out ? to : by) + (e - c * per), c) = slot_at(n0 + i);
+      }
+      before.x += __popc(holes);
+      before.y += __popc(movers);
     }
   }
-  cluster.sync();
+  sync();
 
   const int list = min(per, pairs - rank * per), bytes = p.c.head_dim * (p.c.dtype == MXMOE_F32 ? 4 : p.c.dtype == MXMOE_BF16 ? 2 : 1);
   const int pieces = bytes / 16;
@@ -351,15 +390,15 @@ __global__ void lens_kernel(const EvictParams p, int32_t* lens) {
 }
 
 cudaError_t launch_select(const EvictParams& p, int sms, cudaStream_t st) {
-  // Blocks of a (row, key head): enough for two a SM, no more than leaves each
-  // a thread's slot, and at least what the longest row's keys and lists (8 bytes
-  // a slot) need.
-  constexpr int kSlots = 10 * 1024;  // two blocks share a SM
+  // Blocks of a (row, key head): one, as a cluster's barriers cost more than
+  // they save (MEASURE), unless the longest row's keys and lists (8 bytes a slot)
+  // need more, or long rows leave SMs idle.
+  constexpr int kSlots = 24 * 1024;  // of one block's shared memory
   const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size;
   int C = 1;
-  while (C < kMaxCluster && ((cap + C - 1) / C > kSlots || (p.rows * p.c.kv_heads * C < 2 * sms && cap / C > 2 * kThreads))) C *= 2;
+  while (C < kMaxCluster && ((cap + C - 1) / C > kSlots || (C < 4 && 2 * p.rows * p.c.kv_heads * C < sms && cap / C > 8 * kThreads))) C *= 2;
   const int64_t slots = ((cap + C - 1) / C + 3) / 4 * 4;
-  if (slots > 24 * 1024) {  // past one block's shared memory
+  if (slots > kSlots) {
     return launch_kernel(evict_long_kernel, dim3(p.c.kv_heads, p.rows), dim3(kLongThreads), 0, st, p);
   }
   const size_t smem = (static_cast<size_t>(slots) + 2 * (slots / 2 + 1)) * 4;
