@@ -18,7 +18,6 @@
 namespace mxmoe {
 namespace {
 
-constexpr int kRingBytes = 217 * 1024;  // of an SM's 227 KB, beside the row list
 
 // The register arrays' head size that the kernels are built for.
 int padded_head(const PagedView& c) {
@@ -27,16 +26,11 @@ int padded_head(const PagedView& c) {
   return 256;
 }
 
-// The ring of each warp: at least three stages, so that two are in flight while
-// one is read, with as many warps as that allows.
 DecodePlan decode_plan(const PagedView& c, int sms) {
   DecodePlan d{};
-  const int es = c.dtype == MXMOE_F32 ? 4 : c.dtype == MXMOE_BF16 ? 2 : 1;
-  const int hd = padded_head(c);
-  d.stage_bytes = std::max(32 * decode::tile_halves(hd * es) * decode::ring_row(hd * es), kDecodeHeads * hd * 4);
-  d.warps = kDecodeWarps;
-  while (d.warps > 1 && 3 * d.warps * d.stage_bytes > kRingBytes) d.warps >>= 1;
-  d.stages = std::min(kDecodeMaxStages, kRingBytes / (d.warps * d.stage_bytes));
+  d.stage_bytes = decode::stage_bytes(padded_head(c), c.dtype == MXMOE_F32 ? 4 : c.dtype == MXMOE_BF16 ? 2 : 1);
+  d.warps = decode::warps_for(d.stage_bytes);
+  d.stages = std::min(kDecodeMaxStages, decode::kRingBytes / (d.warps * d.stage_bytes));
   d.smem = d.warps * d.stages * d.stage_bytes + 128;
   d.grid = sms;
   return d;

@@ -49,6 +49,19 @@ constexpr int ring_row(int bytes) { return (bytes / 16 | 1) * 16; }
 // a row is short; longer rows have enough columns for that.
 constexpr int tile_halves(int bytes) { return bytes <= 128 ? 2 : 1; }
 
+// One tile's keys and values, with room for a warp's output of 8 heads.
+constexpr int stage_bytes(int hd, int elem) {
+  const int kv = 32 * tile_halves(hd * elem) * ring_row(hd * elem), out = kDecodeHeads * hd * 4;
+  return kv > out ? kv : out;
+}
+
+// Warps of a block: 8 where each has a ring of at least two stages, else 4 or 2.
+// 16 of them with tiles of 16 keys and 128 registers were slower (64 x 8192
+// tokens 208 us against 203), and so were 4 with deeper rings where two stages
+// of 8 fit (50001 tokens in 32 bits 44 us against 37).
+constexpr int kRingBytes = 217 * 1024;  // of an SM's 227 KB, beside the row list
+constexpr int warps_for(int stage) { return 8 * 2 * stage <= kRingBytes ? 8 : 4 * 2 * stage <= kRingBytes ? 4 : 2; }
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -174,7 +187,8 @@ struct Queries {
 template <int HDT, bool X>
 struct Bf16 {
   static constexpr bool kWide = X;
-  static constexpr int kElem = 2, rb = ring_row(HDT * 2), NT = tile_halves(HDT * 2);
+  static constexpr int kElem = 2, rb = ring_row(HDT * 2), NT = tile_halves(HDT * 2),
+                       kWarps = warps_for(stage_bytes(HDT, 2));
   struct Q {
     uint32_t a[HDT / 16][X ? 6 : 2];
     float back;
@@ -266,7 +280,8 @@ struct Bf16 {
 template <int HDT, bool X>
 struct E4m3 {
   static constexpr bool kWide = X;
-  static constexpr int kElem = 1, rb = ring_row(HDT), NT = tile_halves(HDT);
+  static constexpr int kElem = 1, rb = ring_row(HDT), NT = tile_halves(HDT),
+                       kWarps = warps_for(stage_bytes(HDT, 1));
   struct Q {
     uint32_t a[HDT / 16][4];
     float back;
@@ -366,7 +381,8 @@ struct E4m3 {
 template <int HDT, bool X>
 struct F32 {
   static constexpr bool kWide = true;
-  static constexpr int kElem = 4, rb = ring_row(HDT * 4), NT = tile_halves(HDT * 4);
+  static constexpr int kElem = 4, rb = ring_row(HDT * 4), NT = tile_halves(HDT * 4),
+                       kWarps = warps_for(stage_bytes(HDT, 4));
   struct Q {
     uint32_t a[HDT / 8][4];
     float back;
@@ -561,7 +577,7 @@ __device__ __forceinline__ void store_out(const DecodeParams& p, int row, int h,
 }
 
 template <class C, int HDT>
-__global__ void __launch_bounds__(32 * kDecodeWarps, 1)
+__global__ void __launch_bounds__(32 * C::kWarps, 1)
     attend_kernel(const DecodeParams p, const DecodeScratch ws, const DecodePlan plan) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ int before[kDecodeMaxRows + 1];
@@ -572,7 +588,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
   const Rows rows{before, len_of};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int hd = p.c.head_dim, H = p.c.kv_heads, G = p.c.n_heads / H;
-  const int parts = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * parts, W = plan.warps;
+  const int parts = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * parts;
+  constexpr int W = C::kWarps;
   constexpr int rb = C::rb, NT = C::NT, kTile = 16 * NT, kPairs = HDT / 8;  // column pairs of a lane
   uint8_t* const mine = ring + warp * plan.stages * plan.stage_bytes;
   list_rows(p, rows, kTile);
@@ -844,17 +861,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
     if (lane == 0) join_at[warp] = (warp * plan.stages + ld_stage) * plan.stage_bytes;
     group_sync();
     // nt is a multiple of 32: a thread's head is its lane's for every pair
-    float top = -INFINITY, sum = 0.0f, e[kDecodeWarps];
-    const float2* from[kDecodeWarps];
+    float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w)
+    for (int w = 0; w < W; ++w)
       if (w < wg) top = fmaxf(top, join_ml[w0 + w][g][0]);
 #pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       if (w >= wg) break;
-      e[w] = exp_diff(join_ml[w0 + w][g][0], top);
-      sum = fmaf(join_ml[w0 + w][g][1], e[w], sum);
-      from[w] = reinterpret_cast<const float2*>(ring + join_at[w0 + w]);
+      sum = fmaf(join_ml[w0 + w][g][1], exp_diff(join_ml[w0 + w][g][0], top), sum);
     }
     float f = 1.0f;
     if (to) {
@@ -867,12 +881,12 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
 #pragma unroll 1
     for (int i = tid; i < 32 * kPairs; i += nt) {
       float a = 0.0f, b = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kDecodeWarps; ++w) {
-        if (w >= wg) break;
-        const float2 y = from[w][i];
-        a = fmaf(y.x, e[w], a);
-        b = fmaf(y.y, e[w], b);
+#pragma unroll 4
+      for (int w = w0; w < w0 + wg; ++w) {
+        const float e = exp_diff(join_ml[w][g][0], top);
+        const float2 y = reinterpret_cast<const float2*>(ring + join_at[w])[i];
+        a = fmaf(y.x, e, a);
+        b = fmaf(y.y, e, b);
       }
       if (to)
         to[i] = make_float2(a, b);
@@ -885,6 +899,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps, 1)
 
 template <class C, int HDT>
 cudaError_t launch(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st) {
+  static_assert(2 * C::kWarps * stage_bytes(HDT, C::kElem) <= kRingBytes, "a ring has at least two stages");
   const auto fn = attend_kernel<C, HDT>;
   const cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fn), plan.smem);
   if (e != cudaSuccess) return e;
