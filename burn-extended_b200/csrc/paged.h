@@ -89,8 +89,9 @@ constexpr int kDecodeWarps = 8;       // of a block, at most
 
 // Device memory that decode needs beside its arguments.
 struct DecodeScratch {
-  float* part;    // [2 * workers][8 * (padded head_dim + 2)] partial outputs, maxima and sums
-  int* tickets;   // [workers], zero between calls
+  float* part;    // [2 * ranges][8 * (padded head_dim + 2)] partial outputs, maxima and sums
+  int2* held;     // [kDecodeMaxRows][segments] the first and last range that a segment falls to
+  int* taken;     // [2] ranges taken, warps that have left; zero between calls
   float* scores;  // [score_tiles][tile / 16][32 lanes][4] (track)
   int64_t score_tiles;
   float* lse;  // [kDecodeMaxRows][n_heads] (track)
@@ -100,7 +101,6 @@ cudaError_t launch_paged_append(const AppendParams& p, cudaStream_t st);
 cudaError_t launch_paged_decode(const DecodeParams& p, const DecodeScratch& ws, int sms, cudaStream_t st);
 int decode_tile(const PagedView& c);                     // keys of a tile
 size_t decode_part_floats(const PagedView& c, int sms);  // of DecodeScratch::part
-int decode_workers(const PagedView& c, int sms);         // of DecodeScratch::tickets
 cudaError_t launch_paged_evict(const EvictParams& p, int sms, cudaStream_t st);
 cudaError_t launch_rotary_table(const double* inv_freq, int half, int64_t first, int n, double factor, float* cos,
                                 float* sin, cudaStream_t st);

@@ -200,7 +200,8 @@ int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers*
   const size_t group = cfg->n_heads / cfg->kv_heads, segs = cfg->kv_heads * ((group + mxmoe::kDecodeHeads - 1) / mxmoe::kDecodeHeads);
   int rc = palloc(&w.status, 1, true);
   if (rc == MXMOE_OK) rc = palloc(&ws.part, mxmoe::decode_part_floats(w, c->sms), false);
-  if (rc == MXMOE_OK) rc = palloc(&ws.tickets, mxmoe::decode_workers(w, c->sms), true);
+  if (rc == MXMOE_OK) rc = palloc(&ws.taken, 2, true);
+  if (rc == MXMOE_OK) rc = palloc(&ws.held, mxmoe::kDecodeMaxRows * segs, false);
   if (rc == MXMOE_OK && w.weight) {
     ws.score_tiles = static_cast<int64_t>(
         (static_cast<uint64_t>(cfg->n_pages) * cfg->page_size / mxmoe::decode_tile(w) + mxmoe::kDecodeMaxRows) * segs);
@@ -221,7 +222,8 @@ int mxmqa_paged_destroy(mxmqa_paged_cache* c) {
   PDevice g(c->cfg.device);
   cudaFree(c->view.status);
   cudaFree(c->scratch.part);
-  cudaFree(c->scratch.tickets);
+  cudaFree(c->scratch.taken);
+  cudaFree(c->scratch.held);
   cudaFree(c->scratch.scores);
   cudaFree(c->scratch.lse);
   delete c;
@@ -287,6 +289,7 @@ int mxmqa_paged_append(mxmqa_paged_cache* c, const mxmqa_paged_append_args* a, v
   p.interleaved = a->interleaved ? 1 : 0;
   p.sign = 1.0f;
   PDevice g(c->cfg.device);
+  mxmoe::PdlScope pdl(true);  // every kernel waits for the one before it in the stream
   P_CUDA(mxmoe::launch_paged_append(p, static_cast<cudaStream_t>(stream)));
   return MXMOE_OK;
 }
@@ -332,6 +335,7 @@ int mxmqa_paged_decode(mxmqa_paged_cache* c, const mxmqa_paged_decode_args* a, v
   p.bias_len = static_cast<int>(a->bias_len);
   p.track = a->track ? 1 : 0;
   PDevice g(c->cfg.device);
+  mxmoe::PdlScope pdl(true);  // every kernel waits for the one before it in the stream
   P_CUDA(mxmoe::launch_paged_decode(p, c->scratch, c->sms, static_cast<cudaStream_t>(stream)));
   return MXMOE_OK;
 }
@@ -356,6 +360,7 @@ int mxmqa_paged_evict(mxmqa_paged_cache* c, const mxmqa_paged_evict_args* a, voi
   p.sink = static_cast<int>(a->sink);
   p.recent = static_cast<int>(a->recent);
   PDevice g(c->cfg.device);
+  mxmoe::PdlScope pdl(true);  // every kernel waits for the one before it in the stream
   P_CUDA(mxmoe::launch_paged_evict(p, c->sms, static_cast<cudaStream_t>(stream)));
   return MXMOE_OK;
 }
@@ -424,6 +429,7 @@ int mxmqa_rotary(const mxmqa_rotary_args* a, void* stream) {
   p.interleaved = a->interleaved ? 1 : 0;
   p.sign = a->inverse ? -1.0f : 1.0f;
   PDevice g(a->device);
+  mxmoe::PdlScope pdl(true);  // every kernel waits for the one before it in the stream
   P_CUDA(mxmoe::launch_paged_append(p, static_cast<cudaStream_t>(stream)));
   return MXMOE_OK;
 }

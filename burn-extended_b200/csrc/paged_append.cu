@@ -146,6 +146,7 @@ template <typename T, bool kInterleaved, bool kMany>
 __global__ void __launch_bounds__(kMany ? 128 : 512, kMany ? 7 : 1) append_wide_kernel(const AppendParams p, int units, int per_pass) {
   constexpr int N = Piece<T>::kN;
   griddep_wait();
+  griddep_launch_dependents();
   const int t = blockIdx.x, hd = p.c.head_dim, half = p.rot / 2;
   const int nH = p.q ? p.c.n_heads : 0, H = p.k ? p.c.kv_heads : 0;
   const int unit = threadIdx.x % units, first = threadIdx.x / units;
@@ -251,6 +252,7 @@ constexpr int kCos = kInterleaved ? N / 2 : N, kAtOnce = kCos % 4 ? 2 : 4;
 template <typename T>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   griddep_wait();
+  griddep_launch_dependents();
   const int t = blockIdx.x, hd = p.c.head_dim, half = p.rot / 2;
   const int nH = p.q ? p.c.n_heads : 0, H = p.k ? p.c.kv_heads : 0;
   const Token k = token_of(p, t);

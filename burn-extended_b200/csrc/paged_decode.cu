@@ -46,6 +46,8 @@ __global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const 
   const decode::Rows rows{before, len_of};
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int H = p.c.kv_heads, G = p.c.n_heads / H, hgroups = (G + kDecodeHeads - 1) / kDecodeHeads;
+  griddep_wait();
+  griddep_launch_dependents();
   decode::list_rows(p, rows, 16 * NT);
   const int total = before[p.rows] * H, step = gridDim.x * (blockDim.x / 32);
   for (int x = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); x < total; x += step) {
@@ -90,18 +92,21 @@ int decode_tile(const PagedView& c) {
   return 16 * decode::tile_halves(padded_head(c) * es);
 }
 
-size_t decode_part_floats(const PagedView& c, int sms) {
+// Ranges of the tile list: one for each warp, and twice as many, and one more,
+// of those kept back.
+int decode_ranges(const PagedView& c, int sms) {
   const DecodePlan d = decode_plan(c, sms);
-  return static_cast<size_t>(2) * d.grid * d.warps * kDecodeHeads * (padded_head(c) + 2);
+  return 3 * d.grid * d.warps + 1;
 }
 
-int decode_workers(const PagedView& c, int sms) {
-  const DecodePlan d = decode_plan(c, sms);
-  return d.grid * d.warps;
+size_t decode_part_floats(const PagedView& c, int sms) {
+  return static_cast<size_t>(2) * decode_ranges(c, sms) * kDecodeHeads * (padded_head(c) + 2);
 }
 
 cudaError_t launch_paged_decode(const DecodeParams& all, const DecodeScratch& ws, int sms, cudaStream_t st) {
-  const DecodePlan plan = decode_plan(all.c, sms);
+  DecodePlan plan = decode_plan(all.c, sms);
+  const int64_t longest = std::min<int64_t>(static_cast<int64_t>(all.t.max_pages) * all.c.page_size, all.window ? all.window : INT32_MAX);
+  plan.whole = longest <= kWholeTiles * decode_tile(all.c);
   // Rows of one launch: their tiles are numbered in 32 bits.
   const int G = all.c.n_heads / all.c.kv_heads, segs = all.c.kv_heads * ((G + kDecodeHeads - 1) / kDecodeHeads);
   const int64_t most = (static_cast<int64_t>(all.t.max_pages) * all.c.page_size / decode_tile(all.c) + 1) * segs;

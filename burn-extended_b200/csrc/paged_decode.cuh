@@ -7,9 +7,9 @@
 // tiles through its own shared-memory ring (cp.async, no block barrier) and
 // keeps a running maximum, sum and output for 8 query heads in registers.  At
 // the end of a (row, key head) the group joins its warps in shared memory; a
-// pair that more than one worker holds goes through partial results in global
-// memory, and the last worker to arrive joins them in the workers' order, so the
-// result does not depend on timing.
+// pair that more than one range holds goes through partial results in global
+// memory, which a second kernel joins in the order of the keys, so the result
+// does not depend on timing.
 //
 // The products run on the warp MMA, m = 16: rows 0-7 hold the heads' queries
 // (or shares) rounded to the operand type, rows 8-15 what the rounding left, so
@@ -31,12 +31,15 @@ namespace mxmoe {
 
 constexpr int kDecodeMaxStages = 6;
 
+constexpr int kWholeTiles = 8;
+
 // How one launch is laid out; set by decode_plan in paged_decode.cu.
 struct DecodePlan {
   int warps, stages;
   int stage_bytes;  // K rows, then V rows; room for a warp's 8 x head_dim floats
   int smem;         // of the block: the warps' rings, and 128 bytes that a read past the last row may touch
   int grid;
+  int whole;        // no segment has more than kWholeTiles tiles: none is cut
 };
 
 namespace decode {
@@ -556,6 +559,77 @@ __device__ __forceinline__ void store_lse(const DecodeParams& p, const DecodeScr
   if (p.track) ws.lse[row * p.c.n_heads + h] = lse;
 }
 
+// How the tile list is cut into ranges, each of which one worker, a group of
+// `wg` warps, works through.
+//
+// whole: rows are so short that every segment is a range of its own, and worker
+// w takes the ranges w, w + n_workers and so on.
+// Else the first n_workers ranges are dealt out, one to a worker (no more
+// workers than give each of their warps a tile), the first `more` of them one
+// tile above the others.  SMs are not served alike by the memory, though: with
+// 8 tiles a warp and more, where warps work alone, a quarter of the list is kept
+// back and goes in small ranges (n_big of 2 `small` tiles, then of `small`) to
+// whoever is done.  A segment that several ranges hold has its parts joined by
+// join_kernel.
+struct Cut {
+  Rows rows;
+  int segs, whole, wg, n_workers, n_ranges, dealt, kept, each, more, small, n_big;
+
+  // `total` tiles of n_rows x segs segments over `warps` warps, W to a block.
+  __device__ __forceinline__ Cut(Rows r, int n_rows, int segs_of_row, int total, int warps, int W, int whole_)
+      : rows(r), segs(segs_of_row), whole(whole_), wg(1) {
+    const int n_segs = n_rows * segs;
+    // A warp alone waits for no other; but where there are few segments, warps
+    // in groups leave fewer parts to join.  No more warps than a mean segment
+    // has tiles.
+    const int most = whole ? warps / (2 * n_segs) : warps / (32 * n_segs);
+#pragma unroll 1
+    while (wg < W && wg < most + whole && wg * n_segs < total) wg <<= 1;
+    if (whole) {
+      n_workers = min(warps / wg, n_segs);
+      n_ranges = n_segs;
+      kept = 0;
+      return;
+    }
+    n_workers = min(warps / wg, (total + wg - 1) / wg);
+    kept = wg == 1 && total >= 8 * warps ? total / 4 : 0;
+    dealt = total - kept;
+    each = dealt / n_workers;
+    more = dealt - each * n_workers;
+    small = max(2, (kept + 3 * warps - 1) / (3 * warps));
+    n_big = min(warps, kept / (2 * small));
+    n_ranges = n_workers + n_big + (kept - 2 * small * n_big + small - 1) / small;
+  }
+  // The first tile of range r; whole: its segment's, which may have none.
+  __device__ __forceinline__ int begin_of(int r) const {
+    if (whole) {
+      const int row = r / segs;
+      return rows.before[row] * segs + (r - row * segs) * (rows.before[row + 1] - rows.before[row]);
+    }
+    if (r <= n_workers) return r * each + min(r, more);
+    r -= n_workers;
+    return dealt + (r <= n_big ? 2 * small * r : min(kept, 2 * small * n_big + small * (r - n_big)));
+  }
+  __device__ __forceinline__ int end_of(int r) const {
+    if (!whole) return begin_of(r + 1);
+    const int row = r / segs;
+    return begin_of(r) + rows.before[row + 1] - rows.before[row];
+  }
+  // The range of tile x (not whole).
+  __device__ __forceinline__ int range_of(int x) const {
+    const int edge = more * (each + 1), big = dealt + 2 * small * n_big;
+    if (x < edge) return x / (each + 1);
+    if (x < dealt) return more + (x - edge) / each;
+    return n_workers + (x < big ? (x - dealt) / (2 * small) : n_big + (x - big) / small);
+  }
+  // whole: the next of a worker's ranges from r on that has tiles.
+  __device__ __forceinline__ int filled(int r) const {
+#pragma unroll 1
+    while (r < n_ranges && rows.before[r / segs + 1] == rows.before[r / segs]) r += n_workers;
+    return r;
+  }
+};
+
 // Two finished columns of a head; `apart` is 1 or 4.
 template <int kApart>
 __device__ __forceinline__ void store_out(const DecodeParams& p, int row, int h, int col, float x, float y) {
@@ -582,7 +656,7 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ int before[kDecodeMaxRows + 1];
   __shared__ int len_of[kDecodeMaxRows];
-  __shared__ int arrived[kDecodeWarps][2], join_at[kDecodeWarps];
+  __shared__ int join_at[kDecodeWarps], queue[kDecodeWarps][8];
   __shared__ float join_ml[kDecodeWarps][kDecodeHeads][2];
   __shared__ uint32_t there[kDecodeWarps][kDecodeMaxStages];  // which keys of a stage are in the cache
   const Rows rows{before, len_of};
@@ -592,8 +666,10 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   constexpr int W = C::kWarps;
   constexpr int rb = C::rb, NT = C::NT, kTile = 16 * NT, kPairs = HDT / 8;  // column pairs of a lane
   uint8_t* const mine = ring + warp * plan.stages * plan.stage_bytes;
+  griddep_wait();
+  griddep_launch_dependents();
   list_rows(p, rows, kTile);
-  const int total = before[p.rows] * segs;
+  const int total = before[p.rows] * segs, n_segs = p.rows * segs;
 
   // Rows without keys: zeros.
 #pragma unroll 1
@@ -610,26 +686,27 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
       if (i == h * hd) store_lse(p, ws, r, h, finish(p.sinks ? p.sinks[h] : -INFINITY, p.quiet, -INFINITY, 0.0f).y);
     }
   }
-  if (total == 0) return;
-
-  // Warps of a worker.  Alone, a warp waits for no other; but a segment should
-  // not fall to more than about four workers, whose parts one of them has to
-  // read, and no more warps than a mean segment has tiles.
-  int wg = 1;
-  const int n_segs = p.rows * segs, warps = W * static_cast<int>(gridDim.x);
+  if (total == 0) {
 #pragma unroll 1
-  while (wg < W && 4 * wg * n_segs < warps && wg * n_segs < total) wg <<= 1;
-  const int group = warp / wg, in_group = warp - group * wg, w0 = group * wg, tid = threadIdx.x - w0 * 32, nt = 32 * wg;
-  // No more workers than give each of their warps a tile.  The first `more`
-  // workers have one tile above the others.
-  const int n_workers = min(warps / wg, (total + wg - 1) / wg), each = total / n_workers, more = total - each * n_workers;
+    for (int s = blockIdx.x + gridDim.x * threadIdx.x; s < n_segs && !plan.whole; s += gridDim.x * blockDim.x)
+      ws.held[s] = make_int2(0, 0);
+    return;
+  }
+
+  const Cut cut(rows, p.rows, segs, total, W * gridDim.x, W, plan.whole);
+  const int wg = cut.wg, group = warp / wg, in_group = warp - group * wg, w0 = group * wg, tid = threadIdx.x - w0 * 32, nt = 32 * wg;
+  if (!plan.whole) {
+    // For join_kernel: the first and last range of every segment.
+#pragma unroll 1
+    for (int s = blockIdx.x + gridDim.x * threadIdx.x; s < n_segs; s += gridDim.x * blockDim.x) {
+      const int r = s / segs, tiles = before[r + 1] - before[r], y = before[r] * segs + (s - r * segs) * tiles;
+      ws.held[s] = tiles == 0 ? make_int2(0, 0) : make_int2(cut.range_of(y), cut.range_of(y + tiles - 1));
+    }
+  }
   const int worker = group * gridDim.x + blockIdx.x;
-  if (worker >= n_workers) return;
-  const int begin = worker * each + min(worker, more), end = begin + each + (worker < more ? 1 : 0);
-  auto worker_of = [&](int x) {
-    const int edge = more * (each + 1);
-    return x < edge ? x / (each + 1) : more + (x - edge) / each;
-  };
+  if (worker >= cut.n_workers) return;
+  int range = cut.whole ? cut.filled(worker) : worker;
+  if (range >= cut.n_ranges) return;
   auto group_sync = [&]() {
     if (wg == 1)
       __syncwarp();
@@ -641,7 +718,8 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   // tile's key of that number, two tiles ahead of its use, as the page table's
   // answer takes that long.
   Place ld;
-  ld.find(p, rows, parts, begin);
+  int x = cut.begin_of(range), end = cut.end_of(range), ld_left = end - x, ld_off = in_group, ld_stage = 0;
+  ld.find(p, rows, parts, x);
   Place at = ld;
   // The next segment's queries and its heads' sinks.
   Queries<HDT, C::kWide> queries;
@@ -656,8 +734,16 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
     int page, slot, kvh;  // kvh -1: no tile; page -1: no key, -2: out of range
   };
   Ahead next{-1, 0, -1}, after{-1, 0, -1};
-  int ld_left = end - begin, ld_off = in_group, ld_stage = 0;
   int prime = plan.stages + 1;  // loads before the first tile: two that only look ahead, then all stages but one
+  // Ranges taken after the first.  One that was kept back is asked for when the
+  // one before it begins to be loaded, and waits in `queue` for its use; each
+  // has two tiles at least, so no more than eight are between the two.
+  int ld_range = range, asked = 0, queued = 0, used = 0;
+  bool last_piece = false, fetched = false;  // of the range in use; the next one's queries are on their way
+  auto ask = [&]() {
+    if (cut.kept > 0 && lane == 0) asked = cut.n_workers + atomicAdd(ws.taken, 1);
+  };
+  ask();
   // Loads the next tile into the stage that is free, and looks two further.
   auto load_tile = [&]() {
     if (next.kvh >= 0) {
@@ -696,8 +782,24 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
     while (ld_off >= n && ld_left > 0) {
       ld_left -= n;
       ld_off = in_group;
-      if (ld_left > 0) ld.next_segment(p, rows, parts);
-      n = min(ld.tiles, ld_left);
+      if (ld_left > 0) {
+        ld.next_segment(p, rows, parts);
+      } else if (cut.whole || cut.kept > 0) {
+        ld_range = cut.whole ? cut.filled(ld_range + cut.n_workers) : __shfl_sync(0xFFFFFFFFu, asked, 0);
+        if (cut.kept > 0 && lane == 0) queue[warp][queued & 7] = ld_range;
+        ++queued;
+        if (ld_range < cut.n_ranges) {
+          const int y = cut.begin_of(ld_range);
+          ld_left = cut.end_of(ld_range) - y;
+          ld.find(p, rows, parts, y);
+          ask();
+          if (cut.kept > 0 && last_piece && !fetched && queued - 1 == used) {  // it is the next one
+            fetch(ld);
+            fetched = true;
+          }
+        }
+      }
+      n = min(ld.tiles - ld.tile, ld_left);
     }
     if (ld_left <= 0) return;
     const int key = ld.lo + (ld.tile + ld_off) * kTile + lane % kTile;
@@ -713,29 +815,30 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
 
   constexpr int kPartPairs = 32 * kPairs + kDecodeHeads;  // [pairs][lane] of o, then (m, l) by head
   float2* const part_of = reinterpret_cast<float2*>(ws.part);
-  // Segments of this worker that others hold too: the one that it begins in
-  // (side 0) and the one that it ends in (side 1); row -1: none.
-  int split_row[2] = {-1, -1}, split_kvh[2], split_part[2], split_first[2], split_last[2];
-  int stage = 0, side = -1;
-  for (int x = begin;;) {
-    int row = at.row, kvh = at.kvh, part = at.part;
-    float2* to = nullptr;  // where this worker's part goes; null: the output
+  int stage = 0;
+  while (true) {
+    if (x >= end) {
+      if (!cut.whole && cut.kept == 0) break;
+      range = cut.whole ? cut.filled(range + cut.n_workers) : queue[warp][used++ & 7];
+      if (range >= cut.n_ranges) break;
+      x = cut.begin_of(range);
+      end = cut.end_of(range);
+      at.find(p, rows, parts, x);
+      if (!fetched) fetch(at);
+      fetched = false;
+    }
+    const int row = at.row, kvh = at.kvh, part = at.part;
+    float2* to = nullptr;  // where this range's part of the segment goes; null: the output
     float m = -INFINITY, l = 0.0f;
     float o[kPairs][2];
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) o[i][0] = o[i][1] = 0.0f;
-    float sink = sink_next;
-    if (x < end) {
+    const float sink = sink_next;
+    {
       const int n = min(at.tiles - at.tile, end - x), h0 = kvh * G + part * kDecodeHeads;
       if (n < at.tiles) {
         const int e = at.tile == 0 ? 1 : 0;
-        const int s0 = before[row] * segs + (kvh * parts + part) * at.tiles;
-        split_row[e] = row;
-        split_kvh[e] = kvh;
-        split_part[e] = part;
-        split_first[e] = worker_of(s0);
-        split_last[e] = worker_of(s0 + at.tiles - 1);
-        to = part_of + (2 * worker + e) * kPartPairs;
+        to = part_of + (2 * range + e) * kPartPairs;
       }
       // the queries go through the stage that is free until the next load
       typename C::Q q;
@@ -748,10 +851,20 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
       }
       const float ks = p.scale * q.back * (p.c.k_scale ? p.c.k_scale[kvh] : 1.0f);
       const float* bias = p.bias && part * kDecodeHeads + g < G ? p.bias + row * p.bias_row + (h0 + g) * p.bias_head : nullptr;
-      if (x + n < end) {
+      last_piece = x + n >= end;
+      if (!last_piece) {
         Place then = at;
         then.next_segment(p, rows, parts);
         fetch(then);
+      } else if (cut.whole || queued > used) {
+        // the next range is known (else the load side fetches, when it comes to that)
+        const int r = cut.whole ? cut.filled(range + cut.n_workers) : queue[warp][used & 7];
+        if (r < cut.n_ranges) {
+          Place then;
+          then.find(p, rows, parts, cut.begin_of(r));
+          fetch(then);
+          fetched = true;
+        }
       }
 #pragma unroll 1
       for (int j = in_group; j < n;) {
@@ -809,45 +922,14 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
       l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
       x += n;
       if (x < end) at.next_segment(p, rows, parts);
-    } else {
-      // All tiles are done.  Of the workers that hold a split segment, the last
-      // to come here joins the parts, each warp every wg-th of them.
-      if (side < 0) {
-        cp_wait<0>();
-        if (split_row[0] < 0 && split_row[1] < 0) return;
-        __threadfence();
-        group_sync();
-        if (tid < 2 && split_row[tid] >= 0) arrived[group][tid] = atomicAdd(ws.tickets + split_first[tid], 1);
-        group_sync();
-      }
-      while (++side < 2)
-        if (split_row[side] >= 0 && arrived[group][side] == split_last[side] - split_first[side]) break;
-      if (side >= 2) return;
-      __threadfence();
-      row = split_row[side];
-      kvh = split_kvh[side];
-      part = split_part[side];
-      if (p.sinks && part * kDecodeHeads + g < G) sink = p.sinks[kvh * G + part * kDecodeHeads + g];
-      const int first = split_first[side], last = split_last[side];
-      if (tid == 0) ws.tickets[first] = 0;
-#pragma unroll 2
-      for (int w = first + in_group; w <= last; w += wg) {
-        const float2* from = part_of + (2 * w + (w == first ? 1 : 0)) * kPartPairs;
-        const float2 ml = __ldcg(from + 32 * kPairs + g);
-        float2 y[kPairs];
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) y[i] = __ldcg(from + 32 * i + lane);
-        const float top = fmaxf(m, ml.x), a = exp_diff(m, top), b = exp_diff(ml.x, top);
-        m = top;
-        l = l * a + ml.y * b;
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          o[i][0] = fmaf(y[i].x, b, o[i][0] * a);
-          o[i][1] = fmaf(y[i].y, b, o[i][1] * a);
-        }
-      }
     }
 
+    if (to && wg == 1) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) to[32 * i + lane] = make_float2(o[i][0], o[i][1]);
+      if (t == 0) to[32 * kPairs + g] = make_float2(m, l);
+      continue;
+    }
     // The group's warps join in shared memory, each in the stage that it loads
     // next: nothing uses that until then.
     const int heads = min(kDecodeHeads, G - part * kDecodeHeads), h = kvh * G + part * kDecodeHeads + g;
@@ -895,15 +977,100 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
     }
     group_sync();  // the stages are free again
   }
+  cp_wait<0>();
+  // The last warp to leave sets the counter back.
+  if (cut.kept > 0 && lane == 0 && atomicAdd(ws.taken + 1, 1) == cut.n_workers - 1) {
+    ws.taken[0] = 0;
+    ws.taken[1] = 0;
+  }
+}
+
+// The segments that several ranges hold: a block joins a slice of the columns
+// of one, its warps every eighth part, in the ranges' order; the loads of four
+// parts are in flight at once.
+template <class C, int HDT>
+__global__ void __launch_bounds__(256) join_kernel(const DecodeParams p, const DecodeScratch ws) {
+  constexpr int kPairs = HDT / 8, kSlice = kPairs % 4 ? 5 : 4, kPartPairs = 32 * kPairs + kDecodeHeads, kAtOnce = 4;
+  static_assert(kPairs % kSlice == 0, "slices cover the columns");
+  __shared__ float2 outs[8][32 * kSlice], ml[8][kDecodeHeads];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, p0 = blockIdx.y * kSlice;
+  const int H = p.c.kv_heads, G = p.c.n_heads / H, parts = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * parts;
+  griddep_wait();
+  griddep_launch_dependents();
+#pragma unroll 1
+  for (int s = blockIdx.x; s < p.rows * segs; s += gridDim.x) {
+    const int2 held = __ldcg(ws.held + s);
+    const int row = s / segs, kvh = (s - row * segs) / parts, part = s - row * segs - kvh * parts;
+    const int first = held.x, last = held.y;
+    if (first == last) continue;
+    float m = -INFINITY, l = 0.0f;
+    float2 o[kSlice];
+#pragma unroll
+    for (int i = 0; i < kSlice; ++i) o[i] = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+    for (int w = first + warp; w <= last; w += 8 * kAtOnce) {
+      float2 y[kAtOnce], z[kAtOnce][kSlice];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int v = w + 8 * j;
+        y[j] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int i = 0; i < kSlice; ++i) z[j][i] = make_float2(0.0f, 0.0f);
+        if (v > last) continue;
+        const float2* from = reinterpret_cast<const float2*>(ws.part) + (2 * v + (v == first ? 1 : 0)) * kPartPairs;
+        y[j] = __ldcg(from + 32 * kPairs + g);
+#pragma unroll
+        for (int i = 0; i < kSlice; ++i) z[j][i] = __ldcg(from + 32 * (p0 + i) + lane);
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const float top = fmaxf(m, y[j].x), a = exp_diff(m, top), b = exp_diff(y[j].x, top);
+        m = top;
+        l = l * a + y[j].y * b;
+#pragma unroll
+        for (int i = 0; i < kSlice; ++i) {
+          o[i].x = fmaf(z[j][i].x, b, o[i].x * a);
+          o[i].y = fmaf(z[j][i].y, b, o[i].y * a);
+        }
+      }
+    }
+    __syncthreads();  // the segment before is read out
+#pragma unroll
+    for (int i = 0; i < kSlice; ++i) outs[warp][32 * i + lane] = o[i];
+    if (t == 0) ml[warp][g] = make_float2(m, l);
+    __syncthreads();
+    const int used = min(8, last - first + 1), h = kvh * G + part * kDecodeHeads + g;
+    if (warp >= kSlice || part * kDecodeHeads + g >= G) continue;
+    float top = -INFINITY, sum = 0.0f, a = 0.0f, b = 0.0f;
+    for (int w = 0; w < used; ++w) top = fmaxf(top, ml[w][g].x);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w >= used) break;
+      const float e = exp_diff(ml[w][g].x, top);
+      const float2 y = outs[w][32 * warp + lane];
+      sum = fmaf(ml[w][g].y, e, sum);
+      a = fmaf(y.x, e, a);
+      b = fmaf(y.y, e, b);
+    }
+    const float2 f = finish(p.sinks ? p.sinks[h] : -INFINITY, p.quiet, top, sum);
+    const float by = f.x * (p.c.v_scale ? p.c.v_scale[kvh] : 1.0f);
+    if (p0 + warp == 0 && t == 0) store_lse(p, ws, row, h, f.y);
+    store_out<C::kApart>(p, row, h, C::column(p0 + warp, t), a * by, b * by);
+  }
 }
 
 template <class C, int HDT>
 cudaError_t launch(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st) {
   static_assert(2 * C::kWarps * stage_bytes(HDT, C::kElem) <= kRingBytes, "a ring has at least two stages");
   const auto fn = attend_kernel<C, HDT>;
-  const cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fn), plan.smem);
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fn), plan.smem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(fn, dim3(plan.grid), dim3(32 * plan.warps), plan.smem, st, p, ws, plan);
+  e = launch_kernel(fn, dim3(plan.grid), dim3(32 * plan.warps), plan.smem, st, p, ws, plan);
+  if (e != cudaSuccess || plan.whole) return e;
+  const int G = p.c.n_heads / p.c.kv_heads, n_segs = p.rows * p.c.kv_heads * ((G + kDecodeHeads - 1) / kDecodeHeads);
+  constexpr int slices = HDT / 8 % 4 ? HDT / 40 : HDT / 32;
+  return launch_kernel(join_kernel<C, HDT>, dim3(n_segs < 4 * plan.grid ? n_segs : 4 * plan.grid, slices), dim3(256), 0, st, p,
+                       ws);
 }
 
 }  // namespace decode

@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const EvictParams p,
       cluster.sync();
   };
   griddep_wait();
+  griddep_launch_dependents();
   const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size;
   int len = p.lens[row];
   for (int i = tid; i < 3 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
@@ -276,6 +277,7 @@ __device__ __forceinline__ int block_rank(bool flag, int* warp_sums, int& total)
 // which hand each other holes and movers through shared memory.
 __global__ void __launch_bounds__(kLongThreads) evict_long_kernel(const EvictParams p) {
   griddep_wait();
+  griddep_launch_dependents();
   __shared__ int hist[256], sums[kLongThreads / 32], pick[2];
   __shared__ int64_t holes[kLongThreads], movers[kLongThreads];
   const int h = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
@@ -382,6 +384,7 @@ __global__ void __launch_bounds__(kLongThreads) evict_long_kernel(const EvictPar
 // New lengths in the place of the old ones, once every block has read those.
 __global__ void lens_kernel(const EvictParams p, int32_t* lens) {
   griddep_wait();
+  griddep_launch_dependents();
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= p.rows) return;
   const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size;
@@ -409,12 +412,14 @@ cudaError_t launch_select(const EvictParams& p, int sms, cudaStream_t st) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = C;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, evict_kernel, p, static_cast<int>(slots));
 }
 
