@@ -26,14 +26,8 @@ int padded_head(const PagedView& c) {
   return 256;
 }
 
-DecodePlan decode_plan(const PagedView& c, int sms) {
-  DecodePlan d{};
-  d.stage_bytes = decode::stage_bytes(padded_head(c), c.dtype == MXMOE_F32 ? 4 : c.dtype == MXMOE_BF16 ? 2 : 1);
-  d.warps = decode::warps_for(d.stage_bytes);
-  d.stages = std::min(kDecodeMaxStages, decode::kRingBytes / (d.warps * d.stage_bytes));
-  d.smem = d.warps * d.stages * d.stage_bytes + 128;
-  d.grid = sms;
-  return d;
+int warps_of(const PagedView& c) {
+  return decode::warps_for(decode::stage_bytes(padded_head(c), c.dtype == MXMOE_F32 ? 4 : c.dtype == MXMOE_BF16 ? 2 : 1));
 }
 
 // One warp per tile of cached keys of a (row, key head): the 8 lanes that hold
@@ -92,21 +86,15 @@ int decode_tile(const PagedView& c) {
   return 16 * decode::tile_halves(padded_head(c) * es);
 }
 
-// Ranges of the tile list: one for each warp, and twice as many, and one more,
-// of those kept back.
-int decode_ranges(const PagedView& c, int sms) {
-  const DecodePlan d = decode_plan(c, sms);
-  return 3 * d.grid * d.warps + 1;
-}
-
+// Two for each range of the tile list: one range for each warp, and twice as
+// many, and one more, of those kept back.
 size_t decode_part_floats(const PagedView& c, int sms) {
-  return static_cast<size_t>(2) * decode_ranges(c, sms) * kDecodeHeads * (padded_head(c) + 2);
+  return static_cast<size_t>(2) * (3 * sms * warps_of(c) + 1) * kDecodeHeads * (padded_head(c) + 2);
 }
 
 cudaError_t launch_paged_decode(const DecodeParams& all, const DecodeScratch& ws, int sms, cudaStream_t st) {
-  DecodePlan plan = decode_plan(all.c, sms);
   const int64_t longest = std::min<int64_t>(static_cast<int64_t>(all.t.max_pages) * all.c.page_size, all.window ? all.window : INT32_MAX);
-  plan.whole = longest <= kWholeTiles * decode_tile(all.c);
+  const DecodePlan plan{sms, longest <= kWholeTiles * decode_tile(all.c)};
   // Rows of one launch: their tiles are numbered in 32 bits.
   const int G = all.c.n_heads / all.c.kv_heads, segs = all.c.kv_heads * ((G + kDecodeHeads - 1) / kDecodeHeads);
   const int64_t most = (static_cast<int64_t>(all.t.max_pages) * all.c.page_size / decode_tile(all.c) + 1) * segs;
@@ -130,7 +118,7 @@ cudaError_t launch_paged_decode(const DecodeParams& all, const DecodeScratch& ws
     const cudaError_t e = attend(p, ws, plan, st);
     if (e != cudaSuccess) return e;
     if (!p.track) continue;
-    const cudaError_t f = launch_kernel(decode_tile(p.c) == 32 ? weigh_kernel<2> : weigh_kernel<1>, dim3(4 * sms), dim3(256), 0, st, p, ws);
+    const cudaError_t f = launch_kernel(decode_tile(p.c) == 32 ? weigh_kernel<2> : weigh_kernel<1>, dim3(8 * sms), dim3(256), 0, st, p, ws);
     if (f != cudaSuccess) return f;
   }
   return cudaSuccess;

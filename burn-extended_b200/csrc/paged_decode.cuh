@@ -33,13 +33,10 @@ constexpr int kDecodeMaxStages = 6;
 
 constexpr int kWholeTiles = 8;
 
-// How one launch is laid out; set by decode_plan in paged_decode.cu.
+// How one launch is laid out.
 struct DecodePlan {
-  int warps, stages;
-  int stage_bytes;  // K rows, then V rows; room for a warp's 8 x head_dim floats
-  int smem;         // of the block: the warps' rings, and 128 bytes that a read past the last row may touch
   int grid;
-  int whole;        // no segment has more than kWholeTiles tiles: none is cut
+  int whole;  // no segment has more than kWholeTiles tiles: none is cut
 };
 
 namespace decode {
@@ -65,6 +62,11 @@ constexpr int stage_bytes(int hd, int elem) {
 constexpr int kRingBytes = 217 * 1024;  // of an SM's 227 KB, beside the row list
 constexpr int warps_for(int stage) { return 8 * 2 * stage <= kRingBytes ? 8 : 4 * 2 * stage <= kRingBytes ? 4 : 2; }
 
+constexpr int stages_for(int stage) {
+  const int n = kRingBytes / (warps_for(stage) * stage);
+  return n < kDecodeMaxStages ? n : kDecodeMaxStages;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -84,18 +86,6 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void cp_wait_for(int newer) {
-  switch (newer) {
-    case 0: cp_wait<0>(); break;
-    case 1: cp_wait<1>(); break;
-    case 2: cp_wait<2>(); break;
-    case 3: cp_wait<3>(); break;
-    case 4: cp_wait<4>(); break;
-    case 5: cp_wait<5>(); break;
-    default: cp_wait<6>(); break;
-  }
-}
-
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -113,12 +103,19 @@ __device__ __forceinline__ void lds128(float (&r)[4], uint32_t a) {
   asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]) : "r"(a) : "memory");
 }
 
+// d += a b, and d = a b.
 #define MXMOE_MMA(name, shape)                                                                                      \
   __device__ __forceinline__ void name(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, \
                                        uint32_t b1) {                                                               \
-    asm volatile("mma.sync.aligned." shape " {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                 \
+    asm("mma.sync.aligned." shape " {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                 \
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                   \
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));                                           \
+  }                                                                                                                 \
+  __device__ __forceinline__ void name##_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,     \
+                                             uint32_t b0, uint32_t b1) {                                            \
+    asm("mma.sync.aligned." shape " {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"             \
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                   \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));                                \
   }
 MXMOE_MMA(mma_bf16, "m16n8k16.row.col.f32.bf16.bf16.f32")
 MXMOE_MMA(mma_f16, "m16n8k16.row.col.f32.f16.f16.f32")
@@ -179,9 +176,38 @@ struct Queries {
   static __device__ __forceinline__ void put(uint2&, float4) {}
 };
 
+// A warp's output: pair n of lane (g, t) are two columns of head g.  In 32 bits
+// (X) each tile's products are summed apart and joined by one rounded addition:
+// the MMA's own sums are cut off, and over a long row that would show.  For a
+// bf16 output the MMA adds to the sums, the shares' second terms apart.
+template <int HDT, bool X>
+struct Output {
+  float x[HDT / 8][X ? 2 : 4];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < HDT / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < (X ? 2 : 4); ++e) x[n][e] = 0.0f;
+  }
+  __device__ __forceinline__ void scale(float f) {
+#pragma unroll
+    for (int n = 0; n < HDT / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < (X ? 2 : 4); ++e) x[n][e] *= f;
+  }
+  __device__ __forceinline__ void fold(int n, const float (&d)[4], float f) {
+    x[n][0] = fmaf(x[n][0], f, d[0] + d[2]);
+    x[n][1] = fmaf(x[n][1], f, d[1] + d[3]);
+  }
+  __device__ __forceinline__ float2 pair(int n) const {
+    return X ? make_float2(x[n][0], x[n][1]) : make_float2(x[n][0] + x[n][X ? 0 : 2], x[n][1] + x[n][X ? 1 : 3]);
+  }
+};
+
 // ---- the cache's element types ----
 //
-// Each has: Q, the query operand; load(), which fills it for lane (g, t) =
+// Each has: Q, the query operand; V, values on their way; load(), which fills them for lane (g, t) =
 // (lane / 4, lane % 4) from head g's row in shared memory; scores(), s[4] of keys 2t, 2t + 1,
 // 8 + 2t, 9 + 2t; and add(), o = o corr + p V over the tile's 16 keys.  HDT:
 // head_dim rounded up to the register arrays' size; X: 32-bit activations, a
@@ -190,8 +216,8 @@ struct Queries {
 template <int HDT, bool X>
 struct Bf16 {
   static constexpr bool kWide = X;
-  static constexpr int kElem = 2, rb = ring_row(HDT * 2), NT = tile_halves(HDT * 2),
-                       kWarps = warps_for(stage_bytes(HDT, 2));
+  static constexpr int kElem = 2, rb = ring_row(HDT * 2), NT = tile_halves(HDT * 2), kWarps = warps_for(stage_bytes(HDT, 2));
+  static constexpr int kStageBytes = stage_bytes(HDT, 2), kStages = stages_for(kStageBytes);
   struct Q {
     uint32_t a[HDT / 16][X ? 6 : 2];
     float back;
@@ -214,22 +240,30 @@ struct Bf16 {
       }
   }
   static __device__ __forceinline__ void scores(float (&s)[4 * NT], const Q& q, uint32_t k, int lane) {
-    float c[2 * NT][4] = {};
+    constexpr int kAhead = HDT / 16 * NT <= 8 ? HDT / 16 : 4;  // steps whose keys are loaded together
+    float c[2 * NT][4];
     const uint32_t at = k + ((lane >> 4) * 8 + (lane & 7)) * rb + ((lane >> 3) & 1) * 16;
 #pragma unroll
-    for (int i = 0; i < HDT / 16; ++i) {
+    for (int i0 = 0; i0 < HDT / 16; i0 += kAhead) {
+      uint32_t b[kAhead][NT][4];
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        uint32_t b[4];
-        ldm4(b, at + 16 * u * rb + 32 * i);
+      for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if (X) {
-            mma_bf16(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], b[2 * j], b[2 * j + 1]);
-            mma_bf16(c[2 * u + j], q.a[i][4], 0, q.a[i][5], 0, b[2 * j], b[2 * j + 1]);
-          } else {
-            mma_bf16(c[2 * u + j], q.a[i][0], 0, q.a[i][1], 0, b[2 * j], b[2 * j + 1]);
-          }
+        for (int u = 0; u < NT; ++u)
+          if (i0 + i < HDT / 16) ldm4(b[i][u], at + 16 * u * rb + 32 * (i0 + i));
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const int i = i0 + e;
+        if (i >= HDT / 16) break;
+        const uint32_t l0 = X ? q.a[i][X ? 2 : 0] : 0, l1 = X ? q.a[i][X ? 3 : 0] : 0;
+#pragma unroll
+        for (int j = 0; j < 2 * NT; ++j) {
+          const uint32_t b0 = b[e][j / 2][2 * (j & 1)], b1 = b[e][j / 2][2 * (j & 1) + 1];
+          if (i == 0)
+            mma_bf16_new(c[j], q.a[i][0], l0, q.a[i][1], l1, b0, b1);
+          else
+            mma_bf16(c[j], q.a[i][0], l0, q.a[i][1], l1, b0, b1);
+          if (X) mma_bf16(c[j], q.a[i][X ? 4 : 0], 0, q.a[i][X ? 5 : 0], 0, b0, b1);
         }
       }
     }
@@ -239,56 +273,85 @@ struct Bf16 {
       s[2 * j + 1] = X ? c[j][1] + c[j][3] : c[j][1];
     }
   }
-  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4 * NT], float corr, uint32_t v,
+  // The values of the first kPre pairs of column groups, loaded ahead of the shares.
+  static constexpr int kPre = HDT / 16 * NT <= 8 ? HDT / 16 : 4;
+  struct V {
+    uint32_t b[kPre][NT][4];
+  };
+  static __device__ __forceinline__ uint32_t value_at(uint32_t v, int lane) {
+    return v + (((lane >> 3) & 1) * 8 + (lane & 7)) * rb + (lane >> 4) * 16;
+  }
+  static __device__ __forceinline__ void load(V& x, uint32_t v, int lane) {
+#pragma unroll
+    for (int n = 0; n < kPre; ++n)
+#pragma unroll
+      for (int u = 0; u < NT; ++u) ldm4t(x.b[n][u], value_at(v, lane) + 16 * u * rb + 32 * n);
+  }
+  static __device__ __forceinline__ void add(Output<HDT, X>& o, V& x, const float (&p)[4 * NT], float corr, uint32_t v,
                                              int lane) {
     uint32_t h[2 * NT], l[2 * NT], m[2 * NT];
 #pragma unroll
     for (int j = 0; j < 2 * NT; ++j) {
       h[j] = pack_bf16(p[2 * j], p[2 * j + 1]);
-      const float x = p[2 * j] - lo_of(h[j]), y = p[2 * j + 1] - hi_of(h[j]);
-      l[j] = pack_bf16(x, y);
-      m[j] = X ? pack_bf16(x - lo_of(l[j]), y - hi_of(l[j])) : 0;
+      const float y = p[2 * j] - lo_of(h[j]), z = p[2 * j + 1] - hi_of(h[j]);
+      l[j] = pack_bf16(y, z);
+      m[j] = X ? pack_bf16(y - lo_of(l[j]), z - hi_of(l[j])) : 0;
     }
-    const uint32_t at = v + (((lane >> 3) & 1) * 8 + (lane & 7)) * rb + (lane >> 4) * 16;
 #pragma unroll
-    for (int n = 0; n < HDT / 8; n += 2) {
-      float d[2][4] = {};
+    for (int n0 = 0; n0 < HDT / 16; n0 += kPre) {
+      if (n0 > 0) {
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        uint32_t b[4];
-        ldm4t(b, at + 16 * u * rb + 16 * n);
+        for (int n = 0; n < kPre; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          mma_bf16(d[e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b[2 * e], b[2 * e + 1]);
-          if (X) mma_bf16(d[e], m[2 * u], 0, m[2 * u + 1], 0, b[2 * e], b[2 * e + 1]);
-        }
+          for (int u = 0; u < NT; ++u)
+            if (n0 + n < HDT / 16) ldm4t(x.b[n][u], value_at(v, lane) + 16 * u * rb + 32 * (n0 + n));
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        o[n + e][0] = fmaf(o[n + e][0], corr, d[e][0] + d[e][2]);
-        o[n + e][1] = fmaf(o[n + e][1], corr, d[e][1] + d[e][3]);
+      for (int i = 0; i < 2 * kPre; ++i) {
+        const int n = 2 * n0 + i;
+        if (n >= HDT / 8) break;
+        float d[4];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const uint32_t b0 = x.b[i / 2][u][2 * (i & 1)], b1 = x.b[i / 2][u][2 * (i & 1) + 1];
+          if constexpr (!X)
+            mma_bf16(o.x[n], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
+          else if (u == 0)
+            mma_bf16_new(d, h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
+          else
+            mma_bf16(d, h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
+          if (X) mma_bf16(d, m[2 * u], 0, m[2 * u + 1], 0, b0, b1);
+        }
+        if (X) o.fold(n, d, corr);
       }
     }
   }
-  // The columns of o[n]: the first, and how far the second is.
+  // The columns of pair n: the first, and how far the second is.
   static constexpr int kApart = 1;
   static __device__ __forceinline__ int column(int n, int t) { return 8 * n + 2 * t; }
 };
 
 // 8-bit keys and values widen to f16 without loss.  A query row is scaled by a
 // power of two to a maximum of 2^8 to 2^9 (f16's range is too short for any
-// row), two f16 terms then hold 22 bits of it; a share lies in [0, 1].  The
-// order of the contracted columns within 16 is free as long as both operands
-// agree: lane t takes bytes 4t to 4t + 3 of a key's 16, as one ldmatrix gives.
+// row), two f16 terms then hold 22 bits of it, the first alone a bf16 query's
+// eight; a share lies in [0, 1].  The MMA on 8-bit operands would save the
+// widening, but its sums keep too few bits: scores were off by 6e-4.
+// The order of the contracted columns within 16 is free as long as both
+// operands agree: lane t takes bytes 4t to 4t + 3 of a key's 16, as one ldmatrix
+// gives.
 template <int HDT, bool X>
 struct E4m3 {
   static constexpr bool kWide = X;
-  static constexpr int kElem = 1, rb = ring_row(HDT), NT = tile_halves(HDT),
-                       kWarps = warps_for(stage_bytes(HDT, 1));
+  static constexpr int kElem = 1, rb = ring_row(HDT), NT = tile_halves(HDT), kWarps = warps_for(stage_bytes(HDT, 1));
+  static constexpr int kStageBytes = stage_bytes(HDT, 1), kStages = stages_for(kStageBytes);
   struct Q {
-    uint32_t a[HDT / 16][4];
+    uint32_t a[HDT / 16][X ? 4 : 2];
     float back;
   };
+  static __device__ __forceinline__ uint32_t widen(uint32_t two) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
+    return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+  }
   static __device__ __forceinline__ void load(Q& q, const float* row, int t) {
     float top = 0.0f;
 #pragma unroll
@@ -310,28 +373,34 @@ struct E4m3 {
         const uint32_t h = pack_f16(x.x * f, x.y * f);
         const __half2 hh = *reinterpret_cast<const __half2*>(&h);
         q.a[s][half] = h;
-        q.a[s][2 + half] = X ? pack_f16(x.x * f - __low2float(hh), x.y * f - __high2float(hh)) : 0;
+        if (X) q.a[s][X ? 2 + half : 0] = pack_f16(x.x * f - __low2float(hh), x.y * f - __high2float(hh));
       }
   }
-  static __device__ __forceinline__ uint32_t widen(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
-    return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
-  }
   static __device__ __forceinline__ void scores(float (&s)[4 * NT], const Q& q, uint32_t k, int lane) {
-    float c[2 * NT][4] = {};
+    constexpr int kAhead = HDT / 32 * NT <= 8 ? HDT / 32 : 4;  // ldmatrixes whose keys are loaded together
+    float c[2 * NT][4];
     // one ldmatrix: keys 0-7 and 8-15 of two 16-byte pieces
     const uint32_t at = k + ((lane >> 4) * 8 + (lane & 7)) * rb + ((lane >> 3) & 1) * 16;
 #pragma unroll
-    for (int i = 0; i < HDT / 16; i += 2) {
+    for (int i0 = 0; i0 < HDT / 32; i0 += kAhead) {
+      uint32_t b[kAhead][NT][4];
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        uint32_t b[4];
-        ldm4(b, at + 16 * u * rb + 16 * i);
+      for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e = j & 1;
-          const uint32_t w = b[j];
-          mma_f16(c[2 * u + (j >> 1)], q.a[i + e][0], q.a[i + e][2], q.a[i + e][1], q.a[i + e][3], widen(w & 0xFFFF), widen(w >> 16));
+        for (int u = 0; u < NT; ++u)
+          if (i0 + i < HDT / 32) ldm4(b[i][u], at + 16 * u * rb + 32 * (i0 + i));
+#pragma unroll
+      for (int e = 0; e < 2 * kAhead; ++e) {
+        const int i = 2 * i0 + e;
+        if (i >= HDT / 16) break;
+        const uint32_t l0 = X ? q.a[i][X ? 2 : 0] : 0, l1 = X ? q.a[i][X ? 3 : 0] : 0;
+#pragma unroll
+        for (int j = 0; j < 2 * NT; ++j) {
+          const uint32_t w = b[e / 2][j / 2][2 * (j & 1) + (e & 1)], b0 = widen(w & 0xFFFF), b1 = widen(w >> 16);
+          if (i == 0)
+            mma_f16_new(c[j], q.a[i][0], l0, q.a[i][1], l1, b0, b1);
+          else
+            mma_f16(c[j], q.a[i][0], l0, q.a[i][1], l1, b0, b1);
         }
       }
     }
@@ -341,37 +410,52 @@ struct E4m3 {
       s[2 * j + 1] = X ? c[j][1] + c[j][3] : c[j][1];
     }
   }
-  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4 * NT], float corr, uint32_t v,
+  // All the tile's values, loaded ahead of the shares: of 32 columns and 16
+  // keys, lane g holds columns 4g to 4g + 3 of four keys.
+  struct V {
+    uint32_t w[HDT / 32][NT][4];
+  };
+  static __device__ __forceinline__ void load(V& x, uint32_t v, int lane) {
+    const uint32_t at = v + 2 * (lane & 3) * rb + 4 * (lane >> 2);
+#pragma unroll
+    for (int n = 0; n < HDT / 32; ++n)
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.w[n][u][e] = lds32(at + (16 * u + 8 * (e >> 1) + (e & 1)) * rb + 32 * n);
+  }
+  static __device__ __forceinline__ void add(Output<HDT, X>& o, V& x, const float (&p)[4 * NT], float corr, uint32_t v,
                                              int lane) {
-    const int g = lane >> 2, t = lane & 3;
     uint32_t h[2 * NT], l[2 * NT];
 #pragma unroll
     for (int j = 0; j < 2 * NT; ++j) {
       h[j] = pack_f16(p[2 * j], p[2 * j + 1]);
-      const __half2 x = *reinterpret_cast<const __half2*>(&h[j]);
-      l[j] = pack_f16(p[2 * j] - __low2float(x), p[2 * j + 1] - __high2float(x));
+      const __half2 y = *reinterpret_cast<const __half2*>(&h[j]);
+      l[j] = pack_f16(p[2 * j] - __low2float(y), p[2 * j + 1] - __high2float(y));
     }
-    const uint32_t at = v + 2 * t * rb + 4 * g;
 #pragma unroll
-    for (int n = 0; n < HDT / 8; n += 4) {  // 32 columns: lane g holds 4g to 4g + 3 of four keys
-      float d[4][4] = {};
+    for (int n = 0; n < HDT / 32; ++n) {
+      float d[4][4];
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
-        const uint32_t from = at + 16 * u * rb + 8 * n;
-        const uint32_t w0 = lds32(from), w1 = lds32(from + rb), w2 = lds32(from + 8 * rb), w3 = lds32(from + 9 * rb);
-        const uint32_t x[4] = {__byte_perm(w0, w1, 0x5140), __byte_perm(w0, w1, 0x7362), __byte_perm(w2, w3, 0x5140),
-                               __byte_perm(w2, w3, 0x7362)};
+        const uint32_t* w = x.w[n][u];
+        const uint32_t y[4] = {__byte_perm(w[0], w[1], 0x5140), __byte_perm(w[0], w[1], 0x7362),
+                               __byte_perm(w[2], w[3], 0x5140), __byte_perm(w[2], w[3], 0x7362)};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t y = x[e >> 1], z = x[2 + (e >> 1)];
-          mma_f16(d[e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], widen(e & 1 ? y >> 16 : y & 0xFFFF),
-                  widen(e & 1 ? z >> 16 : z & 0xFFFF));
+          const uint32_t a = y[e >> 1], b = y[2 + (e >> 1)];
+          const uint32_t b0 = widen(e & 1 ? a >> 16 : a & 0xFFFF), b1 = widen(e & 1 ? b >> 16 : b & 0xFFFF);
+          if constexpr (!X)
+            mma_f16(o.x[4 * n + e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
+          else if (u == 0)
+            mma_f16_new(d[e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
+          else
+            mma_f16(d[e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
         }
       }
+      if (X) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[n + e][0] = fmaf(o[n + e][0], corr, d[e][0] + d[e][2]);
-        o[n + e][1] = fmaf(o[n + e][1], corr, d[e][1] + d[e][3]);
+        for (int e = 0; e < 4; ++e) o.fold(4 * n + e, d[e], corr);
       }
     }
   }
@@ -383,9 +467,10 @@ struct E4m3 {
 // exact: 21 bits of either operand.
 template <int HDT, bool X>
 struct F32 {
+  static_assert(X, "a 32-bit cache is read in 32 bits");
   static constexpr bool kWide = true;
-  static constexpr int kElem = 4, rb = ring_row(HDT * 4), NT = tile_halves(HDT * 4),
-                       kWarps = warps_for(stage_bytes(HDT, 4));
+  static constexpr int kElem = 4, rb = ring_row(HDT * 4), NT = tile_halves(HDT * 4), kWarps = warps_for(stage_bytes(HDT, 4));
+  static constexpr int kStageBytes = stage_bytes(HDT, 4), kStages = stages_for(kStageBytes);
   struct Q {
     uint32_t a[HDT / 8][4];
     float back;
@@ -404,7 +489,7 @@ struct F32 {
       }
   }
   static __device__ __forceinline__ void scores(float (&s)[4 * NT], const Q& q, uint32_t k, int lane) {
-    float c[2 * NT][4] = {};
+    float c[2 * NT][4];
     const uint32_t at = k + ((lane >> 4) * 8 + (lane & 7)) * rb + ((lane >> 3) & 1) * 16;
 #pragma unroll
     for (int i = 0; i < HDT / 8; ++i) {
@@ -415,7 +500,10 @@ struct F32 {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float x = __uint_as_float(b[2 * j]), y = __uint_as_float(b[2 * j + 1]);
-          mma_tf32(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], top(x), top(y));
+          if (i == 0)
+            mma_tf32_new(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], top(x), top(y));
+          else
+            mma_tf32(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], top(x), top(y));
           mma_tf32(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], rest(x), rest(y));
         }
       }
@@ -426,13 +514,14 @@ struct F32 {
       s[2 * j + 1] = c[j][1] + c[j][3];
     }
   }
-  static __device__ __forceinline__ void add(float (&o)[HDT / 8][2], const float (&p)[4 * NT], float corr, uint32_t v,
-                                             int lane) {
+  struct V {};
+  static __device__ __forceinline__ void load(V&, uint32_t, int) {}
+  static __device__ __forceinline__ void add(Output<HDT, X>& o, V&, const float (&p)[4 * NT], float corr, uint32_t v, int lane) {
     const int g = lane >> 2, t = lane & 3;
     const uint32_t at = v + 2 * t * rb + 16 * g;
 #pragma unroll
     for (int n = 0; n < HDT / 8; n += 4) {
-      float d[4][4] = {};
+      float d[4][4];
 #pragma unroll
       for (int u = 0; u < 2 * NT; ++u) {  // keys 8u to 8u + 7
         float w[2][4];
@@ -441,15 +530,15 @@ struct F32 {
         const float p0 = p[2 * u], p1 = p[2 * u + 1];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          mma_tf32(d[e], top(p0), rest(p0), top(p1), rest(p1), top(w[0][e]), top(w[1][e]));
+          if (u == 0)
+            mma_tf32_new(d[e], top(p0), rest(p0), top(p1), rest(p1), top(w[0][e]), top(w[1][e]));
+          else
+            mma_tf32(d[e], top(p0), rest(p0), top(p1), rest(p1), top(w[0][e]), top(w[1][e]));
           mma_tf32(d[e], top(p0), rest(p0), top(p1), rest(p1), rest(w[0][e]), rest(w[1][e]));
         }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[n + e][0] = fmaf(o[n + e][0], corr, d[e][0] + d[e][2]);
-        o[n + e][1] = fmaf(o[n + e][1], corr, d[e][1] + d[e][3]);
-      }
+      for (int e = 0; e < 4; ++e) o.fold(n + e, d[e], corr);
     }
   }
   static constexpr int kApart = 4;
@@ -663,9 +752,10 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int hd = p.c.head_dim, H = p.c.kv_heads, G = p.c.n_heads / H;
   const int parts = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * parts;
-  constexpr int W = C::kWarps;
+  constexpr int W = C::kWarps, kStages = C::kStages, kStageBytes = C::kStageBytes;
+  constexpr uint32_t kAllKeys = 0xFFFFFFFFu;
   constexpr int rb = C::rb, NT = C::NT, kTile = 16 * NT, kPairs = HDT / 8;  // column pairs of a lane
-  uint8_t* const mine = ring + warp * plan.stages * plan.stage_bytes;
+  uint8_t* const mine = ring + warp * kStages * kStageBytes;
   griddep_wait();
   griddep_launch_dependents();
   list_rows(p, rows, kTile);
@@ -734,7 +824,7 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
     int page, slot, kvh;  // kvh -1: no tile; page -1: no key, -2: out of range
   };
   Ahead next{-1, 0, -1}, after{-1, 0, -1};
-  int prime = plan.stages + 1;  // loads before the first tile: two that only look ahead, then all stages but one
+  int prime = kStages + 1;  // loads before the first tile: two that only look ahead, then all stages but one
   // Ranges taken after the first.  One that was kept back is asked for when the
   // one before it begins to be loaded, and waits in `queue` for its use; each
   // has two tiles at least, so no more than eight are between the two.
@@ -745,35 +835,53 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   };
   ask();
   // Loads the next tile into the stage that is free, and looks two further.
+  constexpr int kPieces = HDT * C::kElem / 16;  // of a key's row, 16 bytes each; zeros past head_dim
+  constexpr int kLanes = kPieces % 8 == 0 ? 8 : 4, kKeys = 32 / kLanes;
+  const int piece = lane % kLanes * 16;
+  const uint8_t* const k_piece = static_cast<const uint8_t*>(p.c.k) + piece;
+  const int64_t v_apart = static_cast<const uint8_t*>(p.c.v) - static_cast<const uint8_t*>(p.c.k);
   auto load_tile = [&]() {
     if (next.kvh >= 0) {
       if (next.page == -2) atomicOr(p.c.status, kPagedBadPage);
       const uint32_t keys = __ballot_sync(0xFFFFFFFFu, next.page >= 0);
       if (lane == 0) there[warp][ld_stage] = keys;
       const int row = next.page < 0 ? -1 : (next.page * H + next.kvh) * p.c.page_size + next.slot;
-      const uint32_t ks = smem_u32(mine) + ld_stage * plan.stage_bytes, vs = ks + kTile * rb;
-      constexpr int kPieces = HDT * C::kElem / 16;  // 16 bytes each, zeros past head_dim
-      constexpr int kLanes = kPieces % 8 == 0 ? 8 : 4, kKeys = 32 / kLanes;
-      const int piece = lane % kLanes * 16;
+      const uint32_t ks = smem_u32(mine) + ld_stage * kStageBytes, vs = ks + kTile * rb;
+      const bool all = keys == kAllKeys && kPieces * 16 == hd * C::kElem;
+if (all) {
 #pragma unroll
-      for (int i = 0; i < kTile / kKeys; ++i) {
-        const int key = i * kKeys + lane / kLanes;
-        const int from = __shfl_sync(0xFFFFFFFFu, row, key);
-        const int64_t byte = static_cast<int64_t>(max(from, 0)) * (hd * C::kElem);
-        const uint8_t *kf = static_cast<const uint8_t*>(p.c.k) + byte, *vf = static_cast<const uint8_t*>(p.c.v) + byte;
+        for (int i = 0; i < kTile / kKeys; ++i) {
+          const int key = i * kKeys + lane / kLanes;
+          const uint8_t* kf = k_piece + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, row, key)) * (HDT * C::kElem);
+          const uint8_t* vf = kf + v_apart;
 #pragma unroll
-        for (int j = 0; j < (kPieces + kLanes - 1) / kLanes; ++j) {
-          const int c = j * kLanes * 16 + piece;
-          if (kPieces % kLanes && c >= kPieces * 16) break;
-          const bool in = from >= 0 && c < hd * C::kElem;
-          cp16(ks + key * rb + c, kf + (in ? c : 0), in ? 16 : 0);
-          cp16(vs + key * rb + c, vf + (in ? c : 0), in ? 16 : 0);
+          for (int j = 0; j < (kPieces + kLanes - 1) / kLanes; ++j) {
+            const int c = j * kLanes * 16;
+            if (kPieces % kLanes && c + piece >= kPieces * 16) break;
+            cp16(ks + key * rb + piece + c, kf + c, 16);
+            cp16(vs + key * rb + piece + c, vf + c, 16);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kTile / kKeys; ++i) {
+          const int key = i * kKeys + lane / kLanes;
+          const int from = __shfl_sync(0xFFFFFFFFu, row, key);
+          const uint8_t* kf = k_piece + static_cast<int64_t>(max(from, 0)) * (hd * C::kElem) - piece;
+#pragma unroll
+          for (int j = 0; j < (kPieces + kLanes - 1) / kLanes; ++j) {
+            const int c = j * kLanes * 16 + piece;
+            if (kPieces % kLanes && c >= kPieces * 16) break;
+            const bool in = from >= 0 && c < hd * C::kElem;
+            cp16(ks + key * rb + c, kf + (in ? c : 0), in ? 16 : 0);
+            cp16(vs + key * rb + c, kf + v_apart + (in ? c : 0), in ? 16 : 0);
+          }
         }
       }
     }
-    if (prime < plan.stages) {
+    if (prime < kStages) {
       cp_commit();
-      if (++ld_stage == plan.stages) ld_stage = 0;
+      if (++ld_stage == kStages) ld_stage = 0;
     }
     next = after;
     after.kvh = -1;
@@ -829,10 +937,9 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
     }
     const int row = at.row, kvh = at.kvh, part = at.part;
     float2* to = nullptr;  // where this range's part of the segment goes; null: the output
-    float m = -INFINITY, l = 0.0f;
-    float o[kPairs][2];
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) o[i][0] = o[i][1] = 0.0f;
+    float m = -INFINITY, l = 0.0f, unit = 1.0f;
+    Output<HDT, C::kWide> o;
+    o.clear();
     const float sink = sink_next;
     {
       const int n = min(at.tiles - at.tile, end - x), h0 = kvh * G + part * kDecodeHeads;
@@ -843,13 +950,20 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
       // the queries go through the stage that is free until the next load
       typename C::Q q;
       {
-        float* qs = reinterpret_cast<float*>(mine + ld_stage * plan.stage_bytes);
+        float* qs = reinterpret_cast<float*>(mine + ld_stage * kStageBytes);
         queries.store(qs, lane);
         __syncwarp();
         C::load(q, qs + g * HDT, t);
         __syncwarp();
       }
+      // Scores stay as the product gives them where a positive factor alone
+      // stands between them and the exponent: e^(unit (s - m)) = 2^(c (s - m)).
+      // With a bias they are brought to its unit first; the difference comes
+      // before log2 e, so that the type's lowest values stay apart from -inf.
       const float ks = p.scale * q.back * (p.c.k_scale ? p.c.k_scale[kvh] : 1.0f);
+      const bool plain = !p.bias && ks > 0.0f;
+      unit = plain ? ks : 1.0f;
+      const float c = unit * kLog2e;
       const float* bias = p.bias && part * kDecodeHeads + g < G ? p.bias + row * p.bias_row + (h0 + g) * p.bias_head : nullptr;
       last_piece = x + n >= end;
       if (!last_piece) {
@@ -869,7 +983,7 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
 #pragma unroll 1
       for (int j = in_group; j < n;) {
         if (prime == 0) {
-          cp_wait_for(plan.stages - 2);
+          cp_wait<kStages - 2>();
           __syncwarp();
         }
         load_tile();
@@ -877,48 +991,54 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
           --prime;
           continue;
         }
-        const uint32_t k = smem_u32(mine) + stage * plan.stage_bytes, v = k + kTile * rb;
+        const uint32_t k = smem_u32(mine) + stage * kStageBytes, v = k + kTile * rb;
         float s[4 * NT], w[4 * NT];
         C::scores(s, q, k, lane);
-        const uint32_t keys = there[warp][stage] >> (2 * t);
-        float top = m;
-#pragma unroll
-        for (int i = 0; i < 4 * NT; ++i) s[i] *= ks;
-        if (bias) {
+        typename C::V values;
+        C::load(values, v, lane);
+        if (!plain) {
 #pragma unroll
           for (int i = 0; i < 4 * NT; ++i) {
+            s[i] *= ks;
             const int key = at.lo + (at.tile + j) * kTile + 8 * (i >> 1) + (i & 1) + 2 * t;
-            if (key < p.bias_len && key < at.len) s[i] += bias[key];
+            if (bias && key < p.bias_len && key < at.len) s[i] += bias[key];
           }
         }
+        const uint32_t keys = there[warp][stage];
+        if (keys != kAllKeys) {
 #pragma unroll
-        for (int i = 0; i < 4 * NT; ++i) {
-          if (!(keys >> (8 * (i >> 1) + (i & 1)) & 1)) s[i] = -INFINITY;
-          top = fmaxf(top, s[i]);
+          for (int i = 0; i < 4 * NT; ++i)
+            if (!(keys >> (2 * t + 8 * (i >> 1) + (i & 1)) & 1)) s[i] = -INFINITY;
         }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 4 * NT; ++i) top = fmaxf(top, s[i]);
         if (p.track && x + j < ws.score_tiles) {
 #pragma unroll
           for (int u = 0; u < NT; ++u)
             *reinterpret_cast<float4*>(ws.scores + ((static_cast<int64_t>(x + j) * NT + u) * 32 + lane) * 4) =
-                make_float4(s[4 * u], s[4 * u + 1], s[4 * u + 2], s[4 * u + 3]);
+                make_float4(s[4 * u] * unit, s[4 * u + 1] * unit, s[4 * u + 2] * unit, s[4 * u + 3] * unit);
         }
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        const float corr = exp_diff(m, top);
+        top = fmaxf(top, m);
+        const float base = top == -INFINITY ? 0.0f : top, corr = ex2((m - base) * c);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4 * NT; ++i) {
-          w[i] = exp_diff(s[i], top);
+          w[i] = ex2((s[i] - base) * c);
           sum += w[i];
         }
         l = fmaf(l, corr, sum);
+        if (!C::kWide && __any_sync(0xFFFFFFFFu, top != m)) o.scale(corr);
         m = top;
-        C::add(o, w, corr, v, lane);
+        C::add(o, values, w, corr, v, lane);
         __syncwarp();
-        if (++stage == plan.stages) stage = 0;
+        if (++stage == kStages) stage = 0;
         j += wg;
       }
-      l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+      m *= unit;
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
       l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
       x += n;
       if (x < end) at.next_segment(p, rows, parts);
@@ -926,21 +1046,21 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
 
     if (to && wg == 1) {
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) to[32 * i + lane] = make_float2(o[i][0], o[i][1]);
+      for (int i = 0; i < kPairs; ++i) to[32 * i + lane] = o.pair(i);
       if (t == 0) to[32 * kPairs + g] = make_float2(m, l);
       continue;
     }
     // The group's warps join in shared memory, each in the stage that it loads
     // next: nothing uses that until then.
     const int heads = min(kDecodeHeads, G - part * kDecodeHeads), h = kvh * G + part * kDecodeHeads + g;
-    float2* mo = reinterpret_cast<float2*>(mine + ld_stage * plan.stage_bytes);
+    float2* mo = reinterpret_cast<float2*>(mine + ld_stage * kStageBytes);
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) mo[32 * i + lane] = make_float2(o[i][0], o[i][1]);
+    for (int i = 0; i < kPairs; ++i) mo[32 * i + lane] = o.pair(i);
     if (t == 0) {
       join_ml[warp][g][0] = m;
       join_ml[warp][g][1] = l;
     }
-    if (lane == 0) join_at[warp] = (warp * plan.stages + ld_stage) * plan.stage_bytes;
+    if (lane == 0) join_at[warp] = (warp * kStages + ld_stage) * kStageBytes;
     group_sync();
     // nt is a multiple of 32: a thread's head is its lane's for every pair
     float top = -INFINITY, sum = 0.0f;
@@ -1063,9 +1183,11 @@ template <class C, int HDT>
 cudaError_t launch(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st) {
   static_assert(2 * C::kWarps * stage_bytes(HDT, C::kElem) <= kRingBytes, "a ring has at least two stages");
   const auto fn = attend_kernel<C, HDT>;
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fn), plan.smem);
+  // the warps' rings, and 128 bytes that a read past the last row may touch
+  constexpr size_t smem = C::kWarps * C::kStages * C::kStageBytes + 128;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fn), smem);
   if (e != cudaSuccess) return e;
-  e = launch_kernel(fn, dim3(plan.grid), dim3(32 * plan.warps), plan.smem, st, p, ws, plan);
+  e = launch_kernel(fn, dim3(plan.grid), dim3(32 * C::kWarps), smem, st, p, ws, plan);
   if (e != cudaSuccess || plan.whole) return e;
   const int G = p.c.n_heads / p.c.kv_heads, n_segs = p.rows * p.c.kv_heads * ((G + kDecodeHeads - 1) / kDecodeHeads);
   constexpr int slices = HDT / 8 % 4 ? HDT / 40 : HDT / 32;
