@@ -22,6 +22,7 @@ struct mxmqa_paged_cache {
   mxmqa_paged_config cfg{};
   mxmoe::PagedView view{};
   mxmoe::DecodeScratch scratch{};
+  void* workspace = nullptr;
   int sms = 148;
 };
 
@@ -57,17 +58,6 @@ struct PDevice {
     if (prev >= 0) cudaSetDevice(prev);
   }
 };
-
-template <typename T>
-int palloc(T** p, size_t n, bool zero) {
-  const cudaError_t e = cudaMalloc(reinterpret_cast<void**>(p), n * sizeof(T));
-  if (e != cudaSuccess) {
-    *p = nullptr;
-    return pfail(MXMOE_ERR_OOM, "cudaMalloc(%zu bytes): %s", n * sizeof(T), cudaGetErrorString(e));
-  }
-  if (zero) P_CUDA(cudaMemset(*p, 0, n * sizeof(T)));
-  return MXMOE_OK;
-}
 
 constexpr uint64_t kMaxTokens = 0x7FFFFFFFu;
 
@@ -193,26 +183,45 @@ int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers*
     delete c;
     return pfail(MXMOE_ERR_CUDA, "device %d is not available", cfg->device);
   }
-  // Everything that the calls need is allocated here, once: a tracked decode
-  // keeps the scores of every cached token (32 bytes per token, key head and 8
-  // query heads).
+  // Everything that the calls need is allocated here, once and in one piece: a
+  // tracked decode keeps the scores of every cached token (32 bytes per token,
+  // key head and 8 query heads).
   mxmoe::DecodeScratch& ws = c->scratch;
   const size_t group = cfg->n_heads / cfg->kv_heads, segs = cfg->kv_heads * ((group + mxmoe::kDecodeHeads - 1) / mxmoe::kDecodeHeads);
-  int rc = palloc(&w.status, 1, true);
-  if (rc == MXMOE_OK) rc = palloc(&ws.part, mxmoe::decode_part_floats(w, c->sms), false);
-  if (rc == MXMOE_OK) rc = palloc(&ws.taken, 2, true);
-  if (rc == MXMOE_OK) rc = palloc(&ws.held, mxmoe::kDecodeMaxRows * segs, false);
-  if (rc == MXMOE_OK && w.weight) {
-    ws.score_tiles = static_cast<int64_t>(
-        (static_cast<uint64_t>(cfg->n_pages) * cfg->page_size / mxmoe::decode_tile(w) + mxmoe::kDecodeMaxRows) * segs);
-    rc = palloc(&ws.scores, static_cast<size_t>(ws.score_tiles) * mxmoe::decode_tile(w) * 8, false);
-    if (rc == MXMOE_OK) rc = palloc(&ws.lse, static_cast<size_t>(mxmoe::kDecodeMaxRows) * cfg->n_heads, false);
+  const size_t tile = mxmoe::decode_tile(w);
+  if (w.weight)
+    ws.score_tiles = static_cast<int64_t>((static_cast<uint64_t>(cfg->n_pages) * cfg->page_size / tile + mxmoe::kDecodeMaxRows) * segs);
+  size_t bytes = 0;
+  auto room = [&bytes](size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  const size_t head = room(3 * sizeof(int)), held = room(mxmoe::kDecodeMaxRows * segs * sizeof(int2));
+  const size_t part = room(mxmoe::decode_part_floats(w, c->sms) * sizeof(float));
+  const size_t lse = room(w.weight ? mxmoe::kDecodeMaxRows * cfg->n_heads * sizeof(float) : 0);
+  const size_t scores = room(static_cast<size_t>(ws.score_tiles) * tile * 8 * sizeof(float));
+  char* base = nullptr;
+  int rc = MXMOE_OK;
+  const cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&base), bytes);
+  if (e != cudaSuccess) {
+    rc = pfail(MXMOE_ERR_OOM, "cudaMalloc(%zu bytes): %s", bytes, cudaGetErrorString(e));
+  } else if (cudaMemset(base, 0, 3 * sizeof(int)) != cudaSuccess) {
+    cudaFree(base);
+    rc = pfail(MXMOE_ERR_CUDA, "cudaMemset of the workspace failed");
   }
   if (rc != MXMOE_OK) {
     cudaGetLastError();
-    mxmqa_paged_destroy(c);
+    delete c;
     return rc;
   }
+  c->workspace = base;
+  w.status = reinterpret_cast<int*>(base + head);
+  ws.taken = w.status + 1;
+  ws.held = reinterpret_cast<int2*>(base + held);
+  ws.part = reinterpret_cast<float*>(base + part);
+  ws.lse = reinterpret_cast<float*>(base + lse);
+  ws.scores = reinterpret_cast<float*>(base + scores);
   *out = c;
   return MXMOE_OK;
 }
@@ -220,12 +229,7 @@ int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers*
 int mxmqa_paged_destroy(mxmqa_paged_cache* c) {
   if (!c) return MXMOE_OK;
   PDevice g(c->cfg.device);
-  cudaFree(c->view.status);
-  cudaFree(c->scratch.part);
-  cudaFree(c->scratch.taken);
-  cudaFree(c->scratch.held);
-  cudaFree(c->scratch.scores);
-  cudaFree(c->scratch.lse);
+  cudaFree(c->workspace);
   delete c;
   return MXMOE_OK;
 }

@@ -205,6 +205,14 @@ struct Output {
   }
 };
 
+// Two scores of a lane from the two row halves of a product, or added to them:
+// in 32 bits no more than four MMAs in a row add up, as each cuts its sum off.
+template <int N>
+__device__ __forceinline__ void sum_pair(float (&s)[N], int j, const float (&d)[4], bool first) {
+  s[2 * j] = first ? d[0] + d[2] : s[2 * j] + (d[0] + d[2]);
+  s[2 * j + 1] = first ? d[1] + d[3] : s[2 * j + 1] + (d[1] + d[3]);
+}
+
 // ---- the cache's element types ----
 //
 // Each has: Q, the query operand; V, values on their way; load(), which fills them for lane (g, t) =
@@ -259,18 +267,20 @@ struct Bf16 {
 #pragma unroll
         for (int j = 0; j < 2 * NT; ++j) {
           const uint32_t b0 = b[e][j / 2][2 * (j & 1)], b1 = b[e][j / 2][2 * (j & 1) + 1];
-          if (i == 0)
+          if (i == 0 || X && i % 2 == 0)
             mma_bf16_new(c[j], q.a[i][0], l0, q.a[i][1], l1, b0, b1);
           else
             mma_bf16(c[j], q.a[i][0], l0, q.a[i][1], l1, b0, b1);
           if (X) mma_bf16(c[j], q.a[i][X ? 4 : 0], 0, q.a[i][X ? 5 : 0], 0, b0, b1);
+          if (X && (i % 2 == 1 || i + 1 == HDT / 16)) sum_pair(s, j, c[j], i < 2);
         }
       }
     }
+    if (X) return;
 #pragma unroll
     for (int j = 0; j < 2 * NT; ++j) {
-      s[2 * j] = X ? c[j][0] + c[j][2] : c[j][0];
-      s[2 * j + 1] = X ? c[j][1] + c[j][3] : c[j][1];
+      s[2 * j] = c[j][0];
+      s[2 * j + 1] = c[j][1];
     }
   }
   // The values of the first kPre pairs of column groups, loaded ahead of the shares.
@@ -397,17 +407,19 @@ struct E4m3 {
 #pragma unroll
         for (int j = 0; j < 2 * NT; ++j) {
           const uint32_t w = b[e / 2][j / 2][2 * (j & 1) + (e & 1)], b0 = widen(w & 0xFFFF), b1 = widen(w >> 16);
-          if (i == 0)
+          if (i == 0 || X && i % 4 == 0)
             mma_f16_new(c[j], q.a[i][0], l0, q.a[i][1], l1, b0, b1);
           else
             mma_f16(c[j], q.a[i][0], l0, q.a[i][1], l1, b0, b1);
+          if (X && (i % 4 == 3 || i + 1 == HDT / 16)) sum_pair(s, j, c[j], i < 4);
         }
       }
     }
+    if (X) return;
 #pragma unroll
     for (int j = 0; j < 2 * NT; ++j) {
-      s[2 * j] = X ? c[j][0] + c[j][2] : c[j][0];
-      s[2 * j + 1] = X ? c[j][1] + c[j][3] : c[j][1];
+      s[2 * j] = c[j][0];
+      s[2 * j + 1] = c[j][1];
     }
   }
   // All the tile's values, loaded ahead of the shares: of 32 columns and 16
@@ -500,18 +512,15 @@ struct F32 {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float x = __uint_as_float(b[2 * j]), y = __uint_as_float(b[2 * j + 1]);
-          if (i == 0)
-            mma_tf32_new(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], top(x), top(y));
+          float(&d)[4] = c[2 * u + j];
+          if (i % 2 == 0)
+            mma_tf32_new(d, q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], rest(x), rest(y));
           else
-            mma_tf32(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], top(x), top(y));
-          mma_tf32(c[2 * u + j], q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], rest(x), rest(y));
+            mma_tf32(d, q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], rest(x), rest(y));
+          mma_tf32(d, q.a[i][0], q.a[i][2], q.a[i][1], q.a[i][3], top(x), top(y));
+          if (i % 2 == 1) sum_pair(s, 2 * u + j, d, i < 2);
         }
       }
-    }
-#pragma unroll
-    for (int j = 0; j < 2 * NT; ++j) {
-      s[2 * j] = c[j][0] + c[j][2];
-      s[2 * j + 1] = c[j][1] + c[j][3];
     }
   }
   struct V {};
