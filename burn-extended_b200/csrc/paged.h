@@ -111,19 +111,21 @@ __device__ __forceinline__ int page_of(const PagedView& c, int n) {
 }
 
 // The slot of cache index n of a table row: (page * kv_heads + 0) * page_size + n % page_size, head h's is
-// page_size * h further.  -1 where the table has none.
-__device__ __forceinline__ int64_t slot_of(const PagedView& c, const PagedTables& t, int row, int n) {
+// page_size * h further.  -1 where the table has none; its bit joins `bad`.
+__device__ __forceinline__ int64_t slot_of(const PagedView& c, const PagedTables& t, int row, int n, int& bad) {
   const int pi = page_of(c, n);
-  if (n < 0 || pi >= t.max_pages) {
-    atomicOr(c.status, kPagedBadIndex);
-    return -1;
-  }
-  const int page = __ldg(t.tables + row * t.stride + pi);
-  if (page < 0 || page >= c.n_pages) {
-    atomicOr(c.status, kPagedBadPage);
-    return -1;
-  }
-  return static_cast<int64_t>(page) * c.kv_heads * c.page_size + (n - pi * c.page_size);
+  const bool in = n >= 0 && pi < t.max_pages;
+  const int page = in ? __ldg(t.tables + row * t.stride + pi) : 0;
+  const bool ok = page >= 0 && page < c.n_pages;
+  bad |= !in ? kPagedBadIndex : !ok ? kPagedBadPage : 0;
+  return in && ok ? static_cast<int64_t>(page) * c.kv_heads * c.page_size + (n - pi * c.page_size) : -1;
+}
+// The same, its bit set in the status word at once.
+__device__ __forceinline__ int64_t slot_of(const PagedView& c, const PagedTables& t, int row, int n) {
+  int bad = 0;
+  const int64_t s = slot_of(c, t, row, n, bad);
+  if (bad) atomicOr(c.status, bad);
+  return s;
 }
 #endif
 

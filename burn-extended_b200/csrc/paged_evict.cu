@@ -30,8 +30,54 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int sink, int fi
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
 constexpr int kBins = 2 * kThreads;  // 11 bits a pass: the key's 32 in three
-constexpr int kFew = kThreads;       // candidates that are ranked one against another
+constexpr int kFew = 256;            // candidates that are ranked one against another
 constexpr int kMaxCluster = 8;
+
+// A list's pairs, in 16-byte pieces of keys and values, several of a thread in
+// flight: sources and destinations are never the same slots.
+__device__ __forceinline__ void move_pairs(const EvictParams& p, const int* to, const int* by, int pairs) {
+  constexpr int kAtOnce = 4;
+  const int pieces = p.c.head_dim * (p.c.dtype == MXMOE_F32 ? 4 : p.c.dtype == MXMOE_BF16 ? 2 : 1) / 16;
+  uint4 *k = static_cast<uint4*>(p.c.k), *v = static_cast<uint4*>(p.c.v);
+#pragma unroll 1
+  for (int i0 = threadIdx.x; i0 < pairs * pieces; i0 += kAtOnce * kThreads) {
+    uint4 a[kAtOnce], b[kAtOnce];
+    int64_t dst[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = i0 + j * kThreads, e = i / pieces, c = i - e * pieces;
+      dst[j] = -1;
+      if (i >= pairs * pieces || to[e] < 0 || by[e] < 0) continue;
+      dst[j] = static_cast<int64_t>(to[e]) * pieces + c;
+      const int64_t src = static_cast<int64_t>(by[e]) * pieces + c;
+      a[j] = k[src];
+      b[j] = v[src];
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (dst[j] < 0) continue;
+      k[dst[j]] = a[j];
+      v[dst[j]] = b[j];
+    }
+  }
+#pragma unroll 1
+  for (int e = threadIdx.x; e < pairs; e += kThreads) {
+    if (to[e] < 0 || by[e] < 0) continue;
+    p.c.weight[to[e]] = p.c.weight[by[e]];
+    p.c.position[to[e]] = p.c.position[by[e]];
+  }
+}
+
+// One to a bin for every lane that calls: those of the first lane's bin are
+// added together, as weights may all be alike, the others one by one.
+__device__ __forceinline__ void count_bin(int* hist, uint32_t bin) {
+  const uint32_t active = __activemask(), first = __ffs(active) - 1;
+  const uint32_t same = __ballot_sync(active, bin == __shfl_sync(active, bin, first));
+  if (!(same >> (threadIdx.x & 31) & 1))
+    atomicAdd(hist + bin, 1);
+  else if ((threadIdx.x & 31) == first)
+    atomicAdd(hist + bin, __popc(same));
+}
 
 // The sums of the warps before this one and of all, of two counts.
 __device__ __forceinline__ void over_warps(int2 x, int2* sums, int2& before, int2& all) {
@@ -63,7 +109,7 @@ __device__ __forceinline__ void over_warps(int2 x, int2* sums, int2& before, int
 // written to the list of the block that will move it, and the blocks move their
 // pairs in 16-byte pieces.  Bound by the latency of these steps where few
 // tokens move, else by the rows moved.
-__global__ void __launch_bounds__(kThreads, 1) evict_kernel(const EvictParams p, int slots) {
+__global__ void __launch_bounds__(kThreads, 1) evict_kernel(const EvictParams p, int slots, int four) {
   extern __shared__ __align__(16) uint32_t keys[];  // [slots]; then to[slots / 2 + 1], by[slots / 2 + 1]
   __shared__ __align__(16) int hist[3][kBins];
   __shared__ uint2 few[kFew];  // of block 0: the candidates' keys and indexes
@@ -95,29 +141,70 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const EvictParams p,
   const int first_recent = p.seen[row] - p.recent;
   __syncthreads();
 
-  const int share = (len + C - 1) / C, n0 = min(len, rank * share), mine = min(share, len - n0);
+  const int share = ((len + C - 1) / C + 3) / 4 * 4, n0 = min(len, rank * share), mine = min(share, len - n0);
+  int bad = 0;
   auto slot_at = [&](int n) {
-    const int64_t s = slot_of(p.c, p.t, row, n);
+    const int64_t s = slot_of(p.c, p.t, row, n, bad);
     return s < 0 ? -1 : static_cast<int>(s) + h * p.c.page_size;
   };
-#pragma unroll 4
-  for (int i = tid; i < mine; i += kThreads) {
-    const int s = slot_at(n0 + i);
-    const uint32_t k = s < 0 ? 0xFFFFFFFFu : evict_key(p.c.weight[s], p.c.position[s], p.sink, first_recent);
-    keys[i] = k;
-    atomicAdd(&hist[0][k >> 21], 1);
+  if (four) {
+    // four slots of one page at a time: page_size and n0 are multiples of four
+    constexpr int kAtOnce = 4;
+#pragma unroll 1
+    for (int i0 = 4 * tid; i0 < mine; i0 += 4 * kAtOnce * kThreads) {
+      int at[kAtOnce];
+      float4 w[kAtOnce];
+      int4 q[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) at[j] = i0 + 4 * j * kThreads < mine ? slot_at(n0 + i0 + 4 * j * kThreads) : -1;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (at[j] < 0) continue;
+        w[j] = *reinterpret_cast<const float4*>(p.c.weight + at[j]);
+        q[j] = *reinterpret_cast<const int4*>(p.c.position + at[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int i = i0 + 4 * j * kThreads;
+        if (i >= mine) break;
+        uint4 k = make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);
+        if (at[j] >= 0)
+          k = make_uint4(evict_key(w[j].x, q[j].x, p.sink, first_recent), evict_key(w[j].y, q[j].y, p.sink, first_recent),
+                         evict_key(w[j].z, q[j].z, p.sink, first_recent), evict_key(w[j].w, q[j].w, p.sink, first_recent));
+        *reinterpret_cast<uint4*>(keys + i) = k;  // `slots` is a multiple of four
+      }
+    }
+    __syncthreads();
+  } else {
+    constexpr int kAtOnce = 8;  // slots of a thread whose loads are in flight together
+#pragma unroll 1
+    for (int i0 = tid; i0 < mine; i0 += kAtOnce * kThreads) {
+      int at[kAtOnce], position[kAtOnce];
+      float weight[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) at[j] = i0 + j * kThreads < mine ? slot_at(n0 + i0 + j * kThreads) : -1;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        weight[j] = at[j] < 0 ? 0.0f : p.c.weight[at[j]];
+        position[j] = at[j] < 0 ? 0 : p.c.position[at[j]];
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (i0 + j * kThreads < mine)
+          keys[i0 + j * kThreads] = at[j] < 0 ? 0xFFFFFFFFu : evict_key(weight[j], position[j], p.sink, first_recent);
+    }
   }
+  if (bad) atomicOr(p.c.status, bad);
   int need = len - p.budget, candidates = len;  // victims among the keys that share the prefix
   uint32_t prefix = 0;
   int above = 32;  // the prefix's lowest bit
 #pragma unroll 1
   for (int pass = 0; pass < 3 && (pass == 0 || candidates > kFew); ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    if (pass > 0) {
-      for (int i = tid; i < mine; i += kThreads) {
-        const uint32_t k = keys[i];
-        if (k >> above == prefix >> above) atomicAdd(&hist[pass][(k >> shift) & (kBins - 1)], 1);
-      }
+#pragma unroll 2
+    for (int i = tid; i < mine; i += kThreads) {
+      const uint32_t k = keys[i];
+      if (pass == 0 || k >> above == prefix >> above) count_bin(hist[pass], (k >> shift) & (kBins - 1));
     }
     sync();
     int2 bin = make_int2(0, 0);
@@ -219,13 +306,15 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const EvictParams p,
   int* to = reinterpret_cast<int*>(keys + slots);
   int* by = to + room;
   if (own.x + own.y > 0) {
+#pragma unroll 4
     for (int i = s0 + lane; i - lane < s1; i += 32) {
       const bool in = i < s1, out = in && victim(i), low = n0 + i < p.budget;
       const uint32_t holes = __ballot_sync(0xFFFFFFFFu, out && low), movers = __ballot_sync(0xFFFFFFFFu, in && !out && !low);
+      const int slot = in && out == low ? slot_at(n0 + i) : -1;
       if (in && out == low) {
         const int e = out ? before.x + __popc(holes & ((1u << lane) - 1)) : before.y + __popc(movers & ((1u << lane) - 1));
         const int c = C == 1 ? 0 : e / per;
-        *cluster.map_shared_rank((out ? to : by) + (e - c * per), c) = slot_at(n0 + i);
+        *cluster.map_shared_rank((out ? to : by) + (e - c * per), c) = slot;
       }
       before.x += __popc(holes);
       before.y += __popc(movers);
@@ -233,23 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const EvictParams p,
   }
   sync();
 
-  const int list = min(per, pairs - rank * per), bytes = p.c.head_dim * (p.c.dtype == MXMOE_F32 ? 4 : p.c.dtype == MXMOE_BF16 ? 2 : 1);
-  const int pieces = bytes / 16;
-  uint4 *k16 = static_cast<uint4*>(p.c.k), *v16 = static_cast<uint4*>(p.c.v);
-#pragma unroll 4
-  for (int i = tid; i < list * pieces; i += kThreads) {
-    const int e = i / pieces, c = i - e * pieces;
-    if (to[e] < 0 || by[e] < 0) continue;
-    const int64_t d = static_cast<int64_t>(to[e]) * pieces + c, f = static_cast<int64_t>(by[e]) * pieces + c;
-    const uint4 a = k16[f], b = v16[f];
-    k16[d] = a;
-    v16[d] = b;
-  }
-  for (int e = tid; e < list; e += kThreads) {
-    if (to[e] < 0 || by[e] < 0) continue;
-    p.c.weight[to[e]] = p.c.weight[by[e]];
-    p.c.position[to[e]] = p.c.position[by[e]];
-  }
+  move_pairs(p, to, by, min(per, pairs - rank * per));
 }
 
 constexpr int kLongThreads = 1024;
@@ -420,7 +493,9 @@ cudaError_t launch_select(const EvictParams& p, int sms, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = C == 1 ? 1 : 2;  // one block is a cluster by itself
-  return cudaLaunchKernelEx(&cfg, evict_kernel, p, static_cast<int>(slots));
+  const int four = p.c.page_size % 4 == 0 && reinterpret_cast<uintptr_t>(p.c.weight) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(p.c.position) % 16 == 0;
+  return cudaLaunchKernelEx(&cfg, evict_kernel, p, static_cast<int>(slots), four);
 }
 
 }  // namespace
