@@ -97,7 +97,7 @@ struct DecodeScratch {
   float* lse;  // [kDecodeMaxRows][n_heads] (track)
 };
 
-cudaError_t launch_paged_append(const AppendParams& p, cudaStream_t st);
+cudaError_t launch_paged_append(const AppendParams& p, int sms, cudaStream_t st);
 cudaError_t launch_paged_decode(const DecodeParams& p, const DecodeScratch& ws, int sms, cudaStream_t st);
 int decode_tile(const PagedView& c);                     // keys of a tile
 size_t decode_part_floats(const PagedView& c, int sms);  // of DecodeScratch::part

@@ -252,7 +252,7 @@ int mxmqa_paged_status(mxmqa_paged_cache* c, void* stream) {
 int mxmqa_paged_append(mxmqa_paged_cache* c, const mxmqa_paged_append_args* a, void* stream) {
   P_CHECK(c && a, "null argument");
   P_CHECK(act_dtype(a->dtype), "bad dtype");
-  P_CHECK(a->tokens <= kMaxTokens, "too many tokens");
+  P_CHECK(a->tokens <= 1u << 30, "more than 2^30 tokens");
   if (a->tokens == 0) return MXMOE_OK;
   P_CHECK(a->k && a->v && a->index, "null k, v or index");
   P_CHECK((a->q == nullptr) == (a->q_out == nullptr), "q and q_out go together");
@@ -294,7 +294,7 @@ int mxmqa_paged_append(mxmqa_paged_cache* c, const mxmqa_paged_append_args* a, v
   p.sign = 1.0f;
   PDevice g(c->cfg.device);
   mxmoe::PdlScope pdl(true);  // every kernel waits for the one before it in the stream
-  P_CUDA(mxmoe::launch_paged_append(p, static_cast<cudaStream_t>(stream)));
+  P_CUDA(mxmoe::launch_paged_append(p, c->sms, static_cast<cudaStream_t>(stream)));
   return MXMOE_OK;
 }
 
@@ -408,7 +408,7 @@ int mxmqa_rotary_table(const mxmqa_rotary_config* r, uint32_t first, uint32_t n,
 int mxmqa_rotary(const mxmqa_rotary_args* a, void* stream) {
   P_CHECK(a, "null argument");
   P_CHECK(act_dtype(a->dtype), "bad dtype");
-  P_CHECK(a->tokens <= kMaxTokens && a->heads <= 65535 && a->head_dim <= 65536, "too many tokens, heads or columns");
+  P_CHECK(a->tokens <= 1u << 30 && a->heads <= 65535 && a->head_dim <= 65536, "too many tokens, heads or columns");
   if (a->tokens == 0 || a->heads == 0 || a->head_dim == 0) return MXMOE_OK;
   P_CHECK(a->x && a->out && (a->positions || a->rot_dim == 0), "null x, out or positions");
   const size_t es = elem_bytes(a->dtype);
@@ -434,7 +434,9 @@ int mxmqa_rotary(const mxmqa_rotary_args* a, void* stream) {
   p.sign = a->inverse ? -1.0f : 1.0f;
   PDevice g(a->device);
   mxmoe::PdlScope pdl(true);  // every kernel waits for the one before it in the stream
-  P_CUDA(mxmoe::launch_paged_append(p, static_cast<cudaStream_t>(stream)));
+  int sms = 0;
+  P_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, a->device));
+  P_CUDA(mxmoe::launch_paged_append(p, sms, static_cast<cudaStream_t>(stream)));
   return MXMOE_OK;
 }
 

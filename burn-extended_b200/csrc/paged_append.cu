@@ -136,50 +136,83 @@ __device__ __forceinline__ void store_cache(void* pool, int dtype, int64_t at, c
   }
 }
 
+// A unit of a head: one piece, or the two that turn together.
+template <typename T, bool kInterleaved>
+struct Unit {
+  static constexpr int N = Piece<T>::kN;
+  Piece<T> a, b;
+
+  __device__ __forceinline__ void load(const T* x, int apart, bool two) {
+    a.load(x);
+    if (two) b.load(x + apart);
+  }
+  __device__ __forceinline__ void turn(const float (&c)[N], const float (&s)[N], bool turns, bool two, float (&x)[N],
+                                       float (&y)[N]) const {
+    a.open(x);
+    if (two) {
+      b.open(y);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float u = x[j], w = y[j];
+        x[j] = u * c[j] - w * s[j];
+        y[j] = w * c[j] + u * s[j];
+      }
+    } else if (kInterleaved && turns) {
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        const float u = x[j], w = x[j + 1];
+        x[j] = u * c[j / 2] - w * s[j / 2];
+        x[j + 1] = w * c[j / 2] + u * s[j / 2];
+      }
+    }
+  }
+};
+
 // One block per token; everything moves in 16-byte pieces.  A thread keeps one
-// unit of columns (a pair of pieces that turn together, or one piece) for
-// several heads, so the token's cosines are read once per thread; up to
-// kBatch heads' loads are in flight while the token's index, page and cosines
-// come.  Memory-bound: each value is read and written once.
-constexpr int kBatch = 3;
+// unit of columns for every `per_pass`-th query head, so the token's cosines are
+// read once per thread; then the keys' units and the values' pieces are shared
+// out over the block.  The loads of up to kBatch query heads, a key unit and a
+// value piece are in flight while the token's index, page and cosines come.
+// Memory-bound: each value is read and written once.
+constexpr int kBatch = 2;
 template <typename T, bool kInterleaved, bool kMany>
 __global__ void __launch_bounds__(kMany ? 128 : 512, kMany ? 7 : 1) append_wide_kernel(const AppendParams p, int units, int per_pass) {
   constexpr int N = Piece<T>::kN;
   griddep_wait();
   griddep_launch_dependents();
-  const int t = blockIdx.x, hd = p.c.head_dim, half = p.rot / 2;
+  const int t = blockIdx.x, hd = p.c.head_dim, half = p.rot / 2, nt = blockDim.x, tid = threadIdx.x;
   const int nH = p.q ? p.c.n_heads : 0, H = p.k ? p.c.kv_heads : 0;
-  const int unit = threadIdx.x % units, first = threadIdx.x / units;
-  const bool on = first < per_pass;
-  const bool turns = unit * N < (kInterleaved ? p.rot : half);
-  const int ca = kInterleaved || turns ? unit * N : half + unit * N, cb = ca + half;
-  const bool two = !kInterleaved && turns;
-  Piece<T> a[kBatch], b[kBatch];
-  auto load = [&](int h0) {
+  const int first = tid / units, unit = tid - first * units;
+  const bool turns = unit * N < (kInterleaved ? p.rot : half), two = !kInterleaved && turns;
+  const int ca = kInterleaved || turns ? unit * N : half + unit * N;
+  const T* q = static_cast<const T*>(p.q) + t * p.q_token + first * p.q_head + ca;
+  T* q_out = static_cast<T*>(p.q_out) + t * p.qo_token + first * p.qo_head + ca;
+  const int64_t q_step = per_pass * p.q_head, qo_step = per_pass * p.qo_head;
+  const int mine = first < per_pass && first < nH ? (nH - first + per_pass - 1) / per_pass : 0;  // query heads of this thread
+  Unit<T, kInterleaved> u[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int h = h0 + i * per_pass;
-      if (!on || h >= nH + H) continue;
-      const T* x = h < nH ? static_cast<const T*>(p.q) + t * p.q_token + h * p.q_head
-                          : static_cast<const T*>(p.k) + t * p.k_token + (h - nH) * p.k_head;
-      a[i].load(x + ca);
-      if (two) b[i].load(x + cb);
-    }
-  };
-  load(first);
-  const int pieces = hd / N, v_all = H * pieces;
+  for (int i = 0; i < kBatch; ++i)
+    if (i < mine) u[i].load(q + i * q_step, half, two);
+  // Keys: unit e % units of head e / units; a thread's columns are the same as
+  // for the queries where per_pass heads fill the block, so that the first
+  // round takes the cosines that it has.
+  const int v_pieces = hd / N, v_all = H * v_pieces;
+  const bool has_key = first < per_pass && first < H;
+  Unit<T, kInterleaved> ku;
+  if (has_key) ku.load(static_cast<const T*>(p.k) + t * p.k_token + first * p.k_head + ca, half, two);
   auto value_at = [&](int i) {
-    const int h = i / pieces;
-    return static_cast<const T*>(p.v) + t * p.v_token + h * p.v_head + (i - h * pieces) * N;
+    const int h = i / v_pieces;
+    return static_cast<const T*>(p.v) + t * p.v_token + h * p.v_head + (i - h * v_pieces) * N;
   };
+  const int v0 = nt - 1 - tid;  // from the block's other end, where no keys are
   Piece<T> v;
-  if (threadIdx.x < v_all) v.load(value_at(threadIdx.x));
+  if (v0 < v_all) v.load(value_at(v0));
   const Token k = token_of(p, t);
   __align__(16) float c[N];  // interleaved: the first half of them
   __align__(16) float s[N];
-  if (turns && on) {
+  if (turns && (mine > 0 || has_key)) {
     const int from = kInterleaved ? unit * N / 2 : unit * N;
-constexpr int kCos = kInterleaved ? N / 2 : N, kAtOnce = kCos % 4 ? 2 : 4;
+    constexpr int kCos = kInterleaved ? N / 2 : N, kAtOnce = kCos % 4 ? 2 : 4;
 #pragma unroll
     for (int i = 0; i < kCos; i += kAtOnce) {
       if (kAtOnce == 4) {
@@ -193,54 +226,49 @@ constexpr int kCos = kInterleaved ? N / 2 : N, kAtOnce = kCos % 4 ? 2 : 4;
 #pragma unroll
     for (int i = 0; i < kCos; ++i) s[i] *= p.sign;
   }
+  float x[N], y[N];
 #pragma unroll 1
-  for (int h0 = first; on && h0 < nH + H; h0 += kBatch * per_pass) {
-    if (h0 != first) load(h0);
+  for (int i0 = 0; i0 < mine; i0 += kBatch) {
+    if (i0 > 0) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (i0 + i < mine) u[i].load(q + i * q_step, half, two);
+    }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int h = h0 + i * per_pass;
-      if (h >= nH + H) break;
-      float x[N], y[N];
-      a[i].open(x);
-      if (two) {
-        b[i].open(y);
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float u = x[j], w = y[j];
-          x[j] = u * c[j] - w * s[j];
-          y[j] = w * c[j] + u * s[j];
-        }
-      } else if (turns) {
-#pragma unroll
-        for (int j = 0; j < N; j += 2) {
-          const float u = x[j], w = x[j + 1];
-          x[j] = u * c[j / 2] - w * s[j / 2];
-          x[j + 1] = w * c[j / 2] + u * s[j / 2];
-        }
+      if (i0 + i >= mine) break;
+      u[i].turn(c, s, turns, two, x, y);
+      store(q_out + i * qo_step, x);
+      if (two) store(q_out + i * qo_step + half, y);
+    }
+    q += kBatch * q_step;
+    q_out += kBatch * qo_step;
+  }
+  if (first < per_pass) {
+#pragma unroll 1
+    for (int h = first; h < H; h += per_pass) {
+      if (h != first) ku.load(static_cast<const T*>(p.k) + t * p.k_token + h * p.k_head + ca, half, two);
+      ku.turn(c, s, turns, two, x, y);
+      if (p.k_out) {
+        T* out = static_cast<T*>(p.k_out) + t * p.ko_token + h * p.ko_head + ca;
+        store(out, x);
+        if (two) store(out + half, y);
       }
-      const int kh = h - nH;
-      T* out = kh < 0 ? static_cast<T*>(p.q_out) + t * p.qo_token + h * p.qo_head
-                      : (p.k_out ? static_cast<T*>(p.k_out) + t * p.ko_token + kh * p.ko_head : nullptr);
-      if (out) {
-        store(out + ca, x);
-        if (two) store(out + cb, y);
-      }
-      if (kh >= 0 && k.slot >= 0) {
-        const int64_t at = (k.slot + static_cast<int64_t>(kh) * p.c.page_size) * hd;
-        const float inv = p.c.k_scale ? 1.0f / __ldg(p.c.k_scale + kh) : 1.0f;
-        store_cache(p.c.k, p.c.dtype, at + ca, x, inv);
-        if (two) store_cache(p.c.k, p.c.dtype, at + cb, y, inv);
+      if (k.slot >= 0) {
+        const int64_t at = (k.slot + static_cast<int64_t>(h) * p.c.page_size) * hd + ca;
+        const float inv = p.c.k_scale ? 1.0f / __ldg(p.c.k_scale + h) : 1.0f;
+        store_cache(p.c.k, p.c.dtype, at, x, inv);
+        if (two) store_cache(p.c.k, p.c.dtype, at + half, y, inv);
       }
     }
   }
   if (k.slot >= 0) {
 #pragma unroll 1
-    for (int i = threadIdx.x; i < v_all; i += blockDim.x) {
-      if (i >= static_cast<int>(blockDim.x)) v.load(value_at(i));
-      const int h = i / pieces;
-      float x[N];
+    for (int i = v0; i < v_all; i += nt) {
+      if (i != v0) v.load(value_at(i));
+      const int h = i / v_pieces;
       v.open(x);
-      store_cache(p.c.v, p.c.dtype, (k.slot + static_cast<int64_t>(h) * p.c.page_size) * hd + (i - h * pieces) * N, x,
+      store_cache(p.c.v, p.c.dtype, (k.slot + static_cast<int64_t>(h) * p.c.page_size) * hd + (i - h * v_pieces) * N, x,
                   p.c.v_scale ? 1.0f / __ldg(p.c.v_scale + h) : 1.0f);
     }
   }
@@ -315,7 +343,7 @@ bool wide(const void* p, int64_t a, int64_t b, int n, size_t elem) {
 }
 
 template <typename T>
-cudaError_t launch_append(const AppendParams& p, cudaStream_t st) {
+cudaError_t launch_append(const AppendParams& p, int sms, cudaStream_t st) {
   constexpr int N = Piece<T>::kN;
   const int hd = p.c.head_dim, half = p.rot / 2;
   const bool aligned = wide(p.q, p.q_token, p.q_head, hd, sizeof(T)) && wide(p.k, p.k_token, p.k_head, hd, sizeof(T)) &&
@@ -325,9 +353,10 @@ cudaError_t launch_append(const AppendParams& p, cudaStream_t st) {
   if (!aligned || units > 512) return launch_kernel(append_kernel<T>, dim3(p.tokens), dim3(256), 0, st, p);
   // Threads of a token: enough of them to fill the SMs (2048 a SM), up to a
   // thread per unit for the shortest chain; at 128 seven blocks share a SM.
-  const int heads = (p.q ? p.c.n_heads : 0) + (p.k ? p.c.kv_heads : 0);
-  const int want = std::min(512, std::max(128, 148 * 2048 / p.tokens / 32 * 32)), passes = (heads * units + want - 1) / want;
-  const int per_pass = (heads + passes - 1) / passes, threads = (per_pass * units + 31) / 32 * 32;
+  const int heads = p.q ? p.c.n_heads : p.c.kv_heads;
+  const int want = std::max(units, std::min(512, std::max(128, sms * 2048 / p.tokens / 32 * 32)));
+  const int passes = (heads * units + want - 1) / want, per_pass = std::min(want / units, (heads + passes - 1) / passes);
+  const int threads = (per_pass * units + 31) / 32 * 32;
   const auto fn = threads <= 128 ? (p.interleaved ? append_wide_kernel<T, true, true> : append_wide_kernel<T, false, true>)
                                  : (p.interleaved ? append_wide_kernel<T, true, false> : append_wide_kernel<T, false, false>);
   return launch_kernel(fn, dim3(p.tokens), dim3(threads), 0, st, p, units, per_pass);
@@ -335,8 +364,8 @@ cudaError_t launch_append(const AppendParams& p, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_paged_append(const AppendParams& p, cudaStream_t st) {
-  return p.dtype == MXMOE_BF16 ? launch_append<__nv_bfloat16>(p, st) : launch_append<float>(p, st);
+cudaError_t launch_paged_append(const AppendParams& p, int sms, cudaStream_t st) {
+  return p.dtype == MXMOE_BF16 ? launch_append<__nv_bfloat16>(p, sms, st) : launch_append<float>(p, sms, st);
 }
 
 cudaError_t launch_rotary_table(const double* inv_freq, int half, int64_t first, int n, double factor, float* cos,

@@ -48,6 +48,13 @@ __global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const 
     decode::Place at;
     at.find(p, rows, 1, x);
     const int first = (before[at.row] * H + at.kvh * at.tiles) * hgroups + at.tile;
+    // The slot of the key that lane (g, t) will add to, and its weight, are on
+    // their way while the shares are computed.
+    const int n = at.lo + at.tile * 16 * NT + 8 * (g >> 1) + 2 * t + (g & 1);
+    int64_t slot = -1;
+    if (g < 4 * NT && n < at.len) slot = slot_of(p.c, p.t, at.row, n);
+    float* const weight = p.c.weight + slot + static_cast<int64_t>(at.kvh) * p.c.page_size;
+    const float old = slot >= 0 ? *weight : 0.0f;
     float w[4 * NT] = {};
     for (int hg = 0; hg < hgroups; ++hg) {
       const int h = hg * kDecodeHeads + g;
@@ -68,14 +75,10 @@ __global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const 
 #pragma unroll
       for (int i = 0; i < 4 * NT; ++i) w[i] += __shfl_xor_sync(0xFFFFFFFFu, w[i], o);
     // w[i] is key 8 (i / 2) + 2t + i % 2; lane (g, t) takes i = g
-    if (g >= 4 * NT) continue;
-    const int n = at.lo + at.tile * 16 * NT + 8 * (g >> 1) + 2 * t + (g & 1);
-    if (n >= at.len) continue;
     float add = w[0];
 #pragma unroll
     for (int i = 1; i < 4 * NT; ++i) add = g == i ? w[i] : add;
-    const int64_t slot = slot_of(p.c, p.t, at.row, n);
-    if (slot >= 0) p.c.weight[slot + static_cast<int64_t>(at.kvh) * p.c.page_size] += add;
+    if (slot >= 0) *weight = old + add;
   }
 }
 

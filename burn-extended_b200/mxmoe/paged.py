@@ -41,14 +41,12 @@ def _act(name: str, t) -> int:
     return code
 
 
-def _heads(name: str, t, n: int, heads: int, head_dim: int, device):
-    """[n, heads, head_dim] with contiguous columns -> strides of the first two dimensions."""
-    if t.shape != (n, heads, head_dim):
-        _bad(f"{name}: expected [{n}, {heads}, {head_dim}], got {tuple(t.shape)}")
-    if t.device != device:
-        _bad(f"{name}: expected a tensor on {device}, got {t.device}")
+def _heads(name: str, t, shape, device):
+    """A tensor of `shape` [n, heads, head_dim] with contiguous columns -> strides of the first two dimensions."""
+    if t.shape != shape or t.device != device:
+        _bad(f"{name}: expected a tensor {list(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
     a, b, c = t.stride()
-    if c != 1 and head_dim > 1:
+    if c != 1 and shape[2] > 1:
         _bad(f"{name}: the columns of a head must be contiguous")
     return a, b
 
@@ -119,7 +117,7 @@ class RotaryTable:
         if out.dtype != x.dtype or out.shape != x.shape:
             _bad("out: expected x's shape and dtype")
         n, heads, hd = x.shape
-        xs, os = _heads("x", x, n, heads, hd, self.device), _heads("out", out, n, heads, hd, self.device)
+        xs, os = _heads("x", x, x.shape, self.device), _heads("out", out, x.shape, self.device)
         a = RotaryArgs(x.data_ptr(), *xs, out.data_ptr(), *os, _act("x", x), n, heads, hd,
                        _ints("positions", positions, n, self.device), *self._ptrs, int(inverse), self.device.index)
         check(lib().mxmqa_rotary(ctypes.byref(a), _stream(self.device)))
@@ -198,26 +196,27 @@ class PagedKvCache:
         queries (q_out, which may be q; None where q is None); k_out gets the turned keys too.  A written slot's
         weight becomes 0, its position the token's."""
         n, dev, hd, dtype = k.shape[0], self.device, self.head_dim, k.dtype
-        ks, vs = _heads("k", k, n, self.kv_heads, hd, dev), _heads("v", v, n, self.kv_heads, hd, dev)
+        q_shape, k_shape = (n, self.n_heads, hd), (n, self.kv_heads, hd)
+        ks, vs = _heads("k", k, k_shape, dev), _heads("v", v, k_shape, dev)
         code = _act("k", k)
         qs = os = kos = (0, 0)
         if v.dtype != dtype:
             _bad("v: expected k's dtype")
         if q is not None:
-            qs = _heads("q", q, n, self.n_heads, hd, dev)
+            qs = _heads("q", q, q_shape, dev)
             if q.dtype != dtype:
                 _bad("q: expected k's dtype")
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
                 os = (self.n_heads * hd, hd)
             else:
-                os = _heads("q_out", q_out, n, self.n_heads, hd, dev)
+                os = _heads("q_out", q_out, q_shape, dev)
                 if q_out.dtype != dtype:
                     _bad("q_out: expected q's dtype")
         elif q_out is not None:
             _bad("q_out without q")
         if k_out is not None:
-            kos = _heads("k_out", k_out, n, self.kv_heads, hd, dev)
+            kos = _heads("k_out", k_out, k_shape, dev)
             if k_out.dtype != dtype:
                 _bad("k_out: expected k's dtype")
         t, stride, n_rows, max_pages = self._tables(tables)
@@ -242,7 +241,8 @@ class PagedKvCache:
         the log of the normalizer.  Rows may share pages, except with track."""
         dev, hd, nH = self.device, self.head_dim, self.n_heads
         n = q.shape[0]
-        qs = _heads("q", q, n, nH, hd, dev)
+        shape = (n, nH, hd)
+        qs = _heads("q", q, shape, dev)
         t, stride, n_rows, max_pages = self._tables(tables)
         if n_rows != n:
             _bad(f"tables: expected {n} rows, got {n_rows}")
@@ -250,7 +250,7 @@ class PagedKvCache:
             out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
             os = (nH * hd, hd)
         else:
-            os = _heads("out", out, n, nH, hd, dev)
+            os = _heads("out", out, shape, dev)
             if out_dtype is not None and out.dtype != out_dtype:
                 _bad("out: expected out_dtype")
         if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (nH,) or sinks.device != dev

@@ -597,7 +597,7 @@ def test_refusals_with_a_device(torch):
     d = P.cache.decode
     refused(lambda: d(q[:, :7], P.tables, P.lens), "q: expected")
     refused(lambda: d(q.half(), P.tables, P.lens), "unsupported dtype")
-    refused(lambda: d(q.cpu(), P.tables, P.lens), "expected a tensor on")
+    refused(lambda: d(q.cpu(), P.tables, P.lens), "expected a tensor")
     refused(lambda: d(q, P.tables[:1], P.lens), "tables")
     refused(lambda: d(q, P.tables.long(), P.lens), "tables")
     refused(lambda: d(q, P.tables, P.lens.long()), "lens")
