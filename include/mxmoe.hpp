@@ -7,6 +7,7 @@
 //   moe::MoeGatedSwiGLU           src/moe/mod.rs:35-57 (set_resident :95-97,
 //                                 forward :99-115)
 //   loader::mxfp4::dequant_mxfp4_bytes  src/loader/mxfp4.rs:57-79 (device)
+//   attention::PagedKvCache       the paged key-value cache (mxmqa_paged_*)
 //
 // The reference panics on failure (e.g. src/moe/mod.rs:111-113); this mirror
 // throws mxmoe::Error carrying the library status and message.  Exceptions are
@@ -131,6 +132,43 @@ class MoeGatedSwiGLU {
 inline MoeGatedSwiGLU MoeConfig::init(int device) const { return MoeGatedSwiGLU(*this, device); }
 
 }  // namespace moe
+
+namespace attention {
+
+// A paged key-value cache over the caller's device memory.  Arguments are the C
+// structs; calls are stream-ordered.
+class PagedKvCache {
+ public:
+  PagedKvCache(const mxmqa_paged_config& cfg, const mxmqa_paged_buffers& buffers) {
+    check(mxmqa_paged_create(&cfg, &buffers, &cache_));
+  }
+  PagedKvCache(const PagedKvCache&) = delete;
+  PagedKvCache& operator=(const PagedKvCache&) = delete;
+  PagedKvCache(PagedKvCache&& o) noexcept : cache_(std::exchange(o.cache_, nullptr)) {}
+  ~PagedKvCache() {
+    if (cache_) mxmqa_paged_destroy(cache_);
+  }
+
+  mxmqa_paged_cache* raw() const { return cache_; }
+  void append(const mxmqa_paged_append_args& a, void* stream = nullptr) { check(mxmqa_paged_append(cache_, &a, stream)); }
+  void decode(const mxmqa_paged_decode_args& a, void* stream = nullptr) { check(mxmqa_paged_decode(cache_, &a, stream)); }
+  void evict(const mxmqa_paged_evict_args& a, void* stream = nullptr) { check(mxmqa_paged_evict(cache_, &a, stream)); }
+  // Waits for the stream; throws if a call met something out of range.
+  void sync_status(void* stream = nullptr) { check(mxmqa_paged_status(cache_, stream)); }
+
+ private:
+  mxmqa_paged_cache* cache_ = nullptr;
+};
+
+// cos and sin of positions first .. first + n - 1, device [n][rot_dim / 2].
+inline void rotary_table(const mxmqa_rotary_config& cfg, uint32_t first, uint32_t n, float* cos_dev, float* sin_dev,
+                         int device = 0, void* stream = nullptr) {
+  check(mxmqa_rotary_table(&cfg, first, n, cos_dev, sin_dev, device, stream));
+}
+
+inline void rotary(const mxmqa_rotary_args& a, void* stream = nullptr) { check(mxmqa_rotary(&a, stream)); }
+
+}  // namespace attention
 
 namespace loader {
 namespace modelbin {
