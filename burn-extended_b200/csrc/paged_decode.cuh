@@ -358,9 +358,10 @@ struct E4m3 {
     uint32_t a[HDT / 16][X ? 4 : 2];
     float back;
   };
-  static __device__ __forceinline__ uint32_t widen(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
-    return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+  // Two and two of a word's four bytes, widened.
+  static __device__ __forceinline__ void widen(uint32_t four, uint32_t& low, uint32_t& high) {
+    asm("{.reg .b16 x, y;\n mov.b32 {x, y}, %2;\n cvt.rn.f16x2.e4m3x2 %0, x;\n cvt.rn.f16x2.e4m3x2 %1, y;}"
+        : "=r"(low), "=r"(high) : "r"(four));
   }
   static __device__ __forceinline__ void load(Q& q, const float* row, int t) {
     float top = 0.0f;
@@ -406,7 +407,8 @@ struct E4m3 {
         const uint32_t l0 = X ? q.a[i][X ? 2 : 0] : 0, l1 = X ? q.a[i][X ? 3 : 0] : 0;
 #pragma unroll
         for (int j = 0; j < 2 * NT; ++j) {
-          const uint32_t w = b[e / 2][j / 2][2 * (j & 1) + (e & 1)], b0 = widen(w & 0xFFFF), b1 = widen(w >> 16);
+          uint32_t b0, b1;
+          widen(b[e / 2][j / 2][2 * (j & 1) + (e & 1)], b0, b1);
           if (i == 0 || X && i % 4 == 0)
             mma_f16_new(c[j], q.a[i][0], l0, q.a[i][1], l1, b0, b1);
           else
@@ -451,12 +453,15 @@ struct E4m3 {
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         const uint32_t* w = x.w[n][u];
-        const uint32_t y[4] = {__byte_perm(w[0], w[1], 0x5140), __byte_perm(w[0], w[1], 0x7362),
-                               __byte_perm(w[2], w[3], 0x5140), __byte_perm(w[2], w[3], 0x7362)};
+        uint32_t y[2][4];  // [keys 2t, 8 + 2t][column]: a pair of keys each
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          widen(__byte_perm(w[2 * i], w[2 * i + 1], 0x5140), y[i][0], y[i][1]);
+          widen(__byte_perm(w[2 * i], w[2 * i + 1], 0x7362), y[i][2], y[i][3]);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t a = y[e >> 1], b = y[2 + (e >> 1)];
-          const uint32_t b0 = widen(e & 1 ? a >> 16 : a & 0xFFFF), b1 = widen(e & 1 ? b >> 16 : b & 0xFFFF);
+          const uint32_t b0 = y[0][e], b1 = y[1][e];
           if constexpr (!X)
             mma_f16(o.x[4 * n + e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
           else if (u == 0)
