@@ -22,7 +22,7 @@ namespace {
 // The register arrays' head size that the kernels are built for.
 int padded_head(const PagedView& c) {
   for (const int d : {64, 80, 96, 128})
-    if (c.head_dim <= d && (d != 80 || c.dtype == MXMOE_BF16)) return d;
+    if (c.head_dim <= d && (d != 80 || c.dtype != MXMOE_E4M3)) return d;
   return 256;
 }
 

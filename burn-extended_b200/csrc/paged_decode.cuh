@@ -102,6 +102,9 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 __device__ __forceinline__ void lds128(float (&r)[4], uint32_t a) {
   asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]) : "r"(a) : "memory");
 }
+__device__ __forceinline__ void lds64(float (&r)[4], uint32_t a) {
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(r[0]), "=f"(r[1]) : "r"(a) : "memory");
+}
 
 // d += a b, and d = a b.
 #define MXMOE_MMA(name, shape)                                                                                      \
@@ -176,33 +179,34 @@ struct Queries {
   static __device__ __forceinline__ void put(uint2&, float4) {}
 };
 
-// A warp's output: pair n of lane (g, t) are two columns of head g.  In 32 bits
-// (X) each tile's products are summed apart and joined by one rounded addition:
-// the MMA's own sums are cut off, and over a long row that would show.  For a
-// bf16 output the MMA adds to the sums, the shares' second terms apart.
+// A warp's output, transposed: the MMA's rows are 16 columns of the values, its
+// columns the 8 heads, so that shares need no second row half, and a lane keeps
+// half as many sums as with heads as rows.  Of columns' group n, lane (g, t)
+// holds the two that belong to g, for heads 2t and 2t + 1; pair 2n + e is head
+// 2t + e's.  In 32 bits (X) each tile's products are summed apart and joined by
+// one rounded addition: the MMA's own sums are cut off, and over a long row that
+// would show.  For a bf16 output the MMA adds to the sums.
 template <int HDT, bool X>
 struct Output {
-  float x[HDT / 8][X ? 2 : 4];
+  float x[HDT / 16][4];
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int n = 0; n < HDT / 8; ++n)
+    for (int n = 0; n < HDT / 16; ++n)
 #pragma unroll
-      for (int e = 0; e < (X ? 2 : 4); ++e) x[n][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) x[n][e] = 0.0f;
   }
-  __device__ __forceinline__ void scale(float f) {
+  __device__ __forceinline__ void scale(float f, float g) {
 #pragma unroll
-    for (int n = 0; n < HDT / 8; ++n)
+    for (int n = 0; n < HDT / 16; ++n)
 #pragma unroll
-      for (int e = 0; e < (X ? 2 : 4); ++e) x[n][e] *= f;
+      for (int e = 0; e < 4; ++e) x[n][e] *= e & 1 ? g : f;
   }
-  __device__ __forceinline__ void fold(int n, const float (&d)[4], float f) {
-    x[n][0] = fmaf(x[n][0], f, d[0] + d[2]);
-    x[n][1] = fmaf(x[n][1], f, d[1] + d[3]);
+  __device__ __forceinline__ void add(int n, const float (&d)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[n][e] += d[e];
   }
-  __device__ __forceinline__ float2 pair(int n) const {
-    return X ? make_float2(x[n][0], x[n][1]) : make_float2(x[n][0] + x[n][X ? 0 : 2], x[n][1] + x[n][X ? 1 : 3]);
-  }
+  __device__ __forceinline__ float2 pair(int i) const { return make_float2(x[i / 2][i & 1], x[i / 2][2 + (i & 1)]); }
 };
 
 // Two scores of a lane from the two row halves of a product, or added to them:
@@ -297,8 +301,7 @@ struct Bf16 {
 #pragma unroll
       for (int u = 0; u < NT; ++u) ldm4t(x.b[n][u], value_at(v, lane) + 16 * u * rb + 32 * n);
   }
-  static __device__ __forceinline__ void add(Output<HDT, X>& o, V& x, const float (&p)[4 * NT], float corr, uint32_t v,
-                                             int lane) {
+  static __device__ __forceinline__ void add(Output<HDT, X>& o, V& x, const float (&p)[4 * NT], uint32_t v, int lane) {
     uint32_t h[2 * NT], l[2 * NT], m[2 * NT];
 #pragma unroll
     for (int j = 0; j < 2 * NT; ++j) {
@@ -317,28 +320,40 @@ struct Bf16 {
             if (n0 + n < HDT / 16) ldm4t(x.b[n][u], value_at(v, lane) + 16 * u * rb + 32 * (n0 + n));
       }
 #pragma unroll
-      for (int i = 0; i < 2 * kPre; ++i) {
-        const int n = 2 * n0 + i;
-        if (n >= HDT / 8) break;
+      for (int i = 0; i < kPre; ++i) {
+        const int n = n0 + i;
+        if (n >= HDT / 16) break;
         float d[4];
+        // the smallest terms first: what their sum cuts off is small too
+        if constexpr (X) {
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          const uint32_t b0 = x.b[i / 2][u][2 * (i & 1)], b1 = x.b[i / 2][u][2 * (i & 1) + 1];
-          if constexpr (!X)
-            mma_bf16(o.x[n], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
-          else if (u == 0)
-            mma_bf16_new(d, h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
-          else
-            mma_bf16(d, h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
-          if (X) mma_bf16(d, m[2 * u], 0, m[2 * u + 1], 0, b0, b1);
+          for (int u = 0; u < NT; ++u) {
+            const uint32_t(&a)[4] = x.b[i][u];
+            if (u == 0)
+              mma_bf16_new(d, a[0], a[2], a[1], a[3], m[0], m[1]);
+            else
+              mma_bf16(d, a[0], a[2], a[1], a[3], m[2 * u], m[2 * u + 1]);
+            mma_bf16(d, a[0], a[2], a[1], a[3], l[2 * u], l[2 * u + 1]);
+          }
+#pragma unroll
+          for (int u = 0; u < NT; ++u)
+            mma_bf16(d, x.b[i][u][0], x.b[i][u][2], x.b[i][u][1], x.b[i][u][3], h[2 * u], h[2 * u + 1]);
+          o.add(n, d);
+        } else {
+#pragma unroll
+          for (int u = 0; u < NT; ++u) {
+            const uint32_t(&a)[4] = x.b[i][u];
+            mma_bf16(o.x[n], a[0], a[2], a[1], a[3], h[2 * u], h[2 * u + 1]);
+            mma_bf16(o.x[n], a[0], a[2], a[1], a[3], l[2 * u], l[2 * u + 1]);
+          }
         }
-        if (X) o.fold(n, d, corr);
       }
     }
   }
-  // The columns of pair n: the first, and how far the second is.
-  static constexpr int kApart = 1;
-  static __device__ __forceinline__ int column(int n, int t) { return 8 * n + 2 * t; }
+  // The two columns of group n that belong to g: the first, and how far the
+  // second is.
+  static constexpr int kApart = 8;
+  static __device__ __forceinline__ int column(int n, int g) { return 16 * n + g; }
 };
 
 // 8-bit keys and values widen to f16 without loss.  A query row is scaled by a
@@ -438,8 +453,7 @@ struct E4m3 {
 #pragma unroll
         for (int e = 0; e < 4; ++e) x.w[n][u][e] = lds32(at + (16 * u + 8 * (e >> 1) + (e & 1)) * rb + 32 * n);
   }
-  static __device__ __forceinline__ void add(Output<HDT, X>& o, V& x, const float (&p)[4 * NT], float corr, uint32_t v,
-                                             int lane) {
+  static __device__ __forceinline__ void add(Output<HDT, X>& o, V& x, const float (&p)[4 * NT], uint32_t v, int lane) {
     uint32_t h[2 * NT], l[2 * NT];
 #pragma unroll
     for (int j = 0; j < 2 * NT; ++j) {
@@ -449,7 +463,7 @@ struct E4m3 {
     }
 #pragma unroll
     for (int n = 0; n < HDT / 32; ++n) {
-      float d[4][4];
+      float d[2][4];
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         const uint32_t* w = x.w[n][u];
@@ -460,24 +474,27 @@ struct E4m3 {
           widen(__byte_perm(w[2 * i], w[2 * i + 1], 0x7362), y[i][2], y[i][3]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t b0 = y[0][e], b1 = y[1][e];
-          if constexpr (!X)
-            mma_f16(o.x[4 * n + e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
-          else if (u == 0)
-            mma_f16_new(d[e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
-          else
-            mma_f16(d[e], h[2 * u], l[2 * u], h[2 * u + 1], l[2 * u + 1], b0, b1);
+        for (int e = 0; e < 2; ++e) {
+          if constexpr (X) {
+            if (u == 0)
+              mma_f16_new(d[e], y[0][2 * e], y[0][2 * e + 1], y[1][2 * e], y[1][2 * e + 1], l[0], l[1]);
+            else
+              mma_f16(d[e], y[0][2 * e], y[0][2 * e + 1], y[1][2 * e], y[1][2 * e + 1], l[2 * u], l[2 * u + 1]);
+            mma_f16(d[e], y[0][2 * e], y[0][2 * e + 1], y[1][2 * e], y[1][2 * e + 1], h[2 * u], h[2 * u + 1]);
+          } else {
+            mma_f16(o.x[2 * n + e], y[0][2 * e], y[0][2 * e + 1], y[1][2 * e], y[1][2 * e + 1], h[2 * u], h[2 * u + 1]);
+            mma_f16(o.x[2 * n + e], y[0][2 * e], y[0][2 * e + 1], y[1][2 * e], y[1][2 * e + 1], l[2 * u], l[2 * u + 1]);
+          }
         }
       }
-      if (X) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o.fold(4 * n + e, d[e], corr);
+      if constexpr (X) {
+        o.add(2 * n, d[0]);
+        o.add(2 * n + 1, d[1]);
       }
     }
   }
-  static constexpr int kApart = 4;
-  static __device__ __forceinline__ int column(int n, int t) { return 32 * (n / 4) + 8 * t + n % 4; }
+  static constexpr int kApart = 1;
+  static __device__ __forceinline__ int column(int n, int g) { return 32 * (n / 2) + 4 * g + 2 * (n % 2); }
 };
 
 // 32-bit keys and values as two tf32 terms each, cut off so that the second is
@@ -530,33 +547,45 @@ struct F32 {
   }
   struct V {};
   static __device__ __forceinline__ void load(V&, uint32_t, int) {}
-  static __device__ __forceinline__ void add(Output<HDT, X>& o, V&, const float (&p)[4 * NT], float corr, uint32_t v, int lane) {
+  static __device__ __forceinline__ void add(Output<HDT, X>& o, V&, const float (&p)[4 * NT], uint32_t v, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t at = v + 2 * t * rb + 16 * g;
+    const uint32_t at = v + 2 * t * rb;
 #pragma unroll
-    for (int n = 0; n < HDT / 8; n += 4) {
-      float d[4][4];
+    for (int n = 0; n < HDT / 16; n += 2) {
+      const bool both = n + 1 < HDT / 16;  // 32 columns, four a lane, or the last 16, two a lane
+      float d[2][4];
 #pragma unroll
       for (int u = 0; u < 2 * NT; ++u) {  // keys 8u to 8u + 7
         float w[2][4];
-        lds128(w[0], at + 8 * u * rb + 32 * n);
-        lds128(w[1], at + (8 * u + 1) * rb + 32 * n);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (both)
+            lds128(w[i], at + 16 * g + (8 * u + i) * rb + 64 * n);
+          else
+            lds64(w[i], at + 8 * g + (8 * u + i) * rb + 64 * n);
+        }
         const float p0 = p[2 * u], p1 = p[2 * u + 1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2; ++e) {
+          if (e == 1 && !both) break;
+          const float a0 = w[0][2 * e], a1 = w[0][2 * e + 1], a2 = w[1][2 * e], a3 = w[1][2 * e + 1];
           if (u == 0)
-            mma_tf32_new(d[e], top(p0), rest(p0), top(p1), rest(p1), top(w[0][e]), top(w[1][e]));
+            mma_tf32_new(d[e], rest(a0), rest(a1), rest(a2), rest(a3), rest(p0), rest(p1));
           else
-            mma_tf32(d[e], top(p0), rest(p0), top(p1), rest(p1), top(w[0][e]), top(w[1][e]));
-          mma_tf32(d[e], top(p0), rest(p0), top(p1), rest(p1), rest(w[0][e]), rest(w[1][e]));
+            mma_tf32(d[e], rest(a0), rest(a1), rest(a2), rest(a3), rest(p0), rest(p1));
+          mma_tf32(d[e], rest(a0), rest(a1), rest(a2), rest(a3), top(p0), top(p1));
+          mma_tf32(d[e], top(a0), top(a1), top(a2), top(a3), rest(p0), rest(p1));
+          mma_tf32(d[e], top(a0), top(a1), top(a2), top(a3), top(p0), top(p1));
         }
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o.fold(n + e, d[e], corr);
+      o.add(n, d[0]);
+      if (both) o.add(n + 1, d[1]);
     }
   }
-  static constexpr int kApart = 4;
-  static __device__ __forceinline__ int column(int n, int t) { return 32 * (n / 4) + 8 * t + n % 4; }
+  static constexpr int kApart = 1;
+  static __device__ __forceinline__ int column(int n, int g) {
+    return 32 * (n / 2) + (n + 1 < HDT / 16 || n % 2 ? 4 * g + 2 * (n % 2) : 2 * g);
+  }
 };
 
 // ---- the list of tiles ----
@@ -733,7 +762,7 @@ struct Cut {
   }
 };
 
-// Two finished columns of a head; `apart` is 1 or 4.
+// Two finished columns of a head.
 template <int kApart>
 __device__ __forceinline__ void store_out(const DecodeParams& p, int row, int h, int col, float x, float y) {
   const int64_t o = row * p.out_row + h * p.out_head + col;
@@ -1044,9 +1073,9 @@ if (all) {
           sum += w[i];
         }
         l = fmaf(l, corr, sum);
-        if (!C::kWide && __any_sync(0xFFFFFFFFu, top != m)) o.scale(corr);
+        if (__any_sync(0xFFFFFFFFu, top != m)) o.scale(__shfl_sync(0xFFFFFFFFu, corr, 8 * t), __shfl_sync(0xFFFFFFFFu, corr, 8 * t + 4));
         m = top;
-        C::add(o, values, w, corr, v, lane);
+        C::add(o, values, w, v, lane);
         __syncwarp();
         if (++stage == kStages) stage = 0;
         j += wg;
@@ -1066,7 +1095,7 @@ if (all) {
     }
     // The group's warps join in shared memory, each in the stage that it loads
     // next: nothing uses that until then.
-    const int heads = min(kDecodeHeads, G - part * kDecodeHeads), h = kvh * G + part * kDecodeHeads + g;
+    const int heads = min(kDecodeHeads, G - part * kDecodeHeads), h0 = kvh * G + part * kDecodeHeads;
     float2* mo = reinterpret_cast<float2*>(mine + ld_stage * kStageBytes);
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) mo[32 * i + lane] = o.pair(i);
@@ -1076,38 +1105,43 @@ if (all) {
     }
     if (lane == 0) join_at[warp] = (warp * kStages + ld_stage) * kStageBytes;
     group_sync();
-    // nt is a multiple of 32: a thread's head is its lane's for every pair
+    // a lane weighs head lane % 8, and asks others for those of its pairs
+    const int mine_h = lane % kDecodeHeads;
+    const float its_sink = __shfl_sync(0xFFFFFFFFu, sink, 4 * mine_h);
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < W; ++w)
-      if (w < wg) top = fmaxf(top, join_ml[w0 + w][g][0]);
+      if (w < wg) top = fmaxf(top, join_ml[w0 + w][mine_h][0]);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       if (w >= wg) break;
-      sum = fmaf(join_ml[w0 + w][g][1], exp_diff(join_ml[w0 + w][g][0], top), sum);
+      sum = fmaf(join_ml[w0 + w][mine_h][1], exp_diff(join_ml[w0 + w][mine_h][0], top), sum);
     }
     float f = 1.0f;
     if (to) {
-      if (t == 0 && tid < 32) to[32 * kPairs + g] = make_float2(top, sum);
-    } else if (g < heads) {
-      const float2 y = finish(sink, p.quiet, top, sum);
+      if (tid < kDecodeHeads) to[32 * kPairs + tid] = make_float2(top, sum);
+    } else if (mine_h < heads) {
+      const float2 y = finish(its_sink, p.quiet, top, sum);
       f = y.x * (p.c.v_scale ? p.c.v_scale[kvh] : 1.0f);
-      if (t == 0 && tid < 32) store_lse(p, ws, row, h, y.y);
+      if (tid < kDecodeHeads) store_lse(p, ws, row, h0 + mine_h, y.y);
     }
+    __syncwarp();
 #pragma unroll 1
     for (int i = tid; i < 32 * kPairs; i += nt) {
+      const int head = 2 * t + (i / 32 & 1);
+      const float its_top = __shfl_sync(0xFFFFFFFFu, top, head), its_f = __shfl_sync(0xFFFFFFFFu, f, head);
       float a = 0.0f, b = 0.0f;
 #pragma unroll 4
       for (int w = w0; w < w0 + wg; ++w) {
-        const float e = exp_diff(join_ml[w][g][0], top);
+        const float e = exp_diff(join_ml[w][head][0], its_top);
         const float2 y = reinterpret_cast<const float2*>(ring + join_at[w])[i];
         a = fmaf(y.x, e, a);
         b = fmaf(y.y, e, b);
       }
       if (to)
         to[i] = make_float2(a, b);
-      else if (g < heads)
-        store_out<C::kApart>(p, row, h, C::column(i / 32, t), a * f, b * f);
+      else if (head < heads)
+        store_out<C::kApart>(p, row, h0 + head, C::column(i / 64, g), a * its_f, b * its_f);
     }
     group_sync();  // the stages are free again
   }
@@ -1124,7 +1158,7 @@ if (all) {
 // parts are in flight at once.
 template <class C, int HDT>
 __global__ void __launch_bounds__(256) join_kernel(const DecodeParams p, const DecodeScratch ws) {
-  constexpr int kPairs = HDT / 8, kSlice = kPairs % 4 ? 5 : 4, kPartPairs = 32 * kPairs + kDecodeHeads, kAtOnce = 4;
+  constexpr int kPairs = HDT / 8, kSlice = kPairs % 4 ? 2 : 4, kPartPairs = 32 * kPairs + kDecodeHeads, kAtOnce = 4;
   static_assert(kPairs % kSlice == 0, "slices cover the columns");
   __shared__ float2 outs[8][32 * kSlice], ml[8][kDecodeHeads];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, p0 = blockIdx.y * kSlice;
@@ -1137,59 +1171,66 @@ __global__ void __launch_bounds__(256) join_kernel(const DecodeParams p, const D
     const int row = s / segs, kvh = (s - row * segs) / parts, part = s - row * segs - kvh * parts;
     const int first = held.x, last = held.y;
     if (first == last) continue;
-    float m = -INFINITY, l = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {};  // of heads 2t and 2t + 1
     float2 o[kSlice];
 #pragma unroll
     for (int i = 0; i < kSlice; ++i) o[i] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
     for (int w = first + warp; w <= last; w += 8 * kAtOnce) {
-      float2 y[kAtOnce], z[kAtOnce][kSlice];
+      float4 y[kAtOnce];
+      float2 z[kAtOnce][kSlice];
 #pragma unroll
       for (int j = 0; j < kAtOnce; ++j) {
         const int v = w + 8 * j;
-        y[j] = make_float2(-INFINITY, 0.0f);
+        y[j] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
 #pragma unroll
         for (int i = 0; i < kSlice; ++i) z[j][i] = make_float2(0.0f, 0.0f);
         if (v > last) continue;
         const float2* from = reinterpret_cast<const float2*>(ws.part) + (2 * v + (v == first ? 1 : 0)) * kPartPairs;
-        y[j] = __ldcg(from + 32 * kPairs + g);
+        y[j] = __ldcg(reinterpret_cast<const float4*>(from + 32 * kPairs) + t);
 #pragma unroll
         for (int i = 0; i < kSlice; ++i) z[j][i] = __ldcg(from + 32 * (p0 + i) + lane);
       }
 #pragma unroll
       for (int j = 0; j < kAtOnce; ++j) {
-        const float top = fmaxf(m, y[j].x), a = exp_diff(m, top), b = exp_diff(y[j].x, top);
-        m = top;
-        l = l * a + y[j].y * b;
+        float a[2], b[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float ym = e ? y[j].z : y[j].x, top = fmaxf(m[e], ym);
+          a[e] = exp_diff(m[e], top);
+          b[e] = exp_diff(ym, top);
+          m[e] = top;
+          l[e] = l[e] * a[e] + (e ? y[j].w : y[j].y) * b[e];
+        }
 #pragma unroll
         for (int i = 0; i < kSlice; ++i) {
-          o[i].x = fmaf(z[j][i].x, b, o[i].x * a);
-          o[i].y = fmaf(z[j][i].y, b, o[i].y * a);
+          o[i].x = fmaf(z[j][i].x, b[i & 1], o[i].x * a[i & 1]);
+          o[i].y = fmaf(z[j][i].y, b[i & 1], o[i].y * a[i & 1]);
         }
       }
     }
     __syncthreads();  // the segment before is read out
 #pragma unroll
     for (int i = 0; i < kSlice; ++i) outs[warp][32 * i + lane] = o[i];
-    if (t == 0) ml[warp][g] = make_float2(m, l);
+    if (g < 2) ml[warp][2 * t + g] = make_float2(g ? m[1] : m[0], g ? l[1] : l[0]);
     __syncthreads();
-    const int used = min(8, last - first + 1), h = kvh * G + part * kDecodeHeads + g;
-    if (warp >= kSlice || part * kDecodeHeads + g >= G) continue;
+    const int used = min(8, last - first + 1), head = 2 * t + (warp & 1), h = kvh * G + part * kDecodeHeads + head;
+    if (warp >= kSlice || part * kDecodeHeads + head >= G) continue;
     float top = -INFINITY, sum = 0.0f, a = 0.0f, b = 0.0f;
-    for (int w = 0; w < used; ++w) top = fmaxf(top, ml[w][g].x);
+    for (int w = 0; w < used; ++w) top = fmaxf(top, ml[w][head].x);
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
       if (w >= used) break;
-      const float e = exp_diff(ml[w][g].x, top);
+      const float e = exp_diff(ml[w][head].x, top);
       const float2 y = outs[w][32 * warp + lane];
-      sum = fmaf(ml[w][g].y, e, sum);
+      sum = fmaf(ml[w][head].y, e, sum);
       a = fmaf(y.x, e, a);
       b = fmaf(y.y, e, b);
     }
     const float2 f = finish(p.sinks ? p.sinks[h] : -INFINITY, p.quiet, top, sum);
     const float by = f.x * (p.c.v_scale ? p.c.v_scale[kvh] : 1.0f);
-    if (p0 + warp == 0 && t == 0) store_lse(p, ws, row, h, f.y);
-    store_out<C::kApart>(p, row, h, C::column(p0 + warp, t), a * by, b * by);
+    if (p0 == 0 && warp < 2 && g == 0) store_lse(p, ws, row, h, f.y);
+    store_out<C::kApart>(p, row, h, C::column((p0 + warp) / 2, g), a * by, b * by);
   }
 }
 
@@ -1204,7 +1245,7 @@ cudaError_t launch(const DecodeParams& p, const DecodeScratch& ws, const DecodeP
   e = launch_kernel(fn, dim3(plan.grid), dim3(32 * C::kWarps), smem, st, p, ws, plan);
   if (e != cudaSuccess || plan.whole) return e;
   const int G = p.c.n_heads / p.c.kv_heads, n_segs = p.rows * p.c.kv_heads * ((G + kDecodeHeads - 1) / kDecodeHeads);
-  constexpr int slices = HDT / 8 % 4 ? HDT / 40 : HDT / 32;
+  constexpr int slices = HDT / 8 % 4 ? HDT / 16 : HDT / 32;
   return launch_kernel(join_kernel<C, HDT>, dim3(n_segs < 4 * plan.grid ? n_segs : 4 * plan.grid, slices), dim3(256), 0, st, p,
                        ws);
 }
