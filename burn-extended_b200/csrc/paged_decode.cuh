@@ -83,6 +83,9 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -791,6 +794,10 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   __shared__ int join_at[kDecodeWarps], queue[kDecodeWarps][8];
   __shared__ float join_ml[kDecodeWarps][kDecodeHeads][2];
   __shared__ uint32_t there[kDecodeWarps][kDecodeMaxStages];  // which keys of a stage are in the cache
+  // The tiles after the loaded ones: first key, keys left, key head (-1: no
+  // tile), and each lane's page number.
+  __shared__ int4 ahead[C::kWarps][C::kStages - 1];
+  __shared__ int page_at[C::kWarps][C::kStages - 1][32];
   const Rows rows{before, len_of};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int hd = p.c.head_dim, H = p.c.kv_heads, G = p.c.n_heads / H;
@@ -804,22 +811,26 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   list_rows(p, rows, kTile);
   const int total = before[p.rows] * segs, n_segs = p.rows * segs;
 
-  // Rows without keys: zeros.
+  auto idle_rows = [&]() {  // rows without keys: zeros
 #pragma unroll 1
-  for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    if (before[r + 1] != before[r]) continue;
+    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+      if (before[r + 1] != before[r]) continue;
 #pragma unroll 1
-    for (int i = threadIdx.x; i < p.c.n_heads * hd; i += blockDim.x) {
-      const int h = i / hd;
-      const int64_t o = r * p.out_row + h * p.out_head + (i - h * hd);
-      if (p.out_dtype == MXMOE_F32)
-        static_cast<float*>(p.out)[o] = 0.0f;
-      else
-        static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(0.0f);
-      if (i == h * hd) store_lse(p, ws, r, h, finish(p.sinks ? p.sinks[h] : -INFINITY, p.quiet, -INFINITY, 0.0f).y);
+      for (int i = threadIdx.x; i < p.c.n_heads * hd; i += blockDim.x) {
+        const int h = i / hd;
+        const int64_t o = r * p.out_row + h * p.out_head + (i - h * hd);
+        if (p.out_dtype == MXMOE_F32)
+          static_cast<float*>(p.out)[o] = 0.0f;
+        else
+          static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(0.0f);
+      }
+#pragma unroll 1
+      for (int h = threadIdx.x; h < p.c.n_heads; h += blockDim.x)
+        store_lse(p, ws, r, h, finish(p.sinks ? p.sinks[h] : -INFINITY, p.quiet, -INFINITY, 0.0f).y);
     }
-  }
+  };
   if (total == 0) {
+    idle_rows();
 #pragma unroll 1
     for (int s = blockIdx.x + gridDim.x * threadIdx.x; s < n_segs && !plan.whole; s += gridDim.x * blockDim.x)
       ws.held[s] = make_int2(0, 0);
@@ -828,18 +839,9 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
 
   const Cut cut(rows, p.rows, segs, total, W * gridDim.x, W, plan.whole);
   const int wg = cut.wg, group = warp / wg, in_group = warp - group * wg, w0 = group * wg, tid = threadIdx.x - w0 * 32, nt = 32 * wg;
-  if (!plan.whole) {
-    // For join_kernel: the first and last range of every segment.
-#pragma unroll 1
-    for (int s = blockIdx.x + gridDim.x * threadIdx.x; s < n_segs; s += gridDim.x * blockDim.x) {
-      const int r = s / segs, tiles = before[r + 1] - before[r], y = before[r] * segs + (s - r * segs) * tiles;
-      ws.held[s] = tiles == 0 ? make_int2(0, 0) : make_int2(cut.range_of(y), cut.range_of(y + tiles - 1));
-    }
-  }
   const int worker = group * gridDim.x + blockIdx.x;
-  if (worker >= cut.n_workers) return;
   int range = cut.whole ? cut.filled(worker) : worker;
-  if (range >= cut.n_ranges) return;
+  const bool works = worker < cut.n_workers && range < cut.n_ranges;
   auto group_sync = [&]() {
     if (wg == 1)
       __syncwarp();
@@ -847,13 +849,9 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * wg) : "memory");
   };
 
-  // The tiles that this warp loads next: each lane's row of the pools for the
-  // tile's key of that number, two tiles ahead of its use, as the page table's
-  // answer takes that long.
-  Place ld;
-  int x = cut.begin_of(range), end = cut.end_of(range), ld_left = end - x, ld_off = in_group, ld_stage = 0;
-  ld.find(p, rows, parts, x);
-  Place at = ld;
+  // The place of the next tile that this warp looks at.
+  Place ld, at;
+  int x = 0, end = 0, ld_left = 0, ld_off = in_group, ld_stage = 0, turn = 0;
   // The next segment's queries and its heads' sinks.
   Queries<HDT, C::kWide> queries;
   float sink_next = -INFINITY;
@@ -862,36 +860,77 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
     queries.load(p, of.row * p.q_row + h0 * p.q_head, heads, lane);
     if (p.sinks && g < heads) sink_next = p.sinks[h0 + g];
   };
-  fetch(at);
-  struct Ahead {
-    int page, slot, kvh;  // kvh -1: no tile; page -1: no key, -2: out of range
-  };
-  Ahead next{-1, 0, -1}, after{-1, 0, -1};
-  int prime = kStages + 1;  // loads before the first tile: two that only look ahead, then all stages but one
   // Ranges taken after the first.  One that was kept back is asked for when the
   // one before it begins to be loaded, and waits in `queue` for its use; each
-  // has two tiles at least, so no more than eight are between the two.
+  // has two tiles at least but the list's last, and the load side is no more than
+  // ten tiles ahead, so no more than eight are between the two.
   int ld_range = range, asked = 0, queued = 0, used = 0;
   bool last_piece = false, fetched = false;  // of the range in use; the next one's queries are on their way
   auto ask = [&]() {
     if (cut.kept > 0 && lane == 0) asked = cut.n_workers + atomicAdd(ws.taken, 1);
   };
-  ask();
-  // Loads the next tile into the stage that is free, and looks two further.
   constexpr int kPieces = HDT * C::kElem / 16;  // of a key's row, 16 bytes each; zeros past head_dim
   constexpr int kLanes = kPieces % 8 == 0 ? 8 : 4, kKeys = 32 / kLanes;
   const int piece = lane % kLanes * 16;
   const uint8_t* const k_piece = static_cast<const uint8_t*>(p.c.k) + piece;
   const int64_t v_apart = static_cast<const uint8_t*>(p.c.v) - static_cast<const uint8_t*>(p.c.k);
+  // Looks at the next tile: its place into `ahead`, its keys' page numbers on
+  // their way to `page_at`, in the group of copies that is open.  Under a full
+  // memory pipe the answer takes as long as the tiles before it in the pipe, so a
+  // number that travels with one tile's keys is there when that tile is used and
+  // the one kStages - 1 further is loaded.
+  auto look = [&]() {
+    int n = min(ld.tiles - ld.tile, ld_left);
+#pragma unroll 1
+    while (ld_off >= n && ld_left > 0) {
+      ld_left -= n;
+      ld_off = in_group;
+      if (ld_left > 0) {
+        ld.next_segment(p, rows, parts);
+      } else if (cut.whole || cut.kept > 0) {
+        ld_range = cut.whole ? cut.filled(ld_range + cut.n_workers) : __shfl_sync(0xFFFFFFFFu, asked, 0);
+        if (cut.kept > 0 && lane == 0) queue[warp][queued & 7] = ld_range;
+        ++queued;
+        if (ld_range < cut.n_ranges) {
+          const int y = cut.begin_of(ld_range);
+          ld_left = cut.end_of(ld_range) - y;
+          ld.find(p, rows, parts, y);
+          ask();
+          if (cut.kept > 0 && last_piece && !fetched && queued - 1 == used) {  // it is the next one
+            fetch(ld);
+            fetched = true;
+          }
+        }
+      }
+      n = min(ld.tiles - ld.tile, ld_left);
+    }
+    int4 a = make_int4(0, 0, -1, 0);
+    if (ld_left > 0) {
+      a.x = ld.lo + (ld.tile + ld_off) * kTile;
+      a.y = ld.len - a.x;
+      a.z = ld.kvh;
+      ld_off += wg;
+      if (lane % kTile < a.y)
+        cp4(smem_u32(&page_at[warp][turn][lane]), p.t.tables + ld.row * p.t.stride + page_of(p.c, a.x + lane % kTile));
+    }
+    if (lane == 0) ahead[warp][turn] = a;
+    if (++turn == kStages - 1) turn = 0;
+  };
+  // Loads the tile that was looked at kStages - 1 looks before into the stage
+  // that is free, and looks at another.
   auto load_tile = [&]() {
-    if (next.kvh >= 0) {
-      if (next.page == -2) atomicOr(p.c.status, kPagedBadPage);
-      const uint32_t keys = __ballot_sync(0xFFFFFFFFu, next.page >= 0);
+    const int4 a = ahead[warp][turn];
+    if (a.z >= 0) {
+      const int key0 = a.x + lane % kTile;
+      const bool in = lane % kTile < a.y;
+      const int page = in ? page_at[warp][turn][lane] : -1;
+      const bool good = in && page >= 0 && page < p.c.n_pages;
+      if (in && !good) atomicOr(p.c.status, kPagedBadPage);
+      const uint32_t keys = __ballot_sync(0xFFFFFFFFu, good);
       if (lane == 0) there[warp][ld_stage] = keys;
-      const int row = next.page < 0 ? -1 : (next.page * H + next.kvh) * p.c.page_size + next.slot;
+      const int row = good ? (page * H + a.z) * p.c.page_size + key0 - page_of(p.c, key0) * p.c.page_size : -1;
       const uint32_t ks = smem_u32(mine) + ld_stage * kStageBytes, vs = ks + kTile * rb;
-      const bool all = keys == kAllKeys && kPieces * 16 == hd * C::kElem;
-if (all) {
+      if (keys == kAllKeys && kPieces * 16 == hd * C::kElem) {
 #pragma unroll
         for (int i = 0; i < kTile / kKeys; ++i) {
           const int key = i * kKeys + lane / kLanes;
@@ -922,47 +961,39 @@ if (all) {
         }
       }
     }
-    if (prime < kStages) {
-      cp_commit();
-      if (++ld_stage == kStages) ld_stage = 0;
-    }
-    next = after;
-    after.kvh = -1;
-    int n = min(ld.tiles - ld.tile, ld_left);
-#pragma unroll 1
-    while (ld_off >= n && ld_left > 0) {
-      ld_left -= n;
-      ld_off = in_group;
-      if (ld_left > 0) {
-        ld.next_segment(p, rows, parts);
-      } else if (cut.whole || cut.kept > 0) {
-        ld_range = cut.whole ? cut.filled(ld_range + cut.n_workers) : __shfl_sync(0xFFFFFFFFu, asked, 0);
-        if (cut.kept > 0 && lane == 0) queue[warp][queued & 7] = ld_range;
-        ++queued;
-        if (ld_range < cut.n_ranges) {
-          const int y = cut.begin_of(ld_range);
-          ld_left = cut.end_of(ld_range) - y;
-          ld.find(p, rows, parts, y);
-          ask();
-          if (cut.kept > 0 && last_piece && !fetched && queued - 1 == used) {  // it is the next one
-            fetch(ld);
-            fetched = true;
-          }
-        }
-      }
-      n = min(ld.tiles - ld.tile, ld_left);
-    }
-    if (ld_left <= 0) return;
-    const int key = ld.lo + (ld.tile + ld_off) * kTile + lane % kTile;
-    ld_off += wg;
-    after = Ahead{-1, 0, ld.kvh};
-    if (key < ld.len) {
-      const int pi = page_of(p.c, key);
-      after.slot = key - pi * p.c.page_size;
-      after.page = __ldg(p.t.tables + ld.row * p.t.stride + pi);
-      if (after.page < 0 || after.page >= p.c.n_pages) after.page = -2;
-    }
+    __syncwarp();  // `ahead` has been read
+    look();
+    cp_commit();
+    if (++ld_stage == kStages) ld_stage = 0;
   };
+
+  // The first tiles and queries are on their way before anything else is done.
+  if (works) {
+    x = cut.begin_of(range);
+    end = cut.end_of(range);
+    ld_left = end - x;
+    ld.find(p, rows, parts, x);
+    at = ld;
+    ask();
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) look();
+    cp_commit();
+    fetch(at);
+    cp_wait<0>();
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) load_tile();
+  }
+  idle_rows();
+  if (!plan.whole) {
+    // For join_kernel: the first and last range of every segment.
+#pragma unroll 1
+    for (int s = blockIdx.x + gridDim.x * threadIdx.x; s < n_segs; s += gridDim.x * blockDim.x) {
+      const int r = s / segs, tiles = before[r + 1] - before[r], y = before[r] * segs + (s - r * segs) * tiles;
+      ws.held[s] = tiles == 0 ? make_int2(0, 0) : make_int2(cut.range_of(y), cut.range_of(y + tiles - 1));
+    }
+  }
+  if (!works) return;
 
   constexpr int kPartPairs = 32 * kPairs + kDecodeHeads;  // [pairs][lane] of o, then (m, l) by head
   float2* const part_of = reinterpret_cast<float2*>(ws.part);
@@ -1024,16 +1055,10 @@ if (all) {
         }
       }
 #pragma unroll 1
-      for (int j = in_group; j < n;) {
-        if (prime == 0) {
-          cp_wait<kStages - 2>();
-          __syncwarp();
-        }
+      for (int j = in_group; j < n; j += wg) {
+        cp_wait<kStages - 2>();
+        __syncwarp();
         load_tile();
-        if (prime > 0) {
-          --prime;
-          continue;
-        }
         const uint32_t k = smem_u32(mine) + stage * kStageBytes, v = k + kTile * rb;
         float s[4 * NT], w[4 * NT];
         C::scores(s, q, k, lane);
@@ -1078,10 +1103,9 @@ if (all) {
         C::add(o, values, w, v, lane);
         __syncwarp();
         if (++stage == kStages) stage = 0;
-        j += wg;
       }
       m *= unit;
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+      l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
       l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
       x += n;
       if (x < end) at.next_segment(p, rows, parts);
