@@ -40,21 +40,25 @@ __global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const 
   const decode::Rows rows{before, len_of};
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int H = p.c.kv_heads, G = p.c.n_heads / H, hgroups = (G + kDecodeHeads - 1) / kDecodeHeads;
-  griddep_wait();
-  griddep_launch_dependents();
+  // This kernel starts when every block of the one before it has seen the end of
+  // the work before that: lengths, tables and weights are ready.  Only the
+  // normalizers, and the scores where no join came between, have to be waited
+  // for, once the first slots and weights are on their way.
   decode::list_rows(p, rows, 16 * NT);
   const int total = before[p.rows] * H, step = gridDim.x * (blockDim.x / 32);
+  bool waited = false;
   for (int x = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); x < total; x += step) {
     decode::Place at;
     at.find(p, rows, 1, x);
     const int first = (before[at.row] * H + at.kvh * at.tiles) * hgroups + at.tile;
-    // The slot of the key that lane (g, t) will add to, and its weight, are on
-    // their way while the shares are computed.
+    // The slot of the key that lane (g, t) will add to, and its weight.
     const int n = at.lo + at.tile * 16 * NT + 8 * (g >> 1) + 2 * t + (g & 1);
     int64_t slot = -1;
     if (g < 4 * NT && n < at.len) slot = slot_of(p.c, p.t, at.row, n);
     float* const weight = p.c.weight + slot + static_cast<int64_t>(at.kvh) * p.c.page_size;
     const float old = slot >= 0 ? *weight : 0.0f;
+    if (!waited) griddep_wait();
+    waited = true;
     float w[4 * NT] = {};
     for (int hg = 0; hg < hgroups; ++hg) {
       const int h = hg * kDecodeHeads + g;
@@ -80,6 +84,8 @@ __global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const 
     for (int i = 1; i < 4 * NT; ++i) add = g == i ? w[i] : add;
     if (slot >= 0) *weight = old + add;
   }
+  if (!waited) griddep_wait();
+  griddep_launch_dependents();
 }
 
 }  // namespace
