@@ -1178,12 +1178,12 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
 }
 
 // The segments that several ranges hold: a block joins a slice of the columns
-// of one, its warps every eighth part, in the ranges' order; the loads of four
-// parts are in flight at once.
-template <class C, int HDT>
+// of one, its warps every eighth part, in the ranges' order; the loads of
+// kAtOnce parts are in flight at once.
+template <class C, int HDT, int kSlice, int kAtOnce>
 __global__ void __launch_bounds__(256) join_kernel(const DecodeParams p, const DecodeScratch ws) {
-  constexpr int kPairs = HDT / 8, kSlice = kPairs % 4 ? 2 : 4, kPartPairs = 32 * kPairs + kDecodeHeads, kAtOnce = 4;
-  static_assert(kPairs % kSlice == 0, "slices cover the columns");
+  constexpr int kPairs = HDT / 8, kPartPairs = 32 * kPairs + kDecodeHeads;
+  static_assert(kPairs % kSlice == 0 && kSlice <= 8, "slices cover the columns");
   __shared__ float2 outs[8][32 * kSlice], ml[8][kDecodeHeads];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, p0 = blockIdx.y * kSlice;
   const int H = p.c.kv_heads, G = p.c.n_heads / H, parts = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * parts;
@@ -1269,9 +1269,16 @@ cudaError_t launch(const DecodeParams& p, const DecodeScratch& ws, const DecodeP
   e = launch_kernel(fn, dim3(plan.grid), dim3(32 * C::kWarps), smem, st, p, ws, plan);
   if (e != cudaSuccess || plan.whole) return e;
   const int G = p.c.n_heads / p.c.kv_heads, n_segs = p.rows * p.c.kv_heads * ((G + kDecodeHeads - 1) / kDecodeHeads);
-  constexpr int slices = HDT / 8 % 4 ? HDT / 16 : HDT / 32;
-  return launch_kernel(join_kernel<C, HDT>, dim3(n_segs < 4 * plan.grid ? n_segs : 4 * plan.grid, slices), dim3(256), 0, st, p,
-                       ws);
+  // Few segments are long ones: narrow slices, so that their parts are read by
+  // more blocks, eight at once (2 of 50001 tokens 26.8 us in all against 27.8).
+  // Many would not all be resident that way (512 of 8192 tokens 196 us against
+  // 186); fewer parts at once than four are slower where a segment has 20 and
+  // more (64 of 2K to 16K tokens in 8 bits 47 us against 44).
+  constexpr int kWide = HDT / 8 % 4 ? 2 : 4;
+  if (n_segs * HDT / 16 <= 2 * plan.grid)
+    return launch_kernel(join_kernel<C, HDT, 2, 8>, dim3(n_segs, HDT / 16), dim3(256), 0, st, p, ws);
+  return launch_kernel(join_kernel<C, HDT, kWide, 4>, dim3(n_segs < 4 * plan.grid ? n_segs : 4 * plan.grid, HDT / 8 / kWide), dim3(256),
+                       0, st, p, ws);
 }
 
 }  // namespace decode
