@@ -168,54 +168,55 @@ struct Unit {
   }
 };
 
-// One block per token; everything moves in 16-byte pieces.  A thread keeps one
-// unit of columns for every `per_pass`-th query head, so the token's cosines are
-// read once per thread; then the keys' units and the values' pieces are shared
-// out over the block.  The loads of up to kBatch query heads, a key unit and a
-// value piece are in flight while the token's index, page and cosines come.
-// Memory-bound: each value is read and written once.
+// Everything moves in 16-byte pieces, each read and written once: bound by
+// memory, and by latency where tokens are few.  A thread keeps one unit of
+// columns for every `per_pass`-th query head, so the token's cosines are read
+// once per thread; then the keys' units and the values' pieces are shared out
+// over the block.  The loads of up to kBatch query heads, a key unit and a value
+// piece are in flight while the token's place and cosines come.
 constexpr int kBatch = 2;
-template <typename T, bool kInterleaved, bool kMany>
-__global__ void __launch_bounds__(kMany ? 128 : 512, kMany ? 7 : 1) append_wide_kernel(const AppendParams p, int units, int per_pass) {
+constexpr int kAtOnce = 16;     // tokens whose places a block of many looks up together
+constexpr int kManyBlocks = 5;  // such blocks on one SM
+// Token t; place_of() is its Token, asked for once the loads are on their way.
+template <typename T, bool kInterleaved, class PlaceOf>
+__device__ __forceinline__ void append_token(const AppendParams& p, int units, int per_pass, int t, PlaceOf place_of) {
   constexpr int N = Piece<T>::kN;
-  griddep_wait();
-  griddep_launch_dependents();
-  const int t = blockIdx.x, hd = p.c.head_dim, half = p.rot / 2, nt = blockDim.x, tid = threadIdx.x;
+  const int hd = p.c.head_dim, half = p.rot / 2, nt = blockDim.x, tid = threadIdx.x;
   const int nH = p.q ? p.c.n_heads : 0, H = p.k ? p.c.kv_heads : 0;
   const int first = tid / units, unit = tid - first * units;
   const bool turns = unit * N < (kInterleaved ? p.rot : half), two = !kInterleaved && turns;
   const int ca = kInterleaved || turns ? unit * N : half + unit * N;
-  const T* q = static_cast<const T*>(p.q) + t * p.q_token + first * p.q_head + ca;
-  T* q_out = static_cast<T*>(p.q_out) + t * p.qo_token + first * p.qo_head + ca;
   const int64_t q_step = per_pass * p.q_head, qo_step = per_pass * p.qo_head;
   const int mine = first < per_pass && first < nH ? (nH - first + per_pass - 1) / per_pass : 0;  // query heads of this thread
-  Unit<T, kInterleaved> u[kBatch];
-#pragma unroll
-  for (int i = 0; i < kBatch; ++i)
-    if (i < mine) u[i].load(q + i * q_step, half, two);
   // Keys: unit e % units of head e / units; a thread's columns are the same as
   // for the queries where per_pass heads fill the block, so that the first
   // round takes the cosines that it has.
   const int v_pieces = hd / N, v_all = H * v_pieces;
   const bool has_key = first < per_pass && first < H;
+  const int v0 = nt - 1 - tid;  // from the block's other end, where no keys are
+  const T* q = static_cast<const T*>(p.q) + t * p.q_token + first * p.q_head + ca;
+  T* q_out = static_cast<T*>(p.q_out) + t * p.qo_token + first * p.qo_head + ca;
+  Unit<T, kInterleaved> u[kBatch];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i)
+    if (i < mine) u[i].load(q + i * q_step, half, two);
   Unit<T, kInterleaved> ku;
   if (has_key) ku.load(static_cast<const T*>(p.k) + t * p.k_token + first * p.k_head + ca, half, two);
   auto value_at = [&](int i) {
     const int h = i / v_pieces;
     return static_cast<const T*>(p.v) + t * p.v_token + h * p.v_head + (i - h * v_pieces) * N;
   };
-  const int v0 = nt - 1 - tid;  // from the block's other end, where no keys are
   Piece<T> v;
   if (v0 < v_all) v.load(value_at(v0));
-  const Token k = token_of(p, t);
+  const Token k = place_of();
   __align__(16) float c[N];  // interleaved: the first half of them
   __align__(16) float s[N];
   if (turns && (mine > 0 || has_key)) {
     const int from = kInterleaved ? unit * N / 2 : unit * N;
-    constexpr int kCos = kInterleaved ? N / 2 : N, kAtOnce = kCos % 4 ? 2 : 4;
+    constexpr int kCos = kInterleaved ? N / 2 : N, kStep = kCos % 4 ? 2 : 4;
 #pragma unroll
-    for (int i = 0; i < kCos; i += kAtOnce) {
-      if (kAtOnce == 4) {
+    for (int i = 0; i < kCos; i += kStep) {
+      if (kStep == 4) {
         *reinterpret_cast<float4*>(c + i) = __ldg(reinterpret_cast<const float4*>(k.cs + from + i));
         *reinterpret_cast<float4*>(s + i) = __ldg(reinterpret_cast<const float4*>(k.sn + from + i));
       } else {
@@ -273,6 +274,41 @@ __global__ void __launch_bounds__(kMany ? 128 : 512, kMany ? 7 : 1) append_wide_
     }
   }
   mark_slot(p, k);
+}
+
+template <typename T, bool kInterleaved>
+__global__ void __launch_bounds__(512, 1) append_wide_kernel(const AppendParams p, int units, int per_pass) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int t = blockIdx.x;
+  append_token<T, kInterleaved>(p, units, per_pass, t, [&]() { return token_of(p, t); });
+}
+
+// Many tokens: a block goes from one to the next, and looks the places of its
+// next kAtOnce up together, so that index, page table and position cost their
+// latency once for all of them.  8192 tokens of 64 + 8 heads of 64 in bf16: 33.3
+// us, 5.1 TB/s; 37.9 us with a block per token.  Five blocks an SM leave enough
+// registers for the pieces in flight; with four 34.7 us, six 33.7, seven 34.8,
+// and with three query heads in flight 36.1.
+template <typename T, bool kInterleaved>
+__global__ void __launch_bounds__(128, kManyBlocks) append_many_kernel(const AppendParams p, int units, int per_pass) {
+  __shared__ Token places[kAtOnce];
+  griddep_wait();
+  griddep_launch_dependents();
+  int turn = 0;
+#pragma unroll 1
+  for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    append_token<T, kInterleaved>(p, units, per_pass, t, [&]() {
+      if (turn == 0) {
+        __syncthreads();  // the places before are used up
+        const int64_t mine = t + threadIdx.x * static_cast<int64_t>(gridDim.x);
+        if (threadIdx.x < kAtOnce && mine < p.tokens) places[threadIdx.x] = token_of(p, static_cast<int>(mine));
+        __syncthreads();
+      }
+      return places[turn];
+    });
+    if (++turn == kAtOnce) turn = 0;
+  }
 }
 
 // Any layout, stride and alignment, one pair or column per thread.  One block
@@ -352,14 +388,17 @@ cudaError_t launch_append(const AppendParams& p, int sms, cudaStream_t st) {
   const int units = (hd - (p.interleaved ? 0 : half)) / N;
   if (!aligned || units > 512) return launch_kernel(append_kernel<T>, dim3(p.tokens), dim3(256), 0, st, p);
   // Threads of a token: enough of them to fill the SMs (2048 a SM), up to a
-  // thread per unit for the shortest chain; at 128 seven blocks share a SM.
+  // thread per unit for the shortest chain.  1023 tokens of 32 + 8 heads of 128 in
+  // 32 bits into 8: 12.1 us with 288 threads, 13.7 with 224, 15.5 with 128.
   const int heads = p.q ? p.c.n_heads : p.c.kv_heads;
   const int want = std::max(units, std::min(512, std::max(128, sms * 2048 / p.tokens / 32 * 32)));
   const int passes = (heads * units + want - 1) / want, per_pass = std::min(want / units, (heads + passes - 1) / passes);
   const int threads = (per_pass * units + 31) / 32 * 32;
-  const auto fn = threads <= 128 ? (p.interleaved ? append_wide_kernel<T, true, true> : append_wide_kernel<T, false, true>)
-                                 : (p.interleaved ? append_wide_kernel<T, true, false> : append_wide_kernel<T, false, false>);
-  return launch_kernel(fn, dim3(p.tokens), dim3(threads), 0, st, p, units, per_pass);
+  if (threads > 128)
+    return launch_kernel(p.interleaved ? append_wide_kernel<T, true> : append_wide_kernel<T, false>, dim3(p.tokens), dim3(threads), 0, st,
+                         p, units, per_pass);
+  return launch_kernel(p.interleaved ? append_many_kernel<T, true> : append_many_kernel<T, false>,
+                       dim3(std::min(p.tokens, kManyBlocks * sms)), dim3(threads), 0, st, p, units, per_pass);
 }
 
 }  // namespace
