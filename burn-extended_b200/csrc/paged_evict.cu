@@ -466,13 +466,18 @@ __global__ void lens_kernel(const EvictParams p, int32_t* lens) {
 }
 
 cudaError_t launch_select(const EvictParams& p, int sms, cudaStream_t st) {
-  // Blocks of a (row, key head): one, as a cluster's barriers cost more than
-  // they save (MEASURE), unless the longest row's keys and lists (8 bytes a slot)
-  // need more, or long rows leave SMs idle.
-  constexpr int kSlots = 24 * 1024;  // of one block's shared memory
-  const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size;
-  int C = 1;
-  while (C < kMaxCluster && ((cap + C - 1) / C > kSlots || (C < 4 && 2 * p.rows * p.c.kv_heads * C < sms && cap / C > 8 * kThreads))) C *= 2;
+  // Blocks of a (row, key head): as many as its keys and lists (8 bytes a slot)
+  // need.  Rows of more than 8192 slots that leave SMs idle get up to kSpread, of
+  // at least 4096 slots each: 12000 slots of 8 heads 16.2 us with three blocks,
+  // 18.4 with two, 21.8 with one; below that a cluster's barriers cost more than
+  // the shorter share saves (4500 slots 9.4 us alone, 10.4 as two).  Clusters of
+  // seven and eight blocks do not all find room at once (16 of them 55 us
+  // against 30 with six).
+  constexpr int kSlots = 24 * 1024, kSpread = 6;
+  const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size, pairs = static_cast<int64_t>(p.rows) * p.c.kv_heads;
+  const int64_t need = (cap + kSlots - 1) / kSlots;
+  const int64_t spread = cap > 8192 ? std::min({(cap + 4095) / 4096, sms / pairs, static_cast<int64_t>(kSpread)}) : 1;
+  const int C = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxCluster, std::max(need, spread))));
   const int64_t slots = ((cap + C - 1) / C + 3) / 4 * 4;
   if (slots > kSlots) {
     return launch_kernel(evict_long_kernel, dim3(p.c.kv_heads, p.rows), dim3(kLongThreads), 0, st, p);

@@ -374,6 +374,33 @@ def test_append_token_by_row_in_place(torch, tokens):
         assert torch.equal(P.k[pg, :, sl], k[t]) and torch.equal(P.v[pg, :, sl], v[t])
 
 
+@pytest.mark.parametrize("dtype,cache,interleaved", [("bf16", "bf16", False), ("f32", "e4m3", True), ("f32", "f32", False)])
+def test_append_more_tokens_than_blocks(torch, dtype, cache, interleaved):
+    """Blocks that take one token after another, more than they look up together, places among them that are not written."""
+    T, hd, nH, H = 13001, 16, 3, 1
+    lens = [4334, 4334, 4334]
+    P = Pool(torch, lens, nH, H, hd, 16, cache)
+    t = np.arange(T)
+    rows, index = (t % 3).astype(np.int32), np.where(t % 11 == 5, -1, t // 3).astype(np.int32)
+    pos = (t * 7 % 4001).astype(np.int32)
+    g = torch.Generator().manual_seed(8)
+    q, k, v = (torch.randn(T, n, hd, generator=g).to(getattr(torch, DT[dtype])).cuda() for n in (nH, H, H))
+    got = P.cache.append(q, k, v, P.tables, torch.from_numpy(index).cuda(), table(torch, 8, 4001, interleaved),
+                         torch.from_numpy(pos).cuda(), torch.from_numpy(rows).cuda())
+    P.cache.sync_status()
+    inv, f = po.frequencies(8)
+    wq, wk = (po.rotate(x.double().cpu().numpy(), pos, inv, f, interleaved) for x in (q, k))
+    assert same_values(dtype, got.double().cpu().numpy(), wq)
+    s, z = (1.0, 1.0) if P.hks is None else (P.hks[0].astype(np.float64), P.hvs[0].astype(np.float64))
+    hk, hv = (x.to(torch.float64).cpu().numpy() for x in (P.k, P.v))
+    on = index >= 0
+    page, slot = P.htab[rows[on], index[on] // 16], index[on] % 16
+    assert same_values(cache, hk[page, 0, slot], wk[on, 0] / s)
+    assert same_values(cache, hv[page, 0, slot], v.double().cpu().numpy()[on, 0] / z)
+    off = P.htab[rows[~on], (t // 3)[~on] // 16], (t // 3)[~on] % 16
+    assert np.array_equal(hk[off[0], 0, off[1]], P.hk[off[0], 0, off[1]], equal_nan=True)
+
+
 @pytest.mark.parametrize("shift", [0, 1, 3])
 def test_append_strides_and_alignment(torch, shift):
     hd, nH, H = 64, 4, 2
@@ -463,6 +490,16 @@ def test_evict_types_and_pages(torch, cache, hd, page):
                                          ([12000], 11000), ([9000], 17), ([40000, 33000], 20000), ([2, 1, 0, 3], 1)])
 def test_evict_lengths(torch, lens, budget):
     check_evict(torch, lens, budget, min(4, budget // 2), budget // 4, H=1)
+
+
+@pytest.mark.parametrize("alike", [False, True])
+@pytest.mark.parametrize("lens,budget", [([9000], 8800), ([16380, 8193, 40], 8192), ([20000], 4001), ([24570, 100], 16000)])
+def test_evict_rows_of_several_blocks(torch, lens, budget, alike):
+    """Three to six blocks of a row, shares that end short, weights that are nearly all alike."""
+    def few(P):
+        P.hw[:] = np.random.default_rng(2).integers(0, 2, P.hw.shape).astype(np.float32)
+
+    check_evict(torch, lens, budget, 4, budget // 4, mutate=few if alike else None)
 
 
 def test_evict_ties_zeros_and_nan(torch):
