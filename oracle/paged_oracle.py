@@ -1,5 +1,5 @@
 """The paged key-value cache's operators in 64-bit numpy -- test infrastructure
-only (the checker of the CUDA path, never the product).
+only (what the CUDA path is compared with, never the product).
 
 Pools are [n_pages, kv_heads, page_size, head_dim]; the cache index n of a row
 is slot n % page_size of page tables[row, n // page_size].  Written from the
