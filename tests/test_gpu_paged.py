@@ -502,6 +502,12 @@ def test_evict_rows_of_several_blocks(torch, lens, budget, alike):
     check_evict(torch, lens, budget, 4, budget // 4, mutate=few if alike else None)
 
 
+@pytest.mark.parametrize("length,budget", [(160000, 40000), (190000, 189000), (200000, 150000)])
+def test_evict_the_longest_rows(torch, length, budget):
+    """Seven and eight blocks of a row, and rows too long for that."""
+    check_evict(torch, [length, 300], budget, 4, 1000, H=1, hd=16)
+
+
 def test_evict_ties_zeros_and_nan(torch):
     def ties(P):
         P.hw[:] = np.random.default_rng(0).integers(0, 3, P.hw.shape).astype(np.float32)
