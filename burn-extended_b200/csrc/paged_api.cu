@@ -80,6 +80,19 @@ int check_tables(const mxmqa_paged_cache* c, const int32_t* tables, int64_t stri
   return MXMOE_OK;
 }
 
+// Zeros device memory and waits for that on a stream of its own: a memset
+// returns before it is done, and the caller's streams need not wait for the
+// legacy stream, nor this call for what is queued there.
+cudaError_t zero_now(void* p, size_t n) {
+  cudaStream_t st = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  if (e != cudaSuccess) return e;
+  e = cudaMemsetAsync(p, 0, n, st);
+  const cudaError_t f = cudaStreamSynchronize(st);
+  cudaStreamDestroy(st);
+  return e != cudaSuccess ? e : f;
+}
+
 // The inverse frequencies of one rotary table in 64 bits.
 int rotary_frequencies(const mxmqa_rotary_config* r, std::vector<double>& f, double& factor) {
   const int half = static_cast<int>(r->rot_dim) / 2;
@@ -206,9 +219,9 @@ int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers*
   const cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&base), bytes);
   if (e != cudaSuccess) {
     rc = pfail(MXMOE_ERR_OOM, "cudaMalloc(%zu bytes): %s", bytes, cudaGetErrorString(e));
-  } else if (cudaMemset(base, 0, 3 * sizeof(int)) != cudaSuccess) {
+  } else if (const cudaError_t z = zero_now(base + head, 3 * sizeof(int)); z != cudaSuccess) {
     cudaFree(base);
-    rc = pfail(MXMOE_ERR_CUDA, "cudaMemset of the workspace failed");
+    rc = pfail(MXMOE_ERR_CUDA, "zeroing the workspace: %s", cudaGetErrorString(z));
   }
   if (rc != MXMOE_OK) {
     cudaGetLastError();

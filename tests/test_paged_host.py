@@ -1,0 +1,48 @@
+"""The paged cache's host side against a CUDA runtime without a device
+(fake_cudart.c, preloaded): what a call has waited for when it returns, what it
+refuses, how much it launches."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+PRELUDE = """
+import ctypes, importlib.util, sys
+spec = importlib.util.spec_from_file_location("_lib", sys.argv[1])
+_lib = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(_lib)
+L, fake = _lib.lib(), ctypes.CDLL(sys.argv[2])
+keep = ctypes.create_string_buffer(4112)
+P = (ctypes.addressof(keep) + 15) // 16 * 16  # 16-byte aligned memory that no check reads
+
+def create(n_pages=4, page=16, heads=8, kv_heads=2, hd=64, dtype=1, weight=None, position=None):
+    h = ctypes.c_void_p()
+    rc = L.mxmqa_paged_create(ctypes.byref(_lib.PagedConfig(n_pages, page, heads, kv_heads, hd, dtype, 0)),
+                              ctypes.byref(_lib.PagedBuffers(P, P, None, None, weight, position)), ctypes.byref(h))
+    assert rc == 0, _lib.last_error()
+    return h
+"""
+
+
+@pytest.fixture(scope="module")
+def fake(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("fake") / "libfake_cudart.so")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-O1", "-w", os.path.join(HERE, "fake_cudart.c"), "-o", out], check=True)
+    return out
+
+
+def run(fake, body):
+    lib = os.path.join(os.path.dirname(HERE), "burn-extended_b200", "mxmoe", "_lib.py")
+    r = subprocess.run([sys.executable, "-c", PRELUDE + body, lib, fake], env=dict(os.environ, LD_PRELOAD=fake),
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, (r.returncode, r.stdout, r.stderr)
+
+
+def test_create_has_zeroed_its_counters_when_it_returns(fake):
+    """Streams that do not wait for the legacy one may use the cache at once."""
+    run(fake, """
+h = create(weight=P, position=P)
+assert fake.fake_pending() == 0
+""")
