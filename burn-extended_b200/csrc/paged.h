@@ -100,6 +100,8 @@ struct DecodeScratch {
 cudaError_t launch_paged_append(const AppendParams& p, int sms, cudaStream_t st);
 cudaError_t launch_paged_decode(const DecodeParams& p, const DecodeScratch& ws, int sms, cudaStream_t st);
 int decode_tile(const PagedView& c);                     // keys of a tile
+// Rows of one launch, whose tiles are numbered in 32 bits; 0: not even one under a table that wide.
+int decode_rows_at_once(const PagedView& c, int max_pages);
 size_t decode_part_floats(const PagedView& c, int sms);  // of DecodeScratch::part
 cudaError_t launch_paged_evict(const EvictParams& p, int sms, cudaStream_t st);
 cudaError_t launch_rotary_table(const double* inv_freq, int half, int64_t first, int n, double factor, float* cos,

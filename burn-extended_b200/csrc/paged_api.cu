@@ -328,6 +328,10 @@ int mxmqa_paged_decode(mxmqa_paged_cache* c, const mxmqa_paged_decode_args* a, v
   if (const int rc = check_tables(c, a->tables, a->table_stride, a->rows, a->max_pages, p.t)) return rc;
   if (static_cast<uint64_t>(a->max_pages) * c->cfg.page_size * c->cfg.n_heads > 16ull * kMaxTokens)
     return pfail(MXMOE_ERR_UNSUPPORTED, "max_pages x page_size x n_heads must be below 2^35");
+  if (mxmoe::decode_rows_at_once(c->view, p.t.max_pages) < 1)
+    return pfail(MXMOE_ERR_UNSUPPORTED,
+                 "max_pages too large: (max_pages x page_size / %d + 1) x kv_heads x (query heads per key head / 8, rounded up) must be below 2^31",
+                 mxmoe::decode_tile(c->view));
   p.c = c->view;
   p.q = a->q;
   p.q_row = a->q_row;

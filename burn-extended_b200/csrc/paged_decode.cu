@@ -103,13 +103,17 @@ size_t decode_part_floats(const PagedView& c, int sms) {
   return static_cast<size_t>(2) * (3 * sms * warps_of(c) + 1) * kDecodeHeads * (padded_head(c) + 2);
 }
 
+int decode_rows_at_once(const PagedView& c, int max_pages) {
+  const int G = c.n_heads / c.kv_heads, segs = c.kv_heads * ((G + kDecodeHeads - 1) / kDecodeHeads);
+  const int64_t most = (static_cast<int64_t>(max_pages) * c.page_size / decode_tile(c) + 1) * segs;
+  return static_cast<int>(std::min<int64_t>(kDecodeMaxRows, INT32_MAX / most));
+}
+
 cudaError_t launch_paged_decode(const DecodeParams& all, const DecodeScratch& ws, int sms, cudaStream_t st) {
   const int64_t longest = std::min<int64_t>(static_cast<int64_t>(all.t.max_pages) * all.c.page_size, all.window ? all.window : INT32_MAX);
   const DecodePlan plan{sms, longest <= kWholeTiles * decode_tile(all.c)};
-  // Rows of one launch: their tiles are numbered in 32 bits.
-  const int G = all.c.n_heads / all.c.kv_heads, segs = all.c.kv_heads * ((G + kDecodeHeads - 1) / kDecodeHeads);
-  const int64_t most = (static_cast<int64_t>(all.t.max_pages) * all.c.page_size / decode_tile(all.c) + 1) * segs;
-  const int chunk = static_cast<int>(std::min<int64_t>(kDecodeMaxRows, INT32_MAX / most));
+  const int chunk = decode_rows_at_once(all.c, all.t.max_pages);
+  if (chunk < 1) return cudaErrorInvalidValue;
   for (int r0 = 0; r0 < all.rows; r0 += chunk) {
     DecodeParams p = all;
     const int act = all.q_dtype == MXMOE_F32 ? 4 : 2, oact = all.out_dtype == MXMOE_F32 ? 4 : 2;

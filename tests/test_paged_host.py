@@ -46,3 +46,27 @@ def test_create_has_zeroed_its_counters_when_it_returns(fake):
 h = create(weight=P, position=P)
 assert fake.fake_pending() == 0
 """)
+
+
+DECODE = """
+def decode(h, rows=1, max_pages=4, window=0, dtype=1, stride=0):
+    a = _lib.PagedDecodeArgs(P, 64, 64, P, 64, 64, None, dtype, dtype, rows, max_pages, P, stride, P, 0.125, window,
+                             None, None, 0, 0, 0, 0, 0)
+    return L.mxmqa_paged_decode(h, ctypes.byref(a), None)
+"""
+
+
+def test_decode_under_the_widest_tables(fake):
+    """Tiles of a launch are numbered in 32 bits: a table one page too wide for one row is refused, and the widest that
+    is not takes one launch for its row."""
+    run(fake, DECODE + """
+h = create(page=16, heads=64, kv_heads=64, hd=128)  # tiles of 16 keys
+for window in (0, 16):
+    n = fake.fake_launches()
+    assert decode(h, max_pages=(1 << 25) - 1, window=window) == 5 and "max_pages" in _lib.last_error()
+    assert fake.fake_launches() == n
+    assert decode(h, max_pages=(1 << 25) - 2, window=window) == 0
+    assert fake.fake_launches() - n <= 2  # the attention, the join of its parts
+h = create(page=1, heads=1024, kv_heads=1024, hd=128)
+assert decode(h, max_pages=33554431, window=16) == 5
+""")
