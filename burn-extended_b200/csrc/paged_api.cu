@@ -60,19 +60,20 @@ struct PDevice {
 };
 
 constexpr uint64_t kMaxTokens = 0x7FFFFFFFu;
+constexpr uint64_t kMaxIndexes = (1u << 31) - 1024;  // of a row: kernels walk them in 32 bits, up to 1024 at a step
 
 bool act_dtype(int d) { return d == MXMOE_F32 || d == MXMOE_BF16; }
 size_t elem_bytes(int d) { return d == MXMOE_F32 ? 4 : d == MXMOE_BF16 ? 2 : 1; }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// The tables of a call, and that cache indexes of a row stay below 2^31.
+// The tables of a call, and that cache indexes of a row stay a step below 2^31.
 int check_tables(const mxmqa_paged_cache* c, const int32_t* tables, int64_t stride, uint32_t rows, uint32_t max_pages,
                  mxmoe::PagedTables& t) {
   P_CHECK(tables != nullptr, "null tables");
   P_CHECK(aligned(tables, 4), "tables must be 4-byte aligned");
   P_CHECK(rows > 0 && rows <= 65535, "rows must be 1 to 65535");
-  P_CHECK(max_pages > 0 && static_cast<uint64_t>(max_pages) * c->cfg.page_size <= kMaxTokens,
-          "max_pages x page_size must be 1 to 2^31 - 1");
+  P_CHECK(max_pages > 0 && static_cast<uint64_t>(max_pages) * c->cfg.page_size <= kMaxIndexes,
+          "max_pages x page_size must be 1 to 2^31 - 1024");
   t.tables = tables;
   t.stride = stride;
   t.n_rows = static_cast<int>(rows);

@@ -70,3 +70,24 @@ for window in (0, 16):
 h = create(page=1, heads=1024, kv_heads=1024, hd=128)
 assert decode(h, max_pages=33554431, window=16) == 5
 """)
+
+
+def test_cache_indexes_stay_a_stride_below_2_to_the_31(fake):
+    """The kernels walk a row in strides of up to 1024 cache indexes, held in 32 bits."""
+    run(fake, DECODE + """
+h = create(page=1, heads=2, kv_heads=2, weight=P, position=P)
+
+def append(max_pages):
+    a = _lib.PagedAppendArgs(None, P, P, 0, 0, 128, 64, 128, 64, None, 0, 0, None, 0, 0, 1, 1, P, 0, 1, max_pages,
+                             None, P, None, None, None, 0, 0, 0)
+    return L.mxmqa_paged_append(h, ctypes.byref(a), None)
+
+def evict(max_pages):
+    a = _lib.PagedEvictArgs(P, 0, 1, max_pages, P, P, P + 4, 8, 0, 0)
+    return L.mxmqa_paged_evict(h, ctypes.byref(a), None)
+
+for f in (append, lambda n: decode(h, max_pages=n), evict):
+    for n in (2 ** 31 - 1, 2 ** 31 - 1023):
+        assert f(n) == 1 and "max_pages" in _lib.last_error()
+    assert f(2 ** 31 - 1024) == 0, _lib.last_error()
+""")
