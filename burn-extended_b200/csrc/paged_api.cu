@@ -432,6 +432,9 @@ int mxmqa_rotary(const mxmqa_rotary_args* a, void* stream) {
   const size_t es = elem_bytes(a->dtype);
   P_CHECK(aligned(a->x, es) && aligned(a->out, es) && aligned(a->positions, 4), "x, out or positions misaligned");
   if (const int rc = check_rotary(a->cos, a->sin, a->rot_dim, a->n_positions, a->head_dim)) return rc;
+  // a token's pairs and passing columns are numbered in 32 bits, 256 at a step
+  if (static_cast<uint64_t>(a->heads) * (a->head_dim - a->rot_dim / 2) > kMaxTokens - 256)
+    return pfail(MXMOE_ERR_UNSUPPORTED, "heads x (head_dim - rot_dim / 2) must be below 2^31 - 256");
   mxmoe::AppendParams p{};
   p.c.n_heads = static_cast<int>(a->heads);
   p.c.head_dim = static_cast<int>(a->head_dim);

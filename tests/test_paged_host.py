@@ -91,3 +91,21 @@ for f in (append, lambda n: decode(h, max_pages=n), evict):
         assert f(n) == 1 and "max_pages" in _lib.last_error()
     assert f(2 ** 31 - 1024) == 0, _lib.last_error()
 """)
+
+
+def test_rotary_refuses_more_pairs_than_it_can_number(fake):
+    """The kernel for any stride numbers the pairs and passing columns of a token in 32 bits, 256 at a step."""
+    run(fake, """
+def turn(heads, hd, rot):
+    a = _lib.RotaryArgs(P, heads * hd, hd, P, heads * hd, hd, 1, 1, heads, hd, P, P, P, rot, 8, 0, 0, 0)
+    return L.mxmqa_rotary(ctypes.byref(a), None)
+
+for heads, hd, rot in ((65535, 65536, 65536), (65535, 65536, 0), (32768, 65536, 2), (65535, 32768, 0)):
+    n = fake.fake_launches()
+    rc = turn(heads, hd, rot)
+    if heads * (hd - rot // 2) > 2 ** 31 - 257:
+        assert rc == 5 and "heads" in _lib.last_error() and fake.fake_launches() == n, (heads, hd, rot)
+    else:
+        assert rc == 0 and fake.fake_launches() == n + 1, (heads, hd, rot)
+assert turn(32769, 65535, 0) == 5 and turn(32767, 65536, 0) == 0
+""")
