@@ -42,18 +42,17 @@ struct Token {
   const float *cs, *sn;  // its row of the table
 };
 
+// A position outside the table: the outputs turn as position 0, nothing enters
+// the cache.
 __device__ __forceinline__ Token token_of(const AppendParams& p, int t) {
   const int index = p.index ? __ldg(p.index + t) : -1, half = p.rot / 2;
   Token k{-1, p.positions ? __ldg(p.positions + t) : (index > 0 ? index : 0), nullptr, nullptr};
-  if (p.rot && (k.pos < 0 || k.pos >= p.n_positions)) {
-    if (p.c.status) atomicOr(p.c.status, kPagedBadPosition);
-    k.cs = p.cos;
-    k.sn = p.sin;
-  } else {
-    k.cs = p.cos + static_cast<int64_t>(k.pos) * half;  // unread without a rotation
-    k.sn = p.sin + static_cast<int64_t>(k.pos) * half;
-  }
-  if (p.k && index >= 0) {
+  const bool on_table = !p.rot || (k.pos >= 0 && k.pos < p.n_positions);
+  if (!on_table && p.c.status) atomicOr(p.c.status, kPagedBadPosition);
+  const int64_t from = on_table ? static_cast<int64_t>(k.pos) * half : 0;  // unread without a rotation
+  k.cs = p.cos + from;
+  k.sn = p.sin + from;
+  if (p.k && index >= 0 && on_table) {
     const int row = p.rows ? __ldg(p.rows + t) : t;
     if (row < 0 || row >= p.t.n_rows)
       atomicOr(p.c.status, kPagedBadIndex);

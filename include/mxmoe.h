@@ -686,7 +686,9 @@ typedef struct mxmqa_paged_append_args {
 } mxmqa_paged_append_args;
 
 /* Two tokens of one call must not name the same slot.  Where the cache has
- * them, the slot's weight becomes 0 and its position the token's. */
+ * them, the slot's weight becomes 0 and its position the token's.  A token whose
+ * position is outside the table does not enter the cache; its row of q_out and
+ * k_out is turned as position 0. */
 MXMOE_API int mxmqa_paged_append(mxmqa_paged_cache* cache, const mxmqa_paged_append_args* args, void* stream);
 
 typedef struct mxmqa_paged_decode_args {
