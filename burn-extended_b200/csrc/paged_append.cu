@@ -25,14 +25,15 @@ __device__ __forceinline__ void st1(float* p, float x) { *p = x; }
 __device__ __forceinline__ void st1(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // One value into the cache's element type.  8 bits hold x / scale, rounded to
-// nearest and held at +-448.
-__device__ __forceinline__ void st_cache(void* pool, int dtype, int64_t i, float x, float inv_scale) {
+// nearest and held at +-448: the quotient itself, as x times the rounded 1 /
+// scale goes to the other neighbour near a tie.
+__device__ __forceinline__ void st_cache(void* pool, int dtype, int64_t i, float x, float scale) {
   if (dtype == MXMOE_F32)
     static_cast<float*>(pool)[i] = x;
   else if (dtype == MXMOE_BF16)
     static_cast<__nv_bfloat16*>(pool)[i] = __float2bfloat16_rn(x);
   else
-    static_cast<uint8_t*>(pool)[i] = __nv_cvt_float_to_fp8(x * inv_scale, __NV_SATFINITE, __NV_E4M3);
+    static_cast<uint8_t*>(pool)[i] = __nv_cvt_float_to_fp8(x / scale, __NV_SATFINITE, __NV_E4M3);
 }
 
 // Where a token goes, and how far it turns.
@@ -114,7 +115,7 @@ __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&x)[N]) {
     *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]));
 }
 template <int N>
-__device__ __forceinline__ void store_cache(void* pool, int dtype, int64_t at, const float (&x)[N], float inv) {
+__device__ __forceinline__ void store_cache(void* pool, int dtype, int64_t at, const float (&x)[N], float scale) {
   if (dtype == MXMOE_F32) {
     store(static_cast<float*>(pool) + at, x);
   } else if (dtype == MXMOE_BF16) {
@@ -123,8 +124,8 @@ __device__ __forceinline__ void store_cache(void* pool, int dtype, int64_t at, c
     uint32_t w[N / 4];
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i] * inv, x[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2] * inv, x[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i] / scale, x[4 * i + 1] / scale), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2] / scale, x[4 * i + 3] / scale), __NV_SATFINITE, __NV_E4M3);
       w[i] = a | b << 16;
     }
     uint8_t* d = static_cast<uint8_t*>(pool) + at;
@@ -256,9 +257,9 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int units, i
       }
       if (k.slot >= 0) {
         const int64_t at = (k.slot + static_cast<int64_t>(h) * p.c.page_size) * hd + ca;
-        const float inv = p.c.k_scale ? 1.0f / __ldg(p.c.k_scale + h) : 1.0f;
-        store_cache(p.c.k, p.c.dtype, at, x, inv);
-        if (two) store_cache(p.c.k, p.c.dtype, at + half, y, inv);
+        const float scale = p.c.k_scale ? __ldg(p.c.k_scale + h) : 1.0f;
+        store_cache(p.c.k, p.c.dtype, at, x, scale);
+        if (two) store_cache(p.c.k, p.c.dtype, at + half, y, scale);
       }
     }
   }
@@ -269,7 +270,7 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int units, i
       const int h = i / v_pieces;
       v.open(x);
       store_cache(p.c.v, p.c.dtype, (k.slot + static_cast<int64_t>(h) * p.c.page_size) * hd + (i - h * v_pieces) * N, x,
-                  p.c.v_scale ? 1.0f / __ldg(p.c.v_scale + h) : 1.0f);
+                  p.c.v_scale ? __ldg(p.c.v_scale + h) : 1.0f);
     }
   }
   mark_slot(p, k);
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
     T* y = isq ? static_cast<T*>(p.q_out) + t * p.qo_token + h * p.qo_head
                : (p.k_out ? static_cast<T*>(p.k_out) + t * p.ko_token + kh * p.ko_head : nullptr);
     const int64_t kbase = isq || k.slot < 0 ? -1 : (k.slot + static_cast<int64_t>(kh) * p.c.page_size) * hd;
-    const float inv = !isq && p.c.k_scale ? 1.0f / p.c.k_scale[kh] : 1.0f;
+    const float scale = !isq && p.c.k_scale ? p.c.k_scale[kh] : 1.0f;
     const int ca = j < half ? (p.interleaved ? 2 * j : j) : half + j;
     const int cb = p.interleaved ? ca + 1 : ca + half;
     const float a = ld1(x + ca);
@@ -341,20 +342,20 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
         st1(y + cb, w);
       }
       if (kbase >= 0) {
-        st_cache(p.c.k, p.c.dtype, kbase + ca, u, inv);
-        st_cache(p.c.k, p.c.dtype, kbase + cb, w, inv);
+        st_cache(p.c.k, p.c.dtype, kbase + ca, u, scale);
+        st_cache(p.c.k, p.c.dtype, kbase + cb, w, scale);
       }
     } else {
       if (y) st1(y + ca, a);
-      if (kbase >= 0) st_cache(p.c.k, p.c.dtype, kbase + ca, a, inv);
+      if (kbase >= 0) st_cache(p.c.k, p.c.dtype, kbase + ca, a, scale);
     }
   }
   if (k.slot >= 0) {
     for (int i = threadIdx.x; i < H * hd; i += blockDim.x) {
       const int h = i / hd, j = i - h * hd;
-      const float inv = p.c.v_scale ? 1.0f / p.c.v_scale[h] : 1.0f;
+      const float scale = p.c.v_scale ? p.c.v_scale[h] : 1.0f;
       st_cache(p.c.v, p.c.dtype, (k.slot + static_cast<int64_t>(h) * p.c.page_size) * hd + j,
-               ld1(static_cast<const T*>(p.v) + t * p.v_token + h * p.v_head + j), inv);
+               ld1(static_cast<const T*>(p.v) + t * p.v_token + h * p.v_head + j), scale);
     }
   }
   mark_slot(p, k);

@@ -65,3 +65,34 @@ def test_append_skips_positions_outside_the_table(torch, T, nH, H, hd, rot, cach
     for now, was in zip((P.k, P.v, P.weight, P.position), before):
         raw = {2: torch.int16, 4: torch.int32}[now.element_size()]
         assert torch.equal(now.view(raw), was.view(raw))
+
+
+@pytest.mark.parametrize("dtype,hd", [("f32", 64), ("bf16", 64), ("f32", 80)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_append_8_bit_rounds_the_quotient(torch, dtype, hd, shift):
+    """An 8-bit code is the one nearest to x / scale, ties to even, also where x is a rounded tie times the scale: the
+    bits of a correctly rounded quotient rounded again.  shift: off the alignment of wide loads."""
+    T, H = 512, 8
+    P = Pool(torch, [0], H, H, hd, 16, "e4m3", max_pages=T // 16)
+    codes = torch.arange(0, 126, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    ties = (codes[1:] + codes[:-1]) / 2
+    g = torch.Generator().manual_seed(3)
+    x = ties[torch.randint(len(ties), (T, H, hd), generator=g)] * (torch.randint(0, 2, (T, H, hd), generator=g) * 2 - 1)
+    ks, vs = (s.double().cpu()[:, None] for s in (P.ks, P.vs))
+    dt = getattr(torch, DT[dtype])
+    k, v = (x * ks).to(dt), (x * vs).to(dt)
+    k[0, 0, :4] = torch.tensor([float("inf"), float("-inf"), float("nan"), -0.0])
+
+    def off(t):
+        return torch.cat([torch.zeros(shift, dtype=dt), t.flatten()]).cuda()[shift:].view(t.shape)
+
+    P.cache.append(None, off(k), off(v), P.tables, torch.arange(T, dtype=torch.int32, device="cuda"),
+                   rows=torch.zeros(T, dtype=torch.int32, device="cuda"))
+    P.cache.sync_status()
+    pg, sl = po.place(P.htab, 16, 0, np.arange(T))
+    for pool, t, s in ((P.k, k, ks), (P.v, v, vs)):
+        want = (t.float() / s.float()).clamp(-448, 448).to(torch.float8_e4m3fn)
+        got = pool.cpu().view(torch.uint8)[pg, :, sl].view(torch.float8_e4m3fn)
+        nan = want.float().isnan()
+        assert torch.equal(got.float().isnan(), nan)
+        assert torch.equal(got.view(torch.uint8)[~nan], want.view(torch.uint8)[~nan])
