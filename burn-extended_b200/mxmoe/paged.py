@@ -27,6 +27,7 @@ from ._lib import (E4M3, BF16, F32, MxMoeError, PagedAppendArgs, PagedBuffers, P
 
 _ACT = {torch.float32: F32, torch.bfloat16: BF16}
 _CACHE = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3}
+_MOST = (1 << 32) - 1  # of a count in the C structs: ctypes would wrap a larger one around
 _SCALING = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3, "streaming": 4}
 
 
@@ -98,8 +99,8 @@ class RotaryTable:
     def of(cfg: RotaryConfig, n_positions: int, interleaved: bool = False, device: int = 0) -> "RotaryTable":
         if cfg.scaling not in _SCALING:
             _bad(f"scaling {cfg.scaling!r}: expected one of {sorted(_SCALING)}")
-        if cfg.rot_dim <= 0 or n_positions <= 0:
-            _bad("rot_dim and n_positions must be positive")
+        if not 0 < cfg.rot_dim <= _MOST or not 0 < n_positions <= _MOST:
+            _bad("rot_dim and n_positions must be positive and below 2^32")
         dev = torch.device("cuda", device)
         cos, sin = (torch.empty(n_positions, cfg.rot_dim // 2, device=dev) for _ in range(2))
         c = RotaryTableConfig(cfg.rot_dim, _SCALING[cfg.scaling], cfg.theta, cfg.scaling_factor, cfg.initial_context,
@@ -165,6 +166,8 @@ class PagedKvCache:
             if t is not None and (t.dtype != dt or tuple(t.shape) != tuple(shape) or not t.is_contiguous()
                                   or not t.is_cuda or t.device != k.device):
                 _bad(f"{name}: expected contiguous {dt} {tuple(shape)} on the cache's device")
+        if not 0 <= n_heads <= _MOST:
+            _bad("n_heads must not be negative nor reach 2^32")
         self.k, self.v, self.weight, self.position = k, v, weight, position
         self.k_scale, self.v_scale = k_scale, v_scale
         self.n_pages, self.page_size, self.n_heads = n_pages, page_size, n_heads
@@ -266,8 +269,8 @@ class PagedKvCache:
                 _bad(f"bias: expected float32 [{n} or 1, {nH} or 1, length] on {dev}")
             b = (bias.data_ptr(), 0 if bias.shape[0] == 1 else bias.stride(0),
                  0 if bias.shape[1] == 1 else bias.stride(1), bias.shape[2])
-        if window < 0:
-            _bad("window must not be negative")
+        if not 0 <= window <= _MOST:
+            _bad("window must not be negative nor reach 2^32")
         a = PagedDecodeArgs(q.data_ptr(), *qs, out.data_ptr(), *os, None if lse is None else lse.data_ptr(),
                             _act("q", q), _act("out", out), n, max_pages, t, stride, _ints("lens", lens, n, dev),
                             1.0 / math.sqrt(hd) if scale is None else scale, window,
@@ -285,8 +288,8 @@ class PagedKvCache:
         t, stride, n, max_pages = self._tables(tables)
         if new_lens is None:
             new_lens = torch.empty_like(lens)
-        if budget < 0 or sink < 0 or recent < 0:
-            _bad("budget, sink and recent must not be negative")
+        if not (0 <= budget <= _MOST and 0 <= sink <= _MOST and 0 <= recent <= _MOST):
+            _bad("budget, sink and recent must not be negative nor reach 2^32")
         a = PagedEvictArgs(t, stride, n, max_pages, _ints("lens", lens, n, dev), _ints("seen", seen, n, dev),
                            _ints("new_lens", new_lens, n, dev), budget, sink, recent)
         check(self._lib.mxmqa_paged_evict(self._h, ctypes.byref(a), _stream(dev)))

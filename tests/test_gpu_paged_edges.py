@@ -96,3 +96,24 @@ def test_append_8_bit_rounds_the_quotient(torch, dtype, hd, shift):
         nan = want.float().isnan()
         assert torch.equal(got.float().isnan(), nan)
         assert torch.equal(got.view(torch.uint8)[~nan], want.view(torch.uint8)[~nan])
+
+
+def test_numbers_past_32_bits_are_refused(torch):
+    """They do not wrap around on their way to the C structs."""
+    from mxmoe import MxMoeError
+    from mxmoe.paged import PagedKvCache, RotaryConfig, RotaryTable
+    P = Pool(torch, [40, 40], 8, 2, 64, 16, track=True)
+    q = torch.randn(2, 8, 64, device="cuda")
+    before = [x.clone() for x in (P.k, P.v, P.weight, P.position)]
+    w = 1 << 32
+    for f in (lambda: P.cache.decode(q, P.tables, P.lens, window=w + 5),
+              lambda: P.cache.evict(P.tables, P.lens, P.lens, w + 30),
+              lambda: P.cache.evict(P.tables, P.lens, P.lens, 30, sink=w),
+              lambda: P.cache.evict(P.tables, P.lens, P.lens, 30, recent=w),
+              lambda: PagedKvCache(4, 16, w + 8, 2, 64), lambda: PagedKvCache.over(P.k, P.v, w + 8),
+              lambda: RotaryTable.of(RotaryConfig(w + 64), 1)):
+        with pytest.raises(MxMoeError):
+            f()
+    for now, was in zip((P.k, P.v, P.weight, P.position), before):
+        raw = {2: torch.int16, 4: torch.int32}[now.element_size()]
+        assert torch.equal(now.view(raw), was.view(raw))
