@@ -234,13 +234,15 @@ __device__ __forceinline__ void sum_pair(float (&s)[N], int j, const float (&d)[
 //
 // Each has: Q, the query operand; V, values on their way; load(), which fills them for lane (g, t) =
 // (lane / 4, lane % 4) from head g's row in shared memory; scores(), s[4] of keys 2t, 2t + 1,
-// 8 + 2t, 9 + 2t; and add(), o = o corr + p V over the tile's 16 keys.  HDT:
+// 8 + 2t, 9 + 2t; and add(), o = o corr + p V over the tile's 16 keys, with
+// shares p (and so o and their sum l) that are 2^kShareBits too large.  HDT:
 // head_dim rounded up to the register arrays' size; X: 32-bit activations, a
 // third term each for queries and shares where two hold 16 bits only.
 
 template <int HDT, bool X>
 struct Bf16 {
   static constexpr bool kWide = X;
+  static constexpr int kShareBits = 0;
   static constexpr int kElem = 2, rb = ring_row(HDT * 2), NT = tile_halves(HDT * 2), kWarps = warps_for(stage_bytes(HDT, 2));
   static constexpr int kStageBytes = stage_bytes(HDT, 2);
   struct Q {
@@ -372,7 +374,10 @@ struct Bf16 {
 // 8-bit keys and values widen to f16 without loss.  A query row is scaled by a
 // power of two to a maximum of 2^8 to 2^9 (f16's range is too short for any
 // row), two f16 terms then hold 22 bits of it, the first alone a bf16 query's
-// eight; a share lies in [0, 1] and is held in two terms as well.  The MMA on
+// eight.  A share lies in [0, 1] and is held in two terms as well, times 2^14
+// until its segment is summed: f16 ends at 2^-24, so that unscaled terms would
+// lose the shares below 2^-25, thousands of which may stand under one large
+// one.  Scaled they are off by 2^-39 of the largest at most.  The MMA on
 // 8-bit operands would save the widening, but its sums keep too few bits: scores
 // were off by 6e-4.
 // The order of the contracted columns within 16 is free as long as both
@@ -381,6 +386,7 @@ struct Bf16 {
 template <int HDT, bool X>
 struct E4m3 {
   static constexpr bool kWide = X;
+  static constexpr int kShareBits = 14;
   static constexpr int kElem = 1, rb = ring_row(HDT), NT = tile_halves(HDT), kWarps = warps_for(stage_bytes(HDT, 1));
   static constexpr int kStageBytes = stage_bytes(HDT, 1);
   struct Q {
@@ -517,6 +523,7 @@ template <int HDT, bool X>
 struct F32 {
   static_assert(X, "a 32-bit cache is read in 32 bits");
   static constexpr bool kWide = true;
+  static constexpr int kShareBits = 0;
   static constexpr int kElem = 4, rb = ring_row(HDT * 4), NT = tile_halves(HDT * 4), kWarps = warps_for(stage_bytes(HDT, 4));
   static constexpr int kStageBytes = stage_bytes(HDT, 4);
   struct Q {
@@ -1113,7 +1120,7 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4 * NT; ++i) {
-          w[i] = ex2((s[i] - base) * c);
+          w[i] = C::kShareBits ? ex2(fmaf(s[i] - base, c, C::kShareBits)) : ex2((s[i] - base) * c);
           sum += w[i];
         }
         l = fmaf(l, corr, sum);
@@ -1126,6 +1133,11 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
       m *= unit;
       l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
       l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+      if constexpr (C::kShareBits > 0) {
+        constexpr float kBack = 1.0f / (1 << C::kShareBits);
+        l *= kBack;
+        o.scale(kBack, kBack);
+      }
       x += n;
       if (x < end) at.next_segment(p, rows, parts);
     }

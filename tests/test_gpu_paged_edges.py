@@ -117,3 +117,29 @@ def test_numbers_past_32_bits_are_refused(torch):
     for now, was in zip((P.k, P.v, P.weight, P.position), before):
         raw = {2: torch.int16, 4: torch.int32}[now.element_size()]
         assert torch.equal(now.view(raw), was.view(raw))
+
+
+@pytest.mark.parametrize("gap", [14.0, 17.5, 20.0, 24.0])
+@pytest.mark.parametrize("n,hd,every", [(20, 16, 20), (256, 64, 256), (200, 128, 200), (100, 256, 100), (30000, 64, 300)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_decode_8_bit_keeps_small_shares(torch, gap, n, hd, every, dtype):
+    """One key in `every` holds nearly all of the softmax and has a value of 0; the others, `gap` below it, make up the
+    output.  A share is held to half a step of the second of its two terms, 2^-39 of the largest, and as it is held
+    in 22 bits otherwise to 1e-5 of itself."""
+    from mxmoe.paged import PagedKvCache
+    page = 16
+    pages = -(-n // page)
+    k = torch.zeros(pages, 1, page, hd)
+    v = torch.full((pages, 1, page, hd), 448.0)
+    at = np.arange(0, n, every)
+    k[at // page, 0, at % page, 0] = 16.0
+    v[at // page, 0, at % page] = 0.0
+    q = torch.zeros(1, 2, hd, dtype=getattr(torch, DT[dtype]))
+    q[0, :, 0] = gap / 16  # exact in bf16
+    e4 = torch.float8_e4m3fn
+    cache = PagedKvCache.over(k.to(e4).cuda(), v.to(e4).cuda(), 2)
+    tab = np.arange(pages, dtype=np.int32)[None]
+    got = cache.decode(q.cuda(), torch.from_numpy(tab).cuda(), torch.tensor([n], dtype=torch.int32, device="cuda"), scale=1.0)
+    want, _ = po.decode(q.double().numpy(), k.double().numpy(), v.double().numpy(), tab, np.array([n]), 1.0)
+    tol = 448 * every * 2.0 ** -39 + 1e-5 * want + (2.0 ** -8 * want if dtype == "bf16" else 0)
+    assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol)
