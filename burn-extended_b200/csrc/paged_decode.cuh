@@ -243,6 +243,7 @@ template <int HDT, bool X>
 struct Bf16 {
   static constexpr bool kWide = X;
   static constexpr int kShareBits = 0;
+  using Elem = __nv_bfloat16;
   static constexpr int kElem = 2, rb = ring_row(HDT * 2), NT = tile_halves(HDT * 2), kWarps = warps_for(stage_bytes(HDT, 2));
   static constexpr int kStageBytes = stage_bytes(HDT, 2);
   struct Q {
@@ -387,6 +388,7 @@ template <int HDT, bool X>
 struct E4m3 {
   static constexpr bool kWide = X;
   static constexpr int kShareBits = 14;
+  using Elem = __nv_fp8_e4m3;
   static constexpr int kElem = 1, rb = ring_row(HDT), NT = tile_halves(HDT), kWarps = warps_for(stage_bytes(HDT, 1));
   static constexpr int kStageBytes = stage_bytes(HDT, 1);
   struct Q {
@@ -524,6 +526,7 @@ struct F32 {
   static_assert(X, "a 32-bit cache is read in 32 bits");
   static constexpr bool kWide = true;
   static constexpr int kShareBits = 0;
+  using Elem = float;
   static constexpr int kElem = 4, rb = ring_row(HDT * 4), NT = tile_halves(HDT * 4), kWarps = warps_for(stage_bytes(HDT, 4));
   static constexpr int kStageBytes = stage_bytes(HDT, 4);
   struct Q {
@@ -707,6 +710,85 @@ static __device__ __noinline__ float2 finish(float sink, int quiet, float m, flo
   return make_float2(f / sum, top + logf(sum));
 }
 
+__device__ __forceinline__ float element(const float* p, int64_t i) { return p[i]; }
+__device__ __forceinline__ float element(const __nv_bfloat16* p, int64_t i) { return __bfloat162float(p[i]); }
+__device__ __forceinline__ float element(const __nv_fp8_e4m3* p, int64_t i) { return static_cast<float>(p[i]); }
+
+// Head i of the segment at `at` again, over this warp's tiles (`first`, first +
+// step and so on of n), by the formula in 32-bit arithmetic: a key of score -inf
+// does not count, whatever lies there, and an infinite value is infinite in its
+// column.  The products of the tile loop give NaN for both, since they multiply
+// by shares of 0 and split shares, queries and 32-bit keys into terms of either
+// sign; a head whose sums came out NaN there is computed here.  A lane takes a
+// key for the scores, columns for the output, which goes to `out`; the maximum
+// and sum are returned.  64 rows of 8192 tokens with a NaN in one query head of
+// each row take as long as without; with all queries NaN 0.5 ms against 0.2.
+template <class C, int HDT>
+static __device__ __noinline__ float2 plain_head(const DecodeParams& p, const DecodeScratch& ws, const Place& at, int x, int n,
+                                                 int first, int step, int i, float* out) {
+  using Elem = typename C::Elem;
+  constexpr int kTile = 16 * C::NT, kColumns = (HDT + 31) / 32;
+  const int lane = threadIdx.x & 31, hd = p.c.head_dim, G = p.c.n_heads / p.c.kv_heads, h = at.kvh * G + at.part * kDecodeHeads + i;
+  const Elem *k = static_cast<const Elem*>(p.c.k), *v = static_cast<const Elem*>(p.c.v);
+  const int64_t q0 = at.row * p.q_row + h * p.q_head;
+  const float* qf = p.q_dtype == MXMOE_F32 ? static_cast<const float*>(p.q) + q0 : nullptr;
+  const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(p.q) + q0;
+  const float by = p.scale * (p.c.k_scale ? p.c.k_scale[at.kvh] : 1.0f);
+  const float* bias = p.bias ? p.bias + at.row * p.bias_row + h * p.bias_head : nullptr;
+  int slot = -1;  // of this lane's key, -1: none
+  auto score = [&](int j) {
+    const int key = at.lo + (at.tile + j) * kTile + lane;
+    int bad = 0;  // has been reported where the tile was loaded
+    const int64_t s = lane < kTile && key < at.len ? slot_of(p.c, p.t, at.row, key, bad) : -1;
+    slot = s < 0 ? -1 : static_cast<int>(s) + at.kvh * p.c.page_size;
+    if (slot < 0) return -INFINITY;
+    float d[4] = {};
+#pragma unroll 1
+    for (int c = 0; c < hd; c += 4)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        d[e] = fmaf(qf ? qf[c + e] : element(qb, c + e), element(k, static_cast<int64_t>(slot) * hd + c + e), d[e]);
+    const float sum = ((d[0] + d[1]) + (d[2] + d[3])) * by;
+    return bias && key < p.bias_len ? sum + bias[key] : sum;
+  };
+  float m = -INFINITY, l = 0.0f, o[kColumns] = {};
+#pragma unroll 1
+  for (int j = first; j < n; j += step) {
+    const float s = score(j);
+    m = fmaxf(m, s);
+    if (!__any_sync(0xFFFFFFFFu, isnan(s) || s == INFINITY)) continue;
+    // NaN scores, or inf - inf: nothing else can come of the head
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+      if (lane + 32 * c < HDT) out[lane + 32 * c] = NAN;
+    return make_float2(0.0f, NAN);
+  }
+#pragma unroll
+  for (int a = 1; a < 32; a <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, a));
+#pragma unroll 1
+  for (int j = first; j < n; j += step) {
+    const float s = score(j), w = exp_diff(s, m);
+    l += w;
+    if (p.track && x + j < ws.score_tiles && lane < kTile)  // where the tile loop put it
+      ws.scores[((static_cast<int64_t>(x + j) * C::NT + lane / 16) * 32 + 4 * i + lane % 8 / 2) * 4 + lane % 16 / 8 * 2 + lane % 2] = s;
+#pragma unroll 1
+    for (int e = 0; e < kTile; ++e) {
+      const float share = __shfl_sync(0xFFFFFFFFu, w, e);
+      const int64_t from = static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, slot, e)) * hd;
+      if (share == 0.0f) continue;
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c)
+        if (lane + 32 * c < hd) o[c] = fmaf(share, element(v, from + lane + 32 * c), o[c]);
+    }
+  }
+#pragma unroll
+  for (int a = 1; a < 32; a <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, a);
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c)
+    if (lane + 32 * c < HDT) out[lane + 32 * c] = o[c];
+  return make_float2(m, l);
+}
+
 __device__ __forceinline__ void store_lse(const DecodeParams& p, const DecodeScratch& ws, int row, int h, float lse) {
   if (p.lse) p.lse[static_cast<int64_t>(row) * p.c.n_heads + h] = lse;
   if (p.track) ws.lse[row * p.c.n_heads + h] = lse;
@@ -805,7 +887,7 @@ __device__ __forceinline__ void store_out(const DecodeParams& p, int row, int h,
 
 template <class C, int HDT>
 __global__ void __launch_bounds__(32 * C::kWarps, 1)
-    attend_kernel(const DecodeParams p, const DecodeScratch ws, const DecodePlan plan) {
+    attend_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ DecodeScratch ws, const DecodePlan plan) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ int before[kDecodeMaxRows + 1];
   __shared__ int len_of[kDecodeMaxRows];
@@ -1137,6 +1219,37 @@ __global__ void __launch_bounds__(32 * C::kWarps, 1)
         constexpr float kBack = 1.0f / (1 << C::kShareBits);
         l *= kBack;
         o.scale(kBack, kBack);
+      }
+      bool odd[2] = {};  // NaN in a column of head 2t, 2t + 1
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) odd[i & 1] |= isnan(o.pair(i).x) || isnan(o.pair(i).y);
+      const uint32_t evens = __ballot_sync(0xFFFFFFFFu, odd[0]), odds = __ballot_sync(0xFFFFFFFFu, odd[1]), sums = __ballot_sync(0xFFFFFFFFu, isnan(l));
+      if (evens | odds | sums) {
+        float* const out = reinterpret_cast<float*>(mine + ld_stage * kStageBytes);  // [8][HDT] in the free stage
+#pragma unroll 1
+        for (int i = 0; i < min(kDecodeHeads, G - part * kDecodeHeads); ++i) {
+          if (!((i & 1 ? odds : evens) & 0x11111111u << i / 2) && !(sums >> 4 * i & 15)) continue;
+          const float2 ml = plain_head<C, HDT>(p, ws, at, x, n, in_group, wg, i, out + i * HDT);
+          __syncwarp();
+          if (g == i) {
+            m = ml.x;
+            l = ml.y;
+          }
+          if (i / 2 == t) {
+#pragma unroll
+            for (int e = 0; e < HDT / 16; ++e) {
+              const float* from = out + i * HDT + C::column(e, g);
+              if (i & 1) {
+                o.x[e][1] = from[0];
+                o.x[e][3] = from[C::kApart];
+              } else {
+                o.x[e][0] = from[0];
+                o.x[e][2] = from[C::kApart];
+              }
+            }
+          }
+        }
+        __syncwarp();
       }
       x += n;
       if (x < end) at.next_segment(p, rows, parts);

@@ -143,3 +143,54 @@ def test_decode_8_bit_keeps_small_shares(torch, gap, n, hd, every, dtype):
     want, _ = po.decode(q.double().numpy(), k.double().numpy(), v.double().numpy(), tab, np.array([n]), 1.0)
     tol = 448 * every * 2.0 ** -39 + 1e-5 * want + (2.0 ** -8 * want if dtype == "bf16" else 0)
     assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol)
+
+
+def odd_close(got, want, tol):
+    """Alike where NaN or infinite, within tol elsewhere."""
+    fin = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[~fin & ~np.isnan(want)], want[~fin & ~np.isnan(want)])
+    assert np.all(np.abs(got[fin] - want[fin]) <= tol[fin])
+
+
+@pytest.mark.parametrize("cache,q_dtype", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32"), ("e4m3", "bf16"), ("e4m3", "f32")])
+@pytest.mark.parametrize("lens,nH,H,hd", [([40, 100], 8, 2, 64), ([5000, 333], 12, 1, 128), ([70, 1000], 2, 1, 80), ([300, 90], 4, 2, 256)])
+def test_decode_infinite_and_nan_keys_and_values(torch, cache, q_dtype, lens, nH, H, hd):
+    """As the formula has it: a key of score -inf, and what lies at it, does not count; an infinite value with a share
+    gives infinity in its column, both signs give NaN; a NaN value its column; a NaN score the head."""
+    P = Pool(torch, lens, nH, H, hd, 16, cache, track=True)
+    rng = np.random.default_rng(7)
+    q = torch.randn(2, nH, hd, generator=torch.Generator().manual_seed(1)).to(getattr(torch, DT[q_dtype]))
+    bias = np.zeros((2, nH, max(lens)), np.float32)
+    inf, nan = (np.inf, np.nan) if cache != "e4m3" else (np.nan, np.nan)  # e4m3 has no infinities
+    for row, n in enumerate(lens):
+        pg, sl = po.place(P.htab, 16, row, np.arange(n))
+        # values: +inf in column 1, -inf in 2, both in 3, NaN in 5
+        for col, x in ((1, inf), (2, -inf), (3, inf), (3, -inf), (5, nan)):
+            i = rng.integers(n)
+            P.hv[pg[i], H - 1, sl[i], col] = x
+        # masked by the bias: whatever lies there
+        for i in rng.choice(n, 7, replace=False):
+            bias[row, :, i] = -np.inf
+            P.hv[pg[i], :, sl[i]] = rng.choice([inf, -inf, nan], hd)
+    # row 1, first key head: an infinite key, a score of +-inf for each head by its query's sign
+    if cache != "e4m3":
+        pg, sl = po.place(P.htab, 16, 1, 11)
+        bias[1, :, 11] = 0
+        P.hv[pg, 0, sl] = 1.0
+        P.hk[pg, 0, sl, 2] = inf
+    P.k.copy_(torch.from_numpy(P.hk).to(P.k.dtype))
+    P.v.copy_(torch.from_numpy(P.hv).to(P.v.dtype))
+    used = P.hw.copy()
+    lse = torch.empty(2, nH, device="cuda")
+    out = P.cache.decode(q.cuda(), P.tables, P.lens, bias=torch.from_numpy(bias).cuda(), track=True, lse=lse)
+    P.cache.sync_status()
+    w = P.hw.astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        want, want_lse = po.decode(q.double().numpy(), P.hk, P.hv, P.htab, P.hlens, 1 / np.sqrt(hd), bias=bias, weight=w,
+                                   k_scale=P.hks, v_scale=P.hvs)
+    assert np.isfinite(want).any() and not np.isfinite(want).all()
+    tol = 2 * ATOL + (2.0 ** -8 if q_dtype == "bf16" else 2.0 ** -24) * np.abs(want)
+    odd_close(out.double().cpu().numpy(), want, tol)
+    odd_close(lse.cpu().numpy(), want_lse, 2 * ATOL + 2e-6 * np.abs(want_lse))
+    odd_close(P.weight.cpu().numpy(), w, 2e-5 * (w - used) + 2.0 ** -23 * np.abs(w))
