@@ -194,3 +194,99 @@ def test_decode_infinite_and_nan_keys_and_values(torch, cache, q_dtype, lens, nH
     odd_close(out.double().cpu().numpy(), want, tol)
     odd_close(lse.cpu().numpy(), want_lse, 2 * ATOL + 2e-6 * np.abs(want_lse))
     odd_close(P.weight.cpu().numpy(), w, 2e-5 * (w - used) + 2.0 ** -23 * np.abs(w))
+
+
+TYPES = [("bf16", "bf16"), ("bf16", "f32"), ("e4m3", "bf16"), ("e4m3", "f32"), ("f32", "f32")]
+
+
+@pytest.mark.parametrize("cache,q_dtype,nH,H,hd,longest", [(*t, 8, 4, 16, 12000) for t in TYPES]
+                         + [("bf16", "bf16", 18, 2, 16, 12000), ("e4m3", "f32", 18, 2, 16, 12000), ("bf16", "bf16", 4, 4, 128, 6000),
+                            ("e4m3", "bf16", 4, 4, 128, 6000), ("f32", "f32", 2, 2, 256, 6000)])
+def test_decode_ranges_kept_back(torch, cache, q_dtype, nH, H, hd, longest):
+    """More than eight tiles a warp (148 SMs of 8 warps at most, tiles of 16 or 32 keys): a quarter of the list goes to
+    whoever is done, the counters are set back at the end, by calls of every size in turn."""
+    rng = np.random.default_rng(2)
+    lens = [int(x) for x in rng.integers(1, longest, 26)] + [0, 1, 40000, 31, 32, 33]
+    tile = 16 if hd == 256 else 32
+    assert sum(-(-n // tile) for n in lens) * H * -(-nH // H // 8) >= 8 * 8 * 148
+    P, out = check_decode(torch, lens, nH, H, hd, 16, cache, q_dtype, sinks=True)
+    q = torch.randn(len(lens), nH, hd, device="cuda").to(getattr(torch, DT[q_dtype]))
+    few = P.cache.decode(q[:3], P.tables[:3], P.lens[:3])
+    want = P.cache.decode(q, P.tables, P.lens)
+    for _ in range(5):
+        assert torch.equal(P.cache.decode(q[:3], P.tables[:3], P.lens[:3]), few)
+        assert torch.equal(P.cache.decode(q, P.tables, P.lens), want)
+
+
+@pytest.mark.parametrize("cache,q_dtype", [("bf16", "bf16"), ("e4m3", "f32"), ("f32", "f32")])
+def test_decode_track_with_ranges_kept_back(torch, cache, q_dtype):
+    rng = np.random.default_rng(5)
+    lens = [int(x) for x in rng.integers(1, 12000, 28)] + [0, 20000, 1]
+    check_decode(torch, lens, 8, 4, 16, 16, cache, q_dtype, sinks=True, track=True)
+
+
+@pytest.mark.parametrize("rows,longest", [(513, 200), (1100, 200), (513, 1200), (1100, 1200)])
+@pytest.mark.parametrize("cache,q_dtype", [("bf16", "bf16"), ("f32", "f32"), ("e4m3", "f32")])
+@pytest.mark.parametrize("track", [False, True])
+def test_decode_rows_of_several_launches(torch, rows, longest, cache, q_dtype, track):
+    """More than 512 rows: whole segments under a table of 200 tokens, cut ones (kept back among them) under one of 1200;
+    bias and lse by row, weights of one launch while the next begins."""
+    rng = np.random.default_rng(rows)
+    lens = [int(x) for x in rng.integers(0, longest + 1, rows)]
+    lens[0] = lens[511] = lens[-1] = 0
+    lens[512] = longest
+    bias = rng.standard_normal((rows, 1, longest // 2)).astype(np.float32)
+    check_decode(torch, lens, 6, 3, 16, 8, cache, q_dtype, sinks=True, bias=bias, track=track)
+
+
+def test_decode_rows_of_several_launches_by_strides(torch):
+    rows = 700
+    lens = [(37 * i) % 300 for i in range(rows)]
+    P = Pool(torch, lens, 4, 2, 32, 8)
+    q = torch.randn(rows, 4, 32, device="cuda").bfloat16()
+    lse, out_lse = torch.empty(rows, 4, device="cuda"), torch.empty(rows, 4, device="cuda")
+    want = P.cache.decode(q, P.tables, P.lens, lse=lse)
+    wide = torch.zeros(4, rows, 40, device="cuda").bfloat16()
+    wide[:, :, 4:36] = q.transpose(0, 1)
+    room = torch.zeros(4, rows, 48, device="cuda").bfloat16()
+    tables = torch.zeros(rows, P.tables.shape[1] + 3, dtype=torch.int32, device="cuda")
+    tables[:, : P.tables.shape[1]] = P.tables
+    P.cache.decode(wide.transpose(0, 1)[..., 4:36], tables[:, : P.tables.shape[1]], P.lens,
+                   out=room.transpose(0, 1)[..., 8:40], lse=out_lse)
+    assert torch.equal(room.transpose(0, 1)[..., 8:40], want) and torch.equal(out_lse, lse)
+    assert torch.count_nonzero(room) == torch.count_nonzero(want)
+
+
+@pytest.mark.parametrize("cache,q_dtype,out_dtype", [("bf16", "bf16", "f32"), ("bf16", "f32", "bf16"), ("e4m3", "bf16", "f32"),
+                                                     ("e4m3", "f32", "bf16"), ("f32", "bf16", "f32"), ("f32", "bf16", "bf16"),
+                                                     ("f32", "f32", "bf16")])
+@pytest.mark.parametrize("nH,H,hd", [(8, 2, 64), (9, 1, 128), (6, 2, 256)])
+def test_decode_output_types(torch, cache, q_dtype, out_dtype, nH, H, hd):
+    check_decode(torch, [0, 1, 17, 300, 5000], nH, H, hd, 16, cache, q_dtype, out_dtype, sinks=True)
+
+
+@pytest.mark.parametrize("cache,q_dtype", TYPES + [("f32", "bf16")])
+@pytest.mark.parametrize("shape", [(3, 16, 3000), (1, 1, 40)])
+def test_decode_bias_by_type(torch, cache, q_dtype, shape):
+    bias = np.random.default_rng(1).standard_normal(shape).astype(np.float32)
+    check_decode(torch, [3000, 39, 41], 16, 2, 64, 16, cache, q_dtype, bias=bias)
+
+
+@pytest.mark.parametrize("cache,q_dtype", TYPES + [("f32", "bf16")])
+@pytest.mark.parametrize("window", [1, 17, 300])
+def test_decode_window_by_type(torch, cache, q_dtype, window):
+    check_decode(torch, [1, 16, 129, 7000, 0], 16, 2, 64, 24, cache, q_dtype, window=window, sinks=True)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("hd,rot", [(64, 64), (80, 20), (7, 6)])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rotary_bf16(torch, interleaved, hd, rot, inverse):
+    """The turn and its gradient in bf16: one rounding of the 32-bit result."""
+    x = torch.randn(300, 5, hd, generator=torch.Generator().manual_seed(4)).bfloat16()
+    pos = (np.arange(300) * 13 % 1000).astype(np.int32)
+    inv, f = po.frequencies(rot, scaling="yarn", factor=8.0)
+    want = po.rotate(x.double().numpy(), pos, inv, f, interleaved, inverse=inverse)
+    r = table(torch, rot, 1000, interleaved, scaling="yarn", scaling_factor=8.0)
+    got = r.apply(x.cuda(), torch.from_numpy(pos).cuda(), inverse=inverse)
+    assert np.all(np.abs(got.double().cpu().numpy() - want) <= 6e-6 + (2.0 ** -8 + 2.0 ** -20) * np.abs(want))
