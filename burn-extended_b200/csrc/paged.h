@@ -103,6 +103,10 @@ int decode_tile(const PagedView& c);                     // keys of a tile
 // Rows of one launch, whose tiles are numbered in 32 bits; 0: not even one under a table that wide.
 int decode_rows_at_once(const PagedView& c, int max_pages);
 size_t decode_part_floats(const PagedView& c, int sms);  // of DecodeScratch::part
+inline bool apart(const int32_t* a, const int32_t* b, int64_t n) {  // two arrays of n
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b), bytes = static_cast<uintptr_t>(n) * 4;
+  return x + bytes <= y || y + bytes <= x;
+}
 cudaError_t launch_paged_evict(const EvictParams& p, int sms, cudaStream_t st);
 cudaError_t launch_rotary_table(const double* inv_freq, int half, int64_t first, int n, double factor, float* cos,
                                 float* sin, cudaStream_t st);

@@ -368,6 +368,7 @@ int mxmqa_paged_evict(mxmqa_paged_cache* c, const mxmqa_paged_evict_args* a, voi
   P_CHECK(a->lens && a->seen && a->new_lens, "null lens, seen or new_lens");
   P_CHECK(aligned(a->lens, 4) && aligned(a->seen, 4) && aligned(a->new_lens, 4),
           "lens, seen and new_lens must be 4-byte aligned");
+  P_CHECK(a->new_lens == a->lens || mxmoe::apart(a->new_lens, a->lens, a->rows), "new_lens may be lens, but not overlap a part of it");
   P_CHECK(c->view.weight && c->view.position, "evict needs a cache with weight and position buffers");
   P_CHECK(a->budget > 0 && a->budget <= kMaxTokens, "budget must be 1 to 2^31 - 1");
   P_CHECK(static_cast<uint64_t>(a->sink) + a->recent <= a->budget, "sink + recent above the budget");

@@ -459,7 +459,8 @@ __global__ void __launch_bounds__(kLongThreads) evict_long_kernel(const EvictPar
   }
 }
 
-// New lengths in the place of the old ones, once every block has read those.
+// New lengths in the place of the old ones or of `seen`, once every block has
+// read those.
 __global__ void lens_kernel(const EvictParams p, int32_t* lens) {
   griddep_wait();
   griddep_launch_dependents();
@@ -512,7 +513,7 @@ cudaError_t launch_select(const EvictParams& p, int sms, cudaStream_t st) {
 
 cudaError_t launch_paged_evict(const EvictParams& p, int sms, cudaStream_t st) {
   EvictParams q = p;
-  const bool over = p.new_lens < p.lens + p.rows && p.lens < p.new_lens + p.rows;
+  const bool over = !apart(p.new_lens, p.lens, p.rows) || !apart(p.new_lens, p.seen, p.rows);
   if (over) q.new_lens = nullptr;
   const cudaError_t e = launch_select(q, sms, st);
   if (e != cudaSuccess || !over) return e;

@@ -728,7 +728,7 @@ typedef struct mxmqa_paged_evict_args {
   uint32_t max_pages;
   const int32_t* lens;   /* [rows] cached tokens */
   const int32_t* seen;   /* [rows] tokens of the sequence so far: one above its newest position */
-  int32_t* new_lens;     /* [rows] min(lens, budget); may be lens */
+  int32_t* new_lens;     /* [rows] min(lens, budget); may be lens, else apart from it */
   uint32_t budget;       /* tokens that stay */
   uint32_t sink;         /* positions below this stay */
   uint32_t recent;       /* positions from seen - recent on stay; sink + recent <= budget */

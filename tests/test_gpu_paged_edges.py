@@ -290,3 +290,16 @@ def test_rotary_bf16(torch, interleaved, hd, rot, inverse):
     r = table(torch, rot, 1000, interleaved, scaling="yarn", scaling_factor=8.0)
     got = r.apply(x.cuda(), torch.from_numpy(pos).cuda(), inverse=inverse)
     assert np.all(np.abs(got.double().cpu().numpy() - want) <= 6e-6 + (2.0 ** -8 + 2.0 ** -20) * np.abs(want))
+
+
+@pytest.mark.parametrize("over", ["lens", "seen", "askew"])
+def test_evict_writes_lengths_over_others(torch, over):
+    """Into lens, where it is seen too; into seen; over seen by one element."""
+    lens = [700, 90, 3000, 40, 1500]
+    P, R = (Pool(torch, lens, 8, 4, 32, 16, track=True) for _ in range(2))
+    want = R.cache.evict(R.tables, R.lens, R.lens, 300, 4, 50)
+    room = torch.cat([P.lens, P.lens])
+    seen, new = {"lens": (P.lens, P.lens), "seen": (room[:5], room[:5]), "askew": (room[:5], room[1:6])}[over]
+    got = P.cache.evict(P.tables, P.lens, seen, 300, 4, 50, new_lens=new)
+    P.cache.sync_status()
+    assert torch.equal(got, want) and torch.equal(P.position, R.position) and torch.equal(P.weight, R.weight)

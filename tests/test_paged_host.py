@@ -109,3 +109,25 @@ for heads, hd, rot in ((65535, 65536, 65536), (65535, 65536, 0), (32768, 65536, 
         assert rc == 0 and fake.fake_launches() == n + 1, (heads, hd, rot)
 assert turn(32769, 65535, 0) == 5 and turn(32767, 65536, 0) == 0
 """)
+
+
+def test_evict_writes_lengths_over_others_last(fake):
+    """new_lens may be lens or lie over seen: a launch of its own writes it after the one that reads those.  Askew over
+    lens it would be read and written by that launch: refused."""
+    run(fake, """
+h = create(weight=P, position=P)
+
+def evict(new, lens=P + 64, seen=P + 128, rows=8):
+    a = _lib.PagedEvictArgs(P, 4, rows, 4, lens, seen, new, 8, 0, 0)
+    n = fake.fake_launches()
+    rc = L.mxmqa_paged_evict(h, ctypes.byref(a), None)
+    return (rc, fake.fake_launches() - n)
+
+for new in (P + 68, P + 36, P + 92):
+    assert evict(new) == (1, 0) and "new_lens" in _lib.last_error(), new - P
+for new in (P + 32, P + 96, P + 160):
+    assert evict(new) == (0, 1), _lib.last_error()
+for new in (P + 64, P + 100, P + 128, P + 132, P + 156):
+    assert evict(new) == (0, 2), (new - P, _lib.last_error())
+assert evict(P + 64, seen=P + 64) == (0, 2)
+""")
