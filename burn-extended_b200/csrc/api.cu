@@ -28,7 +28,7 @@ using namespace mxmoe;
 
 namespace {
 
-thread_local std::string g_last_error;
+thread_local char g_last_error[1024];  // reporting an error allocates nothing
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -36,7 +36,7 @@ int fail(int code, const char* fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
-  g_last_error = buf;
+  std::snprintf(g_last_error, sizeof(g_last_error), "%s", buf);
   return code;
 }
 
@@ -46,7 +46,7 @@ namespace mxmoe {
 // Lets the other translation units of the library (the model.bin reader)
 // report through mxmoe_last_error().
 int set_last_error(int code, const char* msg) {
-  g_last_error = msg;
+  std::snprintf(g_last_error, sizeof(g_last_error), "%s", msg);
   return code;
 }
 }  // namespace mxmoe
@@ -858,7 +858,7 @@ const char* mxmoe_build_info(void) {
 
 int mxmoe_last_error(char* buf, size_t cap) {
   if (!buf || cap == 0) return MXMOE_ERR_INVALID_ARG;
-  std::snprintf(buf, cap, "%s", g_last_error.c_str());
+  std::snprintf(buf, cap, "%s", g_last_error);
   return MXMOE_OK;
 }
 

@@ -16,12 +16,16 @@ inline cudaError_t ensure_dynamic_smem(const void* func, size_t bytes) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lock(mu);
-  size_t& g = granted[{func, dev}];
-  if (bytes <= g) return cudaSuccess;
-  e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-  if (e == cudaSuccess) g = bytes;
-  return e;
+  try {  // the map allocates, and its callers are C entry points
+    std::lock_guard<std::mutex> lock(mu);
+    size_t& g = granted[{func, dev}];
+    if (bytes <= g) return cudaSuccess;
+    e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess) g = bytes;
+    return e;
+  } catch (...) {
+    return cudaErrorMemoryAllocation;
+  }
 }
 
 // Programmatic dependent launch for the kernels of one forward chain: with

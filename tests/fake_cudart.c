@@ -1,5 +1,7 @@
+#define _GNU_SOURCE
 /* A CUDA runtime without a device, preloaded before the library to test its host side: what runs on a
  * stream is only counted, memory comes from the host's heap, and nothing is ever launched. */
+#include <dlfcn.h>
 #include <stddef.h>
 #include <stdlib.h>
 #include <string.h>
@@ -15,6 +17,13 @@ int fake_pending(void) {
   return n;
 }
 int fake_launches(void) { return launches; }
+
+static int no_memory;
+void fake_no_memory(int on) { no_memory = on; }
+void* _Znwm(size_t n) { /* operator new */
+  if (no_memory) ((void (*)(void))dlsym(dlopen("libstdc++.so.6", RTLD_LAZY), "_ZSt17__throw_bad_allocv"))();
+  return malloc(n);
+}
 
 int cudaGetDevice(int* d) { return *d = 0; }
 int cudaSetDevice(int d) { return d ? 101 : 0; }

@@ -29,7 +29,7 @@ def create(n_pages=4, page=16, heads=8, kv_heads=2, hd=64, dtype=1, weight=None,
 @pytest.fixture(scope="module")
 def fake(tmp_path_factory):
     out = str(tmp_path_factory.mktemp("fake") / "libfake_cudart.so")
-    subprocess.run(["gcc", "-shared", "-fPIC", "-O1", "-w", os.path.join(HERE, "fake_cudart.c"), "-o", out], check=True)
+    subprocess.run(["gcc", "-shared", "-fPIC", "-O1", "-w", "-fexceptions", os.path.join(HERE, "fake_cudart.c"), "-o", out, "-ldl"], check=True)
     return out
 
 
@@ -130,4 +130,20 @@ for new in (P + 32, P + 96, P + 160):
 for new in (P + 64, P + 100, P + 128, P + 132, P + 156):
     assert evict(new) == (0, 2), (new - P, _lib.last_error())
 assert evict(P + 64, seen=P + 64) == (0, 2)
+""")
+
+
+def test_no_exception_leaves_an_entry_point(fake):
+    """Where the host has no memory left, create and a kernel's first launch return an error."""
+    run(fake, DECODE + """
+h, dead = create(weight=P, position=P), ctypes.c_void_p()
+fake.fake_no_memory(1)
+rc = L.mxmqa_paged_create(ctypes.byref(_lib.PagedConfig(4, 16, 8, 2, 64, 1, 0)),
+                          ctypes.byref(_lib.PagedBuffers(P, P, None, None, None, None)), ctypes.byref(dead))
+assert rc == 4 and not dead.value
+assert decode(h) == 3
+a = _lib.PagedEvictArgs(P, 0, 1, 4, P, P, P + 64, 8, 0, 0)
+assert L.mxmqa_paged_evict(h, ctypes.byref(a), None) == 3
+fake.fake_no_memory(0)
+assert decode(h) == 0 and L.mxmqa_paged_evict(h, ctypes.byref(a), None) == 0
 """)
