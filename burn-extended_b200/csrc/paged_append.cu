@@ -53,13 +53,14 @@ __device__ __forceinline__ Token token_of(const AppendParams& p, int t) {
   const int64_t from = on_table ? static_cast<int64_t>(k.pos) * half : 0;  // unread without a rotation
   k.cs = p.cos + from;
   k.sn = p.sin + from;
-  if (p.k && index >= 0 && on_table) {
+  if (p.k && index >= 0) {  // looked up while the position comes
     const int row = p.rows ? __ldg(p.rows + t) : t;
     if (row < 0 || row >= p.t.n_rows)
       atomicOr(p.c.status, kPagedBadIndex);
     else
       k.slot = slot_of(p.c, p.t, row, index);
   }
+  if (!on_table) k.slot = -1;
   return k;
 }
 

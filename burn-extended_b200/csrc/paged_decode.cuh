@@ -724,7 +724,7 @@ __device__ __forceinline__ float element(const __nv_fp8_e4m3* p, int64_t i) { re
 // and sum are returned.  64 rows of 8192 tokens with a NaN in one query head of
 // each row take as long as without; with all queries NaN 0.5 ms against 0.2.
 template <class C, int HDT>
-static __device__ __noinline__ float2 plain_head(const DecodeParams& p, const DecodeScratch& ws, const Place& at, int x, int n,
+static __device__ __noinline__ float2 plain_head(const DecodeParams& p, const DecodeScratch& ws, Place at, int x, int n,
                                                  int first, int step, int i, float* out) {
   using Elem = typename C::Elem;
   constexpr int kTile = 16 * C::NT, kColumns = (HDT + 31) / 32;
