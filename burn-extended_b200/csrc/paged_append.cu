@@ -287,10 +287,10 @@ __global__ void __launch_bounds__(512, 1) append_wide_kernel(const AppendParams 
 
 // Many tokens: a block goes from one to the next, and looks the places of its
 // next kAtOnce up together, so that index, page table and position cost their
-// latency once for all of them.  8192 tokens of 64 + 8 heads of 64 in bf16: 33.3
-// us, 5.1 TB/s; 37.9 us with a block per token.  Five blocks an SM leave enough
-// registers for the pieces in flight; with four 34.7 us, six 33.7, seven 34.8,
-// and with three query heads in flight 36.1.
+// latency once for all of them.  8192 tokens of 64 + 8 heads of 64 in bf16: 32.3
+// us, 5.3 TB/s; 44.1 us with a block per token.  Five blocks an SM leave enough
+// registers for the pieces in flight; with four 34.6 us, six 36.1, seven 36.2,
+// and with three query heads in flight 34.4.
 template <typename T, bool kInterleaved>
 __global__ void __launch_bounds__(128, kManyBlocks) append_many_kernel(const AppendParams p, int units, int per_pass) {
   __shared__ Token places[kAtOnce];
@@ -390,7 +390,7 @@ cudaError_t launch_append(const AppendParams& p, int sms, cudaStream_t st) {
   if (!aligned || units > 512) return launch_kernel(append_kernel<T>, dim3(p.tokens), dim3(256), 0, st, p);
   // Threads of a token: enough of them to fill the SMs (2048 a SM), up to a
   // thread per unit for the shortest chain.  1023 tokens of 32 + 8 heads of 128 in
-  // 32 bits into 8: 12.1 us with 288 threads, 13.7 with 224, 15.5 with 128.
+  // 32 bits into 8: 12.9 us with 256 threads, 14.5 with 224, 16.3 with 128.
   const int heads = p.q ? p.c.n_heads : p.c.kv_heads;
   const int want = std::max(units, std::min(512, std::max(128, sms * 2048 / p.tokens / 32 * 32)));
   const int passes = (heads * units + want - 1) / want, per_pass = std::min(want / units, (heads + passes - 1) / passes);

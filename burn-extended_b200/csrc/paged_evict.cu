@@ -108,11 +108,14 @@ __device__ __forceinline__ void over_warps(int2 x, int2* sums, int2& before, int
 // holes and movers of a stretch of slots by ballots; every hole and mover is
 // written to the list of the block that will move it, and the blocks move their
 // pairs in 16-byte pieces.  Bound by the latency of these steps where few
-// tokens move (one of 2049, 8 key heads: 7.6 us, the launch alone 2.5), else by
-// the rows moved and how many SMs move them (16 rows of 1000 to 8192 tokens to
-// 2048, 8 key heads of 64 in bf16: 17 us, 67 MB, 3.9 TB/s; 2 rows of 60001 and
-// 65536 to 16384, 8-bit heads of 128: 30 us on 96 SMs, 110 MB, 3.7 TB/s).  The
-// moves as a launch of their own were slower: 24 and 41 us.
+// tokens move (one of 2049, 8 key heads: 7.5 us, the launch alone 2.5), else by
+// the selection's instructions first (some 400 warp instructions to 32 keys,
+// issued 46% of the time) and then by the moves.  The first eviction of 16 rows
+// of 1000 to 8192 tokens to 2048, 8 key heads of 64 in bf16, reads and writes 70
+// MB in 32 us, 2.2 TB/s; of 2 rows of 60001 and 65536 to 16384, 8-bit heads of
+// 128, 112 MB in 50 us on 96 SMs, 2.2 TB/s.  The same calls again, on caches
+// where the survivors behind the budget are copies and only 18 and 17 MB move,
+// take 17 and 30 us.
 __global__ void __launch_bounds__(kThreads, 1) evict_kernel(const EvictParams p, int slots, int four) {
   extern __shared__ __align__(16) uint32_t keys[];  // [slots]; then to[slots / 2 + 1], by[slots / 2 + 1]
   __shared__ __align__(16) int hist[3][kBins];
@@ -348,11 +351,13 @@ __device__ __forceinline__ int block_rank(bool flag, int* warp_sums, int& total)
   return before + __popc(b & ((1u << lane) - 1));
 }
 
-// For tables too long for the kernel above (8 x 24K slots); simple, as nobody
-// waits for it each step.  One block per (key head, row): a
-// radix selection of the last victim's key, the keys read anew in each pass,
-// then one walk over the slots below the budget and one over those above it,
-// which hand each other holes and movers through shared memory.
+// For tables too wide for the kernel above (8 x 24K slots), whatever their rows
+// hold.  Simple, and slow: one of 2049 tokens under 262144 slots takes 38 us, 7.5
+// under a table of its size; 2 rows of 60001 and 65536 to 16384 770 us, 50 there.
+// One block per (key head, row): a radix selection of the last victim's key, the
+// keys read anew in each pass, then one walk over the slots below the budget and
+// one over those above it, which hand each other holes and movers through shared
+// memory.
 __global__ void __launch_bounds__(kLongThreads) evict_long_kernel(const EvictParams p) {
   griddep_wait();
   griddep_launch_dependents();
@@ -474,11 +479,18 @@ __global__ void lens_kernel(const EvictParams p, int32_t* lens) {
 cudaError_t launch_select(const EvictParams& p, int sms, cudaStream_t st) {
   // Blocks of a (row, key head): as many as its keys and lists (8 bytes a slot)
   // need.  Rows of more than 8192 slots that leave SMs idle get up to kSpread, of
-  // at least 4096 slots each: 12000 slots of 8 heads 16.2 us with three blocks,
-  // 18.4 with two, 21.8 with one; below that a cluster's barriers cost more than
-  // the shorter share saves (4500 slots 9.4 us alone, 10.4 as two).  Clusters of
-  // seven and eight blocks do not all find room at once (16 of them 55 us
-  // against 30 with six).
+  // at least 4096 slots each.  One row of 8 heads, one token over the budget: 12000
+  // slots 11.5 us with three blocks, 13.6 with one; 8000 slots 11.0 with one, 11.1
+  // with two; 4500 slots 9.2 and 10.3, where a cluster's barriers cost more than
+  // the shorter share saves.  First evictions of many, between two events, 5 us of
+  // which are theirs: half of 12000 slots 29 and 47, of 8000 35 and 29, of 4500 27
+  // and 25, so for those the limit could be lower; 2 rows of 65536 slots, 16
+  // clusters, 56 with six blocks each, 66 with four, 98 with three, and with
+  // eight, which do not all find room at once, 84; the 24 clusters of 3 rows do
+  // not with six either: 104, with four 74.  All of this goes by the table's width,
+  // as the lengths are not known here: under a table much wider than its rows a
+  // call is slower (16 rows of up to 8192 tokens 32 us under a table of 8192
+  // slots, 85 under one of 131072).
   constexpr int kSlots = 24 * 1024, kSpread = 6;
   const int64_t cap = static_cast<int64_t>(p.t.max_pages) * p.c.page_size, pairs = static_cast<int64_t>(p.rows) * p.c.kv_heads;
   const int64_t need = (cap + kSlots - 1) / kSlots;

@@ -131,7 +131,8 @@ class PagedKvCache:
     dtype: torch.float32, torch.bfloat16 or torch.float8_e4m3fn; an 8-bit key
     stands for its code times k_scale[kv_head], a value for v_scale's.  track:
     the cache also keeps every token's accumulated attention weight and position
-    [n_pages, kv_heads, page_size], which `evict` goes by."""
+    [n_pages, kv_heads, page_size], which `evict` goes by, and a workspace of 32 bytes for every token, key head and
+    8 query heads that read it."""
 
     def __init__(self, n_pages: int, page_size: int, n_heads: int, kv_heads: int, head_dim: int,
                  dtype=torch.bfloat16, track: bool = False, k_scale=None, v_scale=None, device: int = 0):
@@ -197,7 +198,8 @@ class PagedKvCache:
         written at cache index `index` [tokens] int32 of table row `rows` [tokens] (None: token t is row t).  A
         negative index is turned but not written.  positions: None for the cache indexes.  Returns the turned
         queries (q_out, which may be q; None where q is None); k_out gets the turned keys too.  A written slot's
-        weight becomes 0, its position the token's."""
+        weight becomes 0, its position the token's.  A position outside the rotary table keeps its token out of the
+        cache; its outputs are turned as position 0."""
         n, dev, hd, dtype = k.shape[0], self.device, self.head_dim, k.dtype
         q_shape, k_shape = (n, self.n_heads, hd), (n, self.kv_heads, hd)
         ks, vs = _heads("k", k, k_shape, dev), _heads("v", v, k_shape, dev)
@@ -283,7 +285,7 @@ class PagedKvCache:
         head its own; positions below `sink` and from seen[row] - recent on stay (seen: tokens of the sequence so
         far, one above its newest position).  Survivors at cache indexes from the budget on move into the places
         below it; the row's later pages are free after that.  Returns min(lens, budget) (new_lens, which may be
-        lens)."""
+        lens, but not overlap a part of it)."""
         dev = self.device
         t, stride, n, max_pages = self._tables(tables)
         if new_lens is None:

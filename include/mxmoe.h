@@ -622,7 +622,8 @@ MXMOE_API int mxmqa_forward_streaming(mxmqa_layer* layer, mxmqa_cache* cache, co
  * asynchronous and may be captured in a CUDA graph (they allocate nothing); a
  * cache serves one stream at a time, as a layer does.  A table entry, index,
  * length or position out of range is skipped on the device and reported by
- * mxmqa_paged_status. */
+ * mxmqa_paged_status.  A row's cache indexes are numbered in 32 bits:
+ * max_pages x page_size is at most 2^31 - 1024. */
 typedef struct mxmqa_paged_config {
   uint32_t n_pages;
   uint32_t page_size;  /* tokens per page, any size up to 65536 */
@@ -644,7 +645,10 @@ typedef struct mxmqa_paged_buffers {
 
 typedef struct mxmqa_paged_cache mxmqa_paged_cache;
 
-/* The buffers must outlive the handle; their contents are left as they are. */
+/* The buffers must outlive the handle; their contents are left as they are.
+ * Allocates the workspace of all calls: 15 to 30 MB, and with a weight buffer 32
+ * bytes per token of the pool, key head and 8 query heads.  The cache may be
+ * used on any stream once this has returned. */
 MXMOE_API int mxmqa_paged_create(const mxmqa_paged_config* cfg, const mxmqa_paged_buffers* buffers,
                                  mxmqa_paged_cache** out);
 MXMOE_API int mxmqa_paged_destroy(mxmqa_paged_cache* cache);
@@ -759,7 +763,8 @@ typedef struct mxmqa_rotary_config {
   float ntk_beta;
 } mxmqa_rotary_config;
 
-/* cos, sin: device [n][rot_dim / 2] for positions first .. first + n - 1. */
+/* cos, sin: device [n][rot_dim / 2] for positions first .. first + n - 1.  Allocates
+ * for a moment and waits for the stream. */
 MXMOE_API int mxmqa_rotary_table(const mxmqa_rotary_config* cfg, uint32_t first, uint32_t n, float* cos,
                                  float* sin, int32_t device, void* stream);
 
@@ -786,7 +791,8 @@ typedef struct mxmqa_rotary_args {
   int32_t device;
 } mxmqa_rotary_args;
 
-/* A position outside the table turns as position 0. */
+/* A position outside the table turns as position 0.
+ * heads x (head_dim - rot_dim / 2) must be below 2^31 - 256. */
 MXMOE_API int mxmqa_rotary(const mxmqa_rotary_args* args, void* stream);
 
 #ifdef __cplusplus
